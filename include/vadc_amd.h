@@ -311,6 +311,75 @@ int  vadc_amd_get_kernel_time(vadc_amd_engine *e, int kernel, int *launches, dou
 int  vadc_amd_reset_kernel_times(vadc_amd_engine *e);
 const char *vadc_amd_kernel_name(int kernel);
 
+/* ---- operators on device tensors -------------------------------------------------------------- */
+/* What a streaming layer of the caller's own is made of, beside the models above and in their manner (the pointwise convolutions with bias, residual and activation; the
+ * recurrence whose state stays on the device from call to call; the normalisation): three operators of any size, on device tensors of the caller, without an engine.
+ *   - a call enqueues kernels on `hip_stream` (a hipStream_t; NULL = HIP's default stream) of device `device` (< 0: the current one) and returns: no allocation, no host
+ *     synchronisation, nothing kept for the next call.  It may be issued while the stream is being captured.  The calling thread's current device is the same afterwards.
+ *   - strides count ELEMENTS; the innermost dimension of every tensor is contiguous.  Tensors need their element's alignment, no more (16-byte aligned ones run faster).
+ *   - x, weights and outputs are of ONE type (`dtype`); sums, statistics and states are float32; an output is rounded once, to nearest even.
+ *   - an output must not overlap another operand, but for the exceptions named; entries of an output must be distinct (no stride 0).
+ *   - a call with a dimension of zero that leaves nothing to write returns VADC_AMD_OK and touches nothing.
+ *   - forward only: the operators have no gradients.
+ * VADC_AMD_EINVAL: an argument out of range (checked before the device is touched); VADC_AMD_ENODEVICE: no gfx950 device; VADC_AMD_EHIP: the launch failed. */
+enum { VADC_AMD_F32 = 0, VADC_AMD_F16 = 1, VADC_AMD_BF16 = 2 };
+enum { VADC_AMD_ACT_NONE = 0, VADC_AMD_ACT_RELU = 1, VADC_AMD_ACT_SILU = 2, VADC_AMD_ACT_GELU = 3 /* y/2 (1 + erf(y / sqrt 2)) */, VADC_AMD_ACT_SIGMOID = 4 };
+
+/* out[row][n] = act(sum_k x[row][k] weight[n][k] + bias[n]) + residual[row][n];  residual_first: the residual is added in front of the activation.
+ * bias, residual: NULL = none.  `out` may be the residual's own memory (same stride). */
+typedef struct vadc_amd_linear_args {
+   const void *x, *weight, *bias, *residual;
+   void *out;
+   int64_t rows, in_features, out_features;
+   int64_t x_stride, weight_stride, residual_stride, out_stride;      /* from row to row */
+   int32_t dtype, activation, residual_first, device;
+} vadc_amd_linear_args;
+int  vadc_amd_linear(const vadc_amd_linear_args *args, void *hip_stream);
+
+/* x [sequences][positions][channels], channels last.  Per sequence and group of channels / groups consecutive channels: mean and variance (biased) over the positions and the
+ * group's channels; y = (x - mean) / sqrt(variance + eps) weight[c] + bias[c]; out = act(y), or y act(gate) where a gate is given.  positions = 1: a norm per token and head.
+ * weight, bias [channels], gate [sequences][positions][channels], lengths [sequences]: NULL = none.  With lengths (int32, on the device), sequence n has its first lengths[n]
+ * positions only (clamped to 0 ... positions): the rows behind them are neither read nor written.  `out` may be x's or gate's own memory (same strides).
+ * workspace: device memory of vadc_amd_group_norm_workspace() bytes (a function of the sizes alone; 0: none needed), 16-byte aligned, for this call alone until it is complete. */
+typedef struct vadc_amd_group_norm_args {
+   const void *x, *weight, *bias, *gate;
+   void *out;
+   const int32_t *lengths;
+   void *workspace;
+   int64_t workspace_bytes;
+   int64_t sequences, positions, channels, groups;
+   int64_t x_stride[2], gate_stride[2], out_stride[2];                /* from sequence to sequence, from position to position */
+   int32_t dtype, activation, device;
+   float eps;
+} vadc_amd_group_norm_args;
+int64_t vadc_amd_group_norm_workspace(const vadc_amd_group_norm_args *args);   /* bytes, or a negative VADC_AMD_E* code */
+int  vadc_amd_group_norm(const vadc_amd_group_norm_args *args, void *hip_stream);
+
+/* The gated delta rule: per stream and head a state S [key_dim][value_dim] (float32, updated in place), and for each step t
+ *     S = e^log_decay[t] S;   u = beta[t] (v[t] - S^T k[t]);   S = S + k[t] u^T;   out[t] = scale S^T q[t]
+ * q, k [streams][steps][key_heads][key_dim], v, out [streams][steps][heads][value_dim], log_decay, beta [streams][steps][heads] (float32), state [streams][heads][key_dim][value_dim]
+ * (each stream's part contiguous).  heads is a multiple of key_heads: head h reads key head h / (heads / key_heads).  1 <= key_dim <= 256.  normalize: q and k are divided by
+ * sqrt(sum of squares + 1e-6) first.  log_decay <= 0 (-inf: the state is forgotten); keys of length one at most keep the recurrence stable, as its definition needs.
+ * lengths [streams] (int32, on the device; NULL = none): stream b has its first lengths[b] steps only (clamped to 0 ... steps); the rest of its inputs is not read, the rest of its
+ * output not written; a stream of no steps keeps its state.  workspace: as above. */
+typedef struct vadc_amd_gated_delta_args {
+   const void *q, *k, *v;
+   const float *log_decay, *beta;
+   float *state;
+   void *out;
+   const int32_t *lengths;
+   void *workspace;
+   int64_t workspace_bytes;
+   int64_t streams, steps, key_heads, heads, key_dim, value_dim;
+   int64_t q_stride[3], k_stride[3], v_stride[3], out_stride[3];      /* from stream to stream, step to step, head to head */
+   int64_t decay_stride[2], beta_stride[2];                           /* from stream to stream, step to step; heads are contiguous */
+   int64_t state_stride;                                              /* from stream to stream */
+   float scale;
+   int32_t normalize, dtype, device;
+} vadc_amd_gated_delta_args;
+int64_t vadc_amd_gated_delta_workspace(const vadc_amd_gated_delta_args *args); /* bytes, or a negative VADC_AMD_E* code */
+int  vadc_amd_gated_delta(const vadc_amd_gated_delta_args *args, void *hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

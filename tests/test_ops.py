@@ -1,0 +1,161 @@
+"""The operators on device tensors, without a device: their refusals (every wrong argument is an error before the device is touched) and the argument structs' layout."""
+import ctypes as C
+import os
+import re
+import subprocess
+
+import pytest
+import torch
+
+from conftest import ROOT
+from vadc_amd import _lib, ops
+from vadc_amd.engine import VadcAmdError
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def test_argument_structs_are_packed_as_the_header_lays_them_out(tmp_path):
+    text = open(os.path.join(ROOT, "include", "vadc_amd.h")).read()
+    names = {"linear": ops._LINEAR, "group_norm": ops._NORM, "gated_delta": ops._DELTA}
+    src = '#include <stdio.h>\n#include "vadc_amd.h"\nint main(void) {\n'
+    for n in names:
+        body = re.search(r"typedef struct vadc_amd_%s_args \{(.*?)\}" % n, text, re.S).group(1)
+        fields = re.findall(r"([a-z_]+)(?:\[\d\])?[,;]", re.sub(r"/\*.*?\*/", "", body, flags=re.S))
+        src += f'printf("%zu", sizeof(vadc_amd_{n}_args));' + "".join(f'printf(" %zu:%zu", offsetof(vadc_amd_{n}_args, {f}), sizeof(((vadc_amd_{n}_args *)0)->{f}));' for f in fields) + 'printf("\\n");\n'
+    (tmp_path / "s.c").write_text(src + "return 0; }\n")
+    subprocess.check_call(["gcc", "-I", os.path.join(ROOT, "include"), str(tmp_path / "s.c"), "-o", str(tmp_path / "s")])
+    for line, (n, packed) in zip(subprocess.check_output([str(tmp_path / "s")], text=True).splitlines(), names.items()):
+        size, *fields = line.split()
+        assert int(size) == packed.size, n
+        at = 0
+        for f in fields:                                             # no holes: "=" packs without padding
+            offset, width = map(int, f.split(":"))
+            assert offset == at, (n, f)
+            at += width
+        assert at == packed.size
+
+
+@pytest.mark.parametrize("kw, error", [
+    (dict(x=t(3, 5), weight=t(4, 6)), ValueError),
+    (dict(x=t(3, 5), weight=t(5)), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5), bias=t(5)), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5), residual=t(3, 5)), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5), out=t(4, 3)), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5), activation="tanh"), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5), activation=None), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5, dtype=torch.bfloat16)), TypeError),
+    (dict(x=t(3, 5, dtype=torch.float64), weight=t(4, 5, dtype=torch.float64)), TypeError),
+    (dict(x=t(5, 3).T, weight=t(4, 5)), ValueError),                 # the last dimension is not contiguous
+    (dict(x=t(3, 5), weight=t(5, 4).T), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5).requires_grad_()), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5)), ValueError),                   # no device
+])
+def test_linear_refuses(kw, error):
+    with pytest.raises(error, match="linear"):
+        ops.linear(**kw)
+
+
+@pytest.mark.parametrize("kw, error", [
+    (dict(x=t(8), groups=2), ValueError),
+    (dict(x=t(3, 8), groups=3), ValueError),
+    (dict(x=t(3, 8), groups=0), ValueError),
+    (dict(x=t(3, 8), groups=2, eps=-1.0), ValueError),
+    (dict(x=t(3, 8), groups=2, eps=float("nan")), ValueError),
+    (dict(x=t(3, 8), groups=2, weight=t(4)), ValueError),
+    (dict(x=t(3, 8), groups=2, gate=t(3, 1, 8)), ValueError),
+    (dict(x=t(3, 8), groups=2, out=t(2, 8)), ValueError),
+    (dict(x=t(3, 4, 8), groups=2, lengths=torch.zeros(3, dtype=torch.int64)), TypeError),
+    (dict(x=t(3, 4, 8), groups=2, lengths=torch.zeros(4, dtype=torch.int32)), ValueError),
+    (dict(x=t(3, 8), groups=2, weight=t(8, dtype=torch.float16)), TypeError),
+    (dict(x=t(8, 4).T, groups=2), ValueError),
+    (dict(x=t(3, 8), groups=2, activation="softmax"), ValueError),
+    (dict(x=t(3, 8).requires_grad_(), groups=2), ValueError),
+    (dict(x=t(3, 8), groups=2), ValueError),
+])
+def test_group_norm_refuses(kw, error):
+    with pytest.raises(error, match="group_norm"):
+        ops.group_norm(**kw)
+
+
+def delta_args(b=2, steps=3, hk=1, h=2, dk=4, dv=5, **kw):
+    a = dict(q=t(b, steps, hk, dk), k=t(b, steps, hk, dk), v=t(b, steps, h, dv), log_decay=t(b, steps, h), beta=t(b, steps, h), state=t(b, h, dk, dv))
+    a.update(kw)
+    return a
+
+
+@pytest.mark.parametrize("kw, error", [
+    (dict(q=t(2, 3, 4)), ValueError),
+    (dict(k=t(2, 3, 1, 5)), ValueError),
+    (dict(v=t(2, 4, 2, 5)), ValueError),
+    (dict(hk=2, h=3), ValueError),
+    (dict(dk=257), ValueError),
+    (dict(beta=t(2, 3)), ValueError),
+    (dict(state=t(2, 2, 5, 4)), ValueError),
+    (dict(state=t(2, 2, 5, 4).transpose(2, 3)), ValueError),
+    (dict(state=t(2, 2, 4, 5, dtype=torch.bfloat16)), TypeError),
+    (dict(beta=t(2, 3, 2, dtype=torch.bfloat16)), TypeError),
+    (dict(v=t(2, 3, 2, 5, dtype=torch.float16)), TypeError),
+    (dict(out=t(2, 3, 5, 2)), ValueError),
+    (dict(lengths=torch.zeros(2)), TypeError),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), ValueError),
+    (dict(q=t(2, 3, 1, 8)[..., ::2]), ValueError),
+    (dict(state=t(2, 2, 4, 5).requires_grad_()), ValueError),
+    (dict(), ValueError),
+])
+def test_gated_delta_refuses(kw, error):
+    with pytest.raises(error, match="gated_delta"):
+        ops.gated_delta(**delta_args(**kw))
+
+
+def pack(fmt, **changed):
+    """a valid argument struct of small sizes at made-up addresses (nothing is read before the checks are through), with fields changed by their place"""
+    fields = {
+        "linear": [0x1000, 0x2000, 0, 0, 0x3000, 2, 8, 8, 8, 8, 8, 8, 0, 0, 0, -1],
+        "group_norm": [0x1000, 0, 0, 0, 0x3000, 0, 0, 0, 2, 3, 8, 2, 24, 8, 24, 8, 24, 8, 0, 0, -1, 1e-5],
+        "gated_delta": [0x1000, 0x2000, 0x3000, 0x4000, 0x5000, 0x6000, 0x7000, 0, 0, 0, 2, 1, 1, 2, 4, 8] + [4, 4, 4] * 2 + [16, 16, 8] * 2 + [2, 2, 2, 2, 64, 1.0, 0, 0, -1],
+    }[fmt]
+    for at, value in changed.items():
+        fields[int(at[1:])] = value
+    return {"linear": ops._LINEAR, "group_norm": ops._NORM, "gated_delta": ops._DELTA}[fmt].pack(*fields)
+
+
+@pytest.mark.parametrize("op, changed", [
+    ("linear", dict(_0=0)), ("linear", dict(_4=0)), ("linear", dict(_0=0x1001)), ("linear", dict(_5=-1)), ("linear", dict(_5=2 ** 41)), ("linear", dict(_11=7)),
+    ("linear", dict(_12=3)), ("linear", dict(_13=9)), ("linear", dict(_5=2 ** 38, _7=2 ** 38, _11=2 ** 38)),
+    ("group_norm", dict(_0=0)), ("group_norm", dict(_4=0x3002)), ("group_norm", dict(_11=3)), ("group_norm", dict(_11=0)), ("group_norm", dict(_16=7)), ("group_norm", dict(_17=0)),
+    ("group_norm", dict(_18=-1)), ("group_norm", dict(_21=-1.0)), ("group_norm", dict(_21=float("inf"))), ("group_norm", dict(_8=2 ** 40)), ("group_norm", dict(_10=2 ** 21, _16=2 ** 23, _17=2 ** 21)),
+    ("gated_delta", dict(_3=0)), ("gated_delta", dict(_5=0x6002)), ("gated_delta", dict(_12=0)), ("gated_delta", dict(_13=3, _12=2)), ("gated_delta", dict(_14=257)), ("gated_delta", dict(_14=0)),
+    ("gated_delta", dict(_25=7)), ("gated_delta", dict(_32=63)), ("gated_delta", dict(_33=float("nan"))), ("gated_delta", dict(_35=5)), ("gated_delta", dict(_10=2 ** 40)), ("gated_delta", dict(_16=-4)),
+])
+def test_entry_points_refuse_before_the_device_is_touched(op, changed):
+    L = _lib.load()
+    assert getattr(L, "vadc_amd_" + op)(pack(op, **changed), None) == -1
+    assert op.encode() in L.vadc_amd_last_error()
+
+
+def test_entry_points_take_nothing_to_do_and_refuse_a_host_without_a_device():
+    L = _lib.load()
+    for op, empty in (("linear", dict(_5=0)), ("linear", dict(_7=0, _0=0)), ("group_norm", dict(_9=0, _0=0)), ("gated_delta", dict(_11=0)), ("gated_delta", dict(_10=0, _5=0))):
+        assert getattr(L, "vadc_amd_" + op)(pack(op, **empty), None) == 0
+    for op in ("linear", "group_norm", "gated_delta"):
+        assert getattr(L, "vadc_amd_" + op)(None, None) == -1
+    for op in ("group_norm", "gated_delta"):
+        assert getattr(L, f"vadc_amd_{op}_workspace")(pack(op)) >= 0
+        assert getattr(L, f"vadc_amd_{op}_workspace")(None) == -1
+    if not torch.cuda.is_available():
+        for op in ("linear", "group_norm", "gated_delta"):
+            assert getattr(L, "vadc_amd_" + op)(pack(op), None) == -3
+            assert b"no CPU fallback" in L.vadc_amd_last_error()
+
+
+def test_overlapping_outputs_are_refused():
+    x, w = t(4, 8), t(8, 8)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops._apart("linear", "out", x[1:], x=x)
+    with pytest.raises(ValueError, match="overlaps"):
+        ops._same_or_apart("linear", x[1:], residual=x[:3])
+    ops._same_or_apart("linear", x, residual=x)
+    ops._apart("linear", "out", x[:2], x=x[2:], weight=w)
+    assert issubclass(VadcAmdError, RuntimeError) and C.sizeof(C.c_void_p) == 8

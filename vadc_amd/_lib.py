@@ -22,6 +22,7 @@ SYMBOLS = [
     "vadc_amd_debug_stage_from_samples", "vadc_amd_debug_stage_from_stage", "vadc_amd_debug_lstm_decoder", "vadc_amd_debug_layer1_block", "vadc_amd_debug_decoder", "vadc_amd_unpin",
     "vadc_amd_set_option", "vadc_amd_get_option", "vadc_amd_set_profiling", "vadc_amd_get_kernel_time", "vadc_amd_reset_kernel_times",
     "vadc_amd_kernel_name",
+    "vadc_amd_linear", "vadc_amd_group_norm", "vadc_amd_group_norm_workspace", "vadc_amd_gated_delta", "vadc_amd_gated_delta_workspace",
 ]
 
 
@@ -102,6 +103,11 @@ def load() -> C.CDLL:
     L.vadc_amd_reset_kernel_times.argtypes = [vp]
     L.vadc_amd_kernel_name.argtypes = [i32]
     L.vadc_amd_kernel_name.restype = C.c_char_p
+    for name in ("linear", "group_norm", "gated_delta"):     # the argument structs travel as packed bytes (vadc_amd/ops.py)
+        getattr(L, "vadc_amd_" + name).argtypes = [C.c_char_p, vp]
+    for name in ("group_norm", "gated_delta"):
+        getattr(L, f"vadc_amd_{name}_workspace").argtypes = [C.c_char_p]
+        getattr(L, f"vadc_amd_{name}_workspace").restype = C.c_int64
     for name in SYMBOLS:
         getattr(L, name)          # AttributeError here == header/library mismatch
     L.vadc_amd_abi_version.restype = C.c_int
