@@ -3,6 +3,8 @@
 #include "ops_internal.h"
 #include "ops_prims.h"
 
+#include <algorithm>
+
 namespace vadc {
 namespace ops {
 
@@ -95,15 +97,398 @@ template <typename T, int VEC, int ROWS> static void launch_step(const vadc_amd_
    const int64_t tiles = (a.value_dim + 16 * VEC - 1) / (16 * VEC);
    hipLaunchKernelGGL((k_delta_step<T, VEC, ROWS>), dim3((unsigned)(a.streams * a.heads * tiles)), dim3(256), 0, s, a);
 }
+
+// ---- blocks of 64 steps ---------------------------------------------------------------------------------------------------------------------------------
+// Inside a block, with G the running sum of log_decay, a = e^G, k and q of unit length where asked (factors rk, rq; rq holds the scale):
+//   A[i][j] = beta_i e^(G_i - G_j) rk_i rk_j k_i.k_j  (j < i),  T = (I + A)^-1,  P[i][j] = e^(G_i - G_j) rq_i rk_j q_i.k_j  (j <= i)
+//   u = T (beta v - beta a rk (K S)),   out = a rq (Q S) + P u,   S = a_63 S + K^T (e^(G_63 - G) rk u)
+// k_delta_blocks computes T, P and the factors of all blocks at once, k_delta_scan walks the blocks with S in registers.  Every product runs on the bf16 matrix pipe with its float32
+// operands in three parts (ops_prims.h): float32 accuracy at three products where k and q are bfloat16, against one sixteenth of the rate on the float32 pipe.
+// Steps behind a stream's last enter as k = q = v = 0, beta = 0, log_decay = 0, which leaves S and the others alone.
+//
+// What is not finite stays where the recurrence puts it: in its column from its step on.  A product with zeros would carry a NaN to the steps BEFORE it, so it is taken out where it
+// enters (k rows, gates in k_delta_blocks; beta v - c1 x in k_delta_scan, which every non-finite operand reaches in its own step) and the column is NaN from that step on.
+constexpr int kBlock = 64;
+constexpr int kTiles = 6;                                            // 16 x 32 tiles of a lower triangle: rows 0, 16 need columns 0 .. 31 only
+struct __align__(16) BlockData {
+   b8 t[kTiles][3][64], p[kTiles][3][64];                            // operand order: a lane's eight columns of its row
+   float c1[kBlock], beta[kBlock], c2[kBlock], c3[kBlock];           // beta a rk, beta, a rq, e^(G_63 - G) rk
+   float end[4];                                                     // a_63
+};
+__device__ __forceinline__ int tile_of(int mt, int ks) { return mt < 2 ? mt : 2 * mt - 2 + ks; }
+// LDS rows of KD bfloat16 in 16-byte pieces; the piece index is mixed with the row so that 16 rows' pieces of one column lie in 16 different places of the 256 bytes of banks
+template <int KD> __device__ __forceinline__ int place(int row, int piece) { return row * KD + 8 * (KD == 64 ? piece ^ ((row >> 1) & 7) : piece ^ (row & 15)); }
+
+template <typename T> __device__ __forceinline__ void load8(const T *p, int left, T (&x)[8])      // elements at and behind `left` are zero
+{
+   if (left >= 8) {
+      const Pack<T, 8> u = *reinterpret_cast<const Pack<T, 8> *>(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = u.v[i];
+   } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = i < left ? p[i] : (T)0.0f;
+   }
+}
+
+struct Segment { int64_t from, blocks; };                            // the blocks from step `from` on that one pair of launches does
+
+template <typename T, int KD>
+__global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta_args a, const Segment seg)
+{
+   constexpr int NT = Parts<T>::n, PITCH = kBlock + 4;
+   __shared__ __attribute__((aligned(16))) __bf16 sk[NT][kBlock * KD];
+   __shared__ __attribute__((aligned(16))) float sa[kBlock * PITCH], sp[kBlock * PITCH], st[kBlock * PITCH];
+   __shared__ double sg[kBlock];
+   __shared__ float sbeta[kBlock], srk[kBlock], srq[kBlock];
+   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, l4 = lane >> 4;
+   const int64_t block = blockIdx.x % seg.blocks, head = blockIdx.x / seg.blocks % a.heads, stream = blockIdx.x / seg.blocks / a.heads;
+   const int64_t t0 = seg.from + block * kBlock;
+   const int live = (int)min((int64_t)kBlock, live_steps(a, stream) - t0), kd = (int)a.key_dim;
+   if (live <= 0) return;
+   const int64_t kh = head / (a.heads / a.key_heads);
+   const T *q = (const T *)a.q + stream * a.q_stride[0] + t0 * a.q_stride[1] + kh * a.q_stride[2], *k = (const T *)a.k + stream * a.k_stride[0] + t0 * a.k_stride[1] + kh * a.k_stride[2];
+   BlockData &out = ((BlockData *)a.workspace)[blockIdx.x];
+   {  // k into LDS in its parts, lengths of k and q: four threads a row
+      const int row = tid >> 2;
+      float kk = 0.0f, qq = 0.0f, odd = 0.0f;
+      T x[KD / 32][8];
+#pragma unroll
+      for (int s = 0; s < KD / 32; ++s) {
+         const int c = 8 * ((tid & 3) + 4 * s), left = row < live ? kd - c : 0;
+         T y[8];
+         load8(k + row * a.k_stride[1] + c, left, x[s]);
+         load8(q + row * a.q_stride[1] + c, a.normalize ? left : 0, y);
+#pragma unroll
+         for (int i = 0; i < 8; ++i) {
+            const float f = (float)x[s][i], g = (float)y[i];
+            kk = fmaf(f, f, kk); qq = fmaf(g, g, qq); odd = fmaf(f, 0.0f, odd);
+         }
+      }
+      kk = sum_lanes(kk, 4); qq = sum_lanes(qq, 4); odd = sum_lanes(odd, 4);
+#pragma unroll
+      for (int s = 0; s < KD / 32; ++s) {
+         if (odd != 0.0f)                                            // NaN: an element is not finite
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[s][i] = (T)0.0f;
+         b8 p[NT];
+         split8<T>(x[s], p);
+#pragma unroll
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&sk[n][place<KD>(row, (tid & 3) + 4 * s)]) = p[n];
+      }
+      if ((tid & 3) == 0) {
+         srk[row] = a.normalize ? 1.0f / sqrtf((odd != 0.0f ? 1.0f : kk) + 1e-6f) : 1.0f;
+         srq[row] = a.normalize ? a.scale / sqrtf(qq + 1e-6f) : a.scale;
+      }
+   }
+   if (wave == 0) {  // G in 64 bits: differences of neighbours far down the block keep their digits.  e^-200 is zero in float32, as e^-inf is
+      const int64_t t = t0 + lane;
+      float g = lane < live ? a.log_decay[stream * a.decay_stride[0] + t * a.decay_stride[1] + head] : 0.0f;
+      float beta = lane < live ? a.beta[stream * a.beta_stride[0] + t * a.beta_stride[1] + head] : 0.0f;
+      const bool bad = !(g < INFINITY) || !(fabsf(beta) < INFINITY);
+      g = bad ? 0.0f : fmaxf(g, -200.0f);
+      double sum = g;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(sum, d); sum += lane >= d ? o : 0.0; }
+      sg[lane] = sum;
+      sbeta[lane] = bad ? 0.0f : beta;
+      out.beta[lane] = bad ? NAN : beta;
+   }
+   __syncthreads();
+   {  // wave w: rows 16 w .. of k.k and q.k, tiles at and below the diagonal
+      b8 fk[KD / 32][NT], fq[KD / 32][NT];
+      const int row = 16 * wave + l15;
+#pragma unroll
+      for (int s = 0; s < KD / 32; ++s) {
+         T y[8];
+         load8(q + row * a.q_stride[1] + 32 * s + 8 * l4, row < live ? kd - (32 * s + 8 * l4) : 0, y);
+         split8<T>(y, fq[s]);
+#pragma unroll
+         for (int n = 0; n < NT; ++n) fk[s][n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(row, 4 * s + l4)]);
+      }
+      for (int nt = 0; nt <= wave; ++nt) {
+         f4 ck = {0, 0, 0, 0}, cq = {0, 0, 0, 0};
+#pragma unroll
+         for (int s = 0; s < KD / 32; ++s) {
+            b8 fb[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) fb[n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(16 * nt + l15, 4 * s + l4)]);
+            ck = mfma_parts<NT, NT>(fk[s], fb, ck);
+            cq = mfma_parts<NT, NT>(fq[s], fb, cq);
+         }
+         const int j = 16 * nt + l15;
+#pragma unroll
+         for (int r = 0; r < 4; ++r) {
+            const int i = 16 * wave + 4 * l4 + r;
+            const float e = j <= i ? expf((float)(sg[i] - sg[j])) * srk[j] : 0.0f;
+            sa[i * PITCH + j] = j < i ? sbeta[i] * srk[i] * e * ck[r] : 0.0f;
+            sp[i * PITCH + j] = j <= i ? srq[i] * e * cq[r] : 0.0f;
+         }
+      }
+   }
+   __syncthreads();
+   {  // the diagonal blocks of T by substitution, a wave each: lane = column (the four quarters of the wave do the same)
+      float t[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+         float c = i == l15 ? 1.0f : 0.0f;
+#pragma unroll
+         for (int m4 = 0; m4 < i; m4 += 4) {
+            const f4 row = *reinterpret_cast<const f4 *>(&sa[(16 * wave + i) * PITCH + 16 * wave + m4]);
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+               if (m4 + m < i) c = fmaf(-row[m], t[m4 + m], c);
+         }
+         t[i] = c;
+      }
+      if (lane < 16)
+#pragma unroll
+         for (int i = 0; i < 16; ++i) st[(16 * wave + i) * PITCH + 16 * wave + l15] = t[i];
+   }
+   __syncthreads();
+   {  // T[i][j] = -T[i][i] sum_m A[i][m] T[m][j], wave = block column j, on the float32 pipe; a result's four rows per lane are the four k's of the next product's B operand
+      f4 t[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+         if (i < wave) continue;
+         if (i == wave) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) t[i][r] = st[(16 * i + 4 * l4 + r) * PITCH + 16 * i + l15];
+            continue;
+         }
+         f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+#pragma unroll
+         for (int m = 0; m < i; ++m) {
+            if (m < wave) continue;
+            const f4 f = *reinterpret_cast<const f4 *>(&sa[(16 * i + l15) * PITCH + 16 * m + 4 * l4]);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) x = __builtin_amdgcn_mfma_f32_16x16x4f32(f[s], t[m][s], x, 0, 0, 0);
+         }
+         const f4 f = *reinterpret_cast<const f4 *>(&st[(16 * i + l15) * PITCH + 16 * i + 4 * l4]);
+#pragma unroll
+         for (int s = 0; s < 4; ++s) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[s], x[s], y, 0, 0, 0);
+#pragma unroll
+         for (int r = 0; r < 4; ++r) { t[i][r] = -y[r]; st[(16 * i + 4 * l4 + r) * PITCH + 16 * wave + l15] = -y[r]; }
+      }
+   }
+   __syncthreads();
+   for (int w = wave; w < 2 * kTiles; w += 4) {
+      const int tile = w % kTiles, mt = tile < 2 ? tile : 2 + (tile - 2) / 2, ks = tile < 2 ? 0 : (tile - 2) % 2;
+      const int i = 16 * mt + l15, j = 32 * ks + 8 * l4;
+      const float *src = (w < kTiles ? st : sp) + i * PITCH + j;
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = j + e <= i ? src[e] : 0.0f;     // tiles above the diagonal were never written
+      b8 p[3];
+      split8<float>(x, p);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) (w < kTiles ? out.t : out.p)[tile][n][lane] = p[n];
+   }
+   if (wave == 0) {
+      const float g = expf((float)sg[lane]);
+      out.c1[lane] = sbeta[lane] * g * srk[lane];
+      out.c2[lane] = g * srq[lane];
+      out.c3[lane] = expf((float)(sg[kBlock - 1] - sg[lane])) * srk[lane];
+      if (lane == 0) out.end[0] = expf((float)sg[kBlock - 1]);
+   }
+}
+
+// A workgroup of eight waves walks the blocks of one stream and head with 32 columns of S: wave (mt, nt) does rows 16 mt .. of the block's products and rows 16 mt .., 16 mt + 64 .. of S,
+// columns 16 nt ...  Operands whose k runs along memory rows (k, q, T, P) come straight from global memory in operand order, a block ahead; S, r, u and the scaled u pass
+// through LDS in three parts, written as four consecutive k's from the accumulators; k^T is staged by columns.  Three barriers a block.
+template <typename T, int KD>
+__global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_args a, const Segment seg)
+{
+   constexpr int NT = Parts<T>::n, KS = KD / 32, ST = KD / 64, COLS = 32;
+   __shared__ __attribute__((aligned(16))) __bf16 ss[3][COLS * KD], skt[NT][KD * kBlock], sr[3][COLS * kBlock], su[3][COLS * kBlock], sw[3][COLS * kBlock];
+   __shared__ int spoison[COLS];
+   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, l4 = lane >> 4, mt = wave & 3, nt = wave >> 2;
+   const int64_t tiles = (a.value_dim + COLS - 1) / COLS;
+   const int64_t tile = blockIdx.x % tiles, head = blockIdx.x / tiles % a.heads, stream = blockIdx.x / tiles / a.heads;
+   const int64_t steps = live_steps(a, stream) - seg.from;
+   if (steps <= 0) return;
+   const int blocks = (int)min(seg.blocks, (steps + kBlock - 1) / kBlock), kd = (int)a.key_dim;
+   const int64_t kh = head / (a.heads / a.key_heads);
+   const int col = 16 * nt + l15;                                    // of this workgroup's columns
+   const int64_t column = tile * COLS + col;
+   const bool there = column < a.value_dim;
+   const T *q = (const T *)a.q + stream * a.q_stride[0] + seg.from * a.q_stride[1] + kh * a.q_stride[2], *k = (const T *)a.k + stream * a.k_stride[0] + seg.from * a.k_stride[1] + kh * a.k_stride[2];
+   const T *v = (const T *)a.v + stream * a.v_stride[0] + seg.from * a.v_stride[1] + head * a.v_stride[2] + column;
+   T *o = (T *)a.out + stream * a.out_stride[0] + seg.from * a.out_stride[1] + head * a.out_stride[2] + column;
+   const BlockData *data = (const BlockData *)a.workspace + (stream * a.heads + head) * seg.blocks;
+   float *state = a.state + stream * a.state_stride + head * a.key_dim * a.value_dim + column;
+   f4 S[ST];
+#pragma unroll
+   for (int i = 0; i < ST; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+         const int row = 64 * i + 16 * mt + 4 * l4 + r;
+         S[i][r] = there && row < kd ? state[(int64_t)row * a.value_dim] : 0.0f;
+      }
+   if (tid < COLS) spoison[tid] = kBlock;
+   bool dead = false;
+
+   T xk[KS][8], xq[KS][8], xt[8][ST], xv[4];
+   const auto fetch = [&](int b) {                                   // block b's rows of k, q, v for this lane
+      const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock), row = 16 * mt + l15;
+      const int64_t t = (int64_t)b * kBlock;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+         const int c = 32 * s + 8 * l4, left = row < live ? kd - c : 0;
+         load8(k + (t + row) * a.k_stride[1] + c, left, xk[s]);
+         load8(q + (t + row) * a.q_stride[1] + c, left, xq[s]);
+      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+#pragma unroll
+         for (int e = 0; e < ST; ++e) xt[r][e] = 8 * wave + r < live && ST * lane + e < kd ? k[(t + 8 * wave + r) * a.k_stride[1] + ST * lane + e] : (T)0.0f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) xv[r] = there && 16 * mt + 4 * l4 + r < live ? v[(t + 16 * mt + 4 * l4 + r) * a.v_stride[1]] : (T)0.0f;
+   };
+   fetch(0);
+   for (int b = 0; b < blocks; ++b) {
+      const BlockData &d = data[b];
+      const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock);
+      b8 ft[2][3], fp[2][3];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+         if (s == 0 || mt >= 2)
+#pragma unroll
+            for (int n = 0; n < 3; ++n) { ft[s][n] = d.t[tile_of(mt, s)][n][lane]; fp[s][n] = d.p[tile_of(mt, s)][n][lane]; }
+      const f4 c1 = *reinterpret_cast<const f4 *>(&d.c1[16 * mt + 4 * l4]), beta = *reinterpret_cast<const f4 *>(&d.beta[16 * mt + 4 * l4]);
+      const f4 c2 = *reinterpret_cast<const f4 *>(&d.c2[16 * mt + 4 * l4]), c3 = *reinterpret_cast<const f4 *>(&d.c3[16 * mt + 4 * l4]);
+      const float end = d.end[0];
+#pragma unroll
+      for (int i = 0; i < ST; ++i) {
+         b4 p[3];
+         split4(S[i], p);
+#pragma unroll
+         for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&ss[n][place<KD>(col, 8 * i + 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+      }
+      lds_barrier();
+      f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+         b8 fs[3], f[NT];
+#pragma unroll
+         for (int n = 0; n < 3; ++n) fs[n] = *reinterpret_cast<const b8 *>(&ss[n][place<KD>(col, 4 * s + l4)]);
+         split8<T>(xk[s], f);
+         x = mfma_parts<NT, 3>(f, fs, x);
+         split8<T>(xq[s], f);
+         y = mfma_parts<NT, 3>(f, fs, y);
+      }
+#pragma unroll
+      for (int e = 0; e < ST; ++e) {                                 // k^T: read behind the last barrier of this block, last read before its first
+         T c[8];
+#pragma unroll
+         for (int r = 0; r < 8; ++r) c[r] = xt[r][e];
+         b8 p[NT];
+         split8<T>(c, p);
+#pragma unroll
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&skt[n][place<kBlock>(ST * lane + e, wave)]) = p[n];
+      }
+      f4 r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+         r[i] = beta[i] * (float)xv[i] - c1[i] * x[i];
+         if (!(fabsf(r[i]) < INFINITY)) { r[i] = 0.0f; atomicMin(&spoison[col], 16 * mt + 4 * l4 + i); }
+      }
+      if (b + 1 < blocks) fetch(b + 1);
+      b4 p[3];
+      split4(r, p);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&sr[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+      lds_barrier();
+      const int poison = dead ? 0 : spoison[col];
+      f4 u = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+         if (s == 0 || mt >= 2) {
+            b8 f[3];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) f[n] = *reinterpret_cast<const b8 *>(&sr[n][place<kBlock>(col, 4 * s + l4)]);
+            u = mfma_parts<3, 3>(ft[s], f, u);
+         }
+      split4(u, p);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&su[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+      split4(c3 * u, p);
+#pragma unroll
+      for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&sw[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+      lds_barrier();
+      if (tid < COLS) spoison[tid] = kBlock;
+      b8 fw[2][3];
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+         for (int n = 0; n < 3; ++n) fw[s][n] = *reinterpret_cast<const b8 *>(&sw[n][place<kBlock>(col, 4 * s + l4)]);
+#pragma unroll
+      for (int i = 0; i < ST; ++i) {
+         S[i] *= end;
+#pragma unroll
+         for (int s = 0; s < 2; ++s) {
+            b8 f[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) f[n] = *reinterpret_cast<const b8 *>(&skt[n][place<kBlock>(64 * i + 16 * mt + l15, 4 * s + l4)]);
+            S[i] = mfma_parts<NT, 3>(f, fw[s], S[i]);
+         }
+      }
+      y *= c2;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+         if (s == 0 || mt >= 2) {
+            b8 f[3];
+#pragma unroll
+            for (int n = 0; n < 3; ++n) f[n] = *reinterpret_cast<const b8 *>(&su[n][place<kBlock>(col, 4 * s + l4)]);
+            y = mfma_parts<3, 3>(fp[s], f, y);
+         }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+         const int row = 16 * mt + 4 * l4 + i;
+         if (there && row < live) o[((int64_t)b * kBlock + row) * a.out_stride[1]] = (T)(row < poison ? y[i] : NAN);
+      }
+      dead = dead || poison < kBlock;
+   }
+#pragma unroll
+   for (int i = 0; i < ST; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+         const int row = 64 * i + 16 * mt + 4 * l4 + r;
+         if (there && row < kd) state[(int64_t)row * a.value_dim] = dead ? NAN : S[i][r];
+      }
+}
+
+// ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
+// Blocks from 16 steps on, for keys of up to 128; the workspace holds as many blocks as stay in the last-level cache between the two launches, longer calls go out in segments of steps
+static bool in_blocks(const vadc_amd_gated_delta_args &a) { return a.steps >= 16 && a.key_dim <= 128; }
+static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
+{
+   const int64_t blocks = (a.steps + kBlock - 1) / kBlock, most = std::max<int64_t>(1, 4096 / (a.streams * a.heads));
+   return std::min(blocks, most);
+}
+template <typename T, int KD> static void launch_blocks(const vadc_amd_gated_delta_args &a, hipStream_t s)
+{
+   const int64_t step = segment_blocks(a), tiles = (a.value_dim + 31) / 32;
+   for (Segment seg = {0, 0}; seg.from < a.steps; seg.from += step * kBlock) {
+      seg.blocks = std::min(step, (a.steps - seg.from + kBlock - 1) / kBlock);
+      hipLaunchKernelGGL((k_delta_blocks<T, KD>), dim3((unsigned)(a.streams * a.heads * seg.blocks)), dim3(256), 0, s, a, seg);
+      hipLaunchKernelGGL((k_delta_scan<T, KD>), dim3((unsigned)(a.streams * a.heads * tiles)), dim3(512), 0, s, a, seg);
+   }
+}
+
 template <typename T> static void launch(const vadc_amd_gated_delta_args &a, hipStream_t s)
 {
+   if (in_blocks(a)) return a.key_dim <= 64 ? launch_blocks<T, 64>(a, s) : launch_blocks<T, 128>(a, s);
    const bool four = a.value_dim % 4 == 0;
    if (a.key_dim <= 64) four ? launch_step<T, 4, 4>(a, s) : launch_step<T, 1, 4>(a, s);
    else if (a.key_dim <= 128) four ? launch_step<T, 4, 8>(a, s) : launch_step<T, 1, 8>(a, s);
    else four ? launch_step<T, 4, 16>(a, s) : launch_step<T, 1, 16>(a, s);
 }
 
-int64_t gated_delta_workspace(const vadc_amd_gated_delta_args &) { return 0; }
+int64_t gated_delta_workspace(const vadc_amd_gated_delta_args &a)
+{
+   return in_blocks(a) ? a.streams * a.heads * segment_blocks(a) * (int64_t)sizeof(BlockData) : 0;
+}
 
 void launch_gated_delta(const vadc_amd_gated_delta_args &a, hipStream_t s)
 {

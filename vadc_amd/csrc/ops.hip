@@ -1,6 +1,7 @@
 // ops.hip -- entry points of the operators on device tensors (include/vadc_amd.h): argument checks, the device, the launch.  The kernels: kernels_ops_*.hip.
 #include "ops_internal.h"
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstring>
@@ -10,7 +11,7 @@ using vadc::fail;
 namespace {
 
 constexpr int64_t kMaxSize = int64_t(1) << 40;        // every size and stride; products of two stay inside 64 bits by the checks below
-constexpr int64_t kMaxBlocks = (int64_t(1) << 32) / 1024;      // a launch has fewer than 2^32 threads, in workgroups of up to 1024
+constexpr int64_t kMaxBlocks = (int64_t(1) << 32) / 1024;      // a launch has fewer than 2^32 threads, in workgroups of up to 1024: longer calls go out in slices
 
 bool ranged(std::initializer_list<int64_t> vs)
 {
@@ -78,7 +79,9 @@ int check_linear(const vadc_amd_linear_args *a)
    const int64_t w = width(a->dtype);
    if (!aligned(a->x, w) || !aligned(a->weight, w) || !aligned(a->bias, w) || !aligned(a->residual, w) || !aligned(a->out, w))
       return fail(VADC_AMD_EINVAL, "linear: a tensor is not aligned to its element");
-   if (product_over(kMaxBlocks, {(a->rows + 63) / 64, (a->out_features + 63) / 64})) return fail(VADC_AMD_EINVAL, "linear: too many outputs for one call");
+   if (a->out_features > (1 << 24)) return fail(VADC_AMD_EINVAL, "linear: out_features over 2^24");
+   if (product_over(kMaxSize, {a->rows, std::max({a->x_stride, a->residual_stride, a->out_stride, a->out_features})}) || product_over(kMaxSize, {a->out_features, a->weight_stride}))
+      return fail(VADC_AMD_EINVAL, "linear: a tensor spans over 2^40 elements");
    return VADC_AMD_OK;
 }
 
@@ -93,7 +96,8 @@ int check_norm(const vadc_amd_group_norm_args *a)
    if (!(a->eps >= 0.0f) || !std::isfinite(a->eps)) return fail(VADC_AMD_EINVAL, "group_norm: eps must be finite and not negative");
    if (a->sequences == 0 || a->positions == 0 || a->channels == 0) return VADC_AMD_OK;
    if (a->channels > (1 << 20)) return fail(VADC_AMD_EINVAL, "group_norm: more than 2^20 channels");
-   if (product_over(kMaxBlocks, {a->sequences, a->groups})) return fail(VADC_AMD_EINVAL, "group_norm: too many sequences and groups for one call");
+   for (const int64_t *st : {a->x_stride, a->gate_stride, a->out_stride})
+      if (product_over(kMaxSize, {a->sequences, st[0]}) || product_over(kMaxSize, {a->positions, std::max(st[1], a->channels)})) return fail(VADC_AMD_EINVAL, "group_norm: a tensor spans over 2^40 elements");
    return VADC_AMD_OK;
 }
 
@@ -109,10 +113,25 @@ int check_delta(const vadc_amd_gated_delta_args *a)
    if (a->key_heads < 1 || a->heads % a->key_heads) return fail(VADC_AMD_EINVAL, "gated_delta: %lld heads are no multiple of %lld key heads", (long long)a->heads, (long long)a->key_heads);
    if (!std::isfinite(a->scale)) return fail(VADC_AMD_EINVAL, "gated_delta: scale must be finite");
    if (a->streams == 0 || a->steps == 0 || a->heads == 0 || a->value_dim == 0) return VADC_AMD_OK;
-   if (a->value_dim > (1 << 20)) return fail(VADC_AMD_EINVAL, "gated_delta: value_dim over 2^20");
-   if (product_over(kMaxBlocks, {a->streams, a->heads, (a->value_dim + 15) / 16})) return fail(VADC_AMD_EINVAL, "gated_delta: too many streams and heads for one call");
-   if (product_over(kMaxBlocks, {a->streams, a->heads, (a->steps + 63) / 64})) return fail(VADC_AMD_EINVAL, "gated_delta: too many steps for one call");
+   if (a->value_dim > (1 << 20) || a->heads > (1 << 20) || product_over(1 << 20, {a->heads, (a->value_dim + 15) / 16})) return fail(VADC_AMD_EINVAL, "gated_delta: heads and value_dim over 2^24 values a step");
+   if (a->steps > (1 << 26)) return fail(VADC_AMD_EINVAL, "gated_delta: more than 2^26 steps");
+   for (const int64_t *st : {a->q_stride, a->k_stride, a->v_stride, a->out_stride})
+      if (product_over(kMaxSize, {a->streams, st[0]}) || product_over(kMaxSize, {a->steps, st[1]}) || product_over(kMaxSize, {a->heads, st[2]})) return fail(VADC_AMD_EINVAL, "gated_delta: a tensor spans over 2^40 elements");
+   for (const int64_t *st : {a->decay_stride, a->beta_stride})
+      if (product_over(kMaxSize, {a->streams, st[0]}) || product_over(kMaxSize, {a->steps, st[1]})) return fail(VADC_AMD_EINVAL, "gated_delta: a tensor spans over 2^40 elements");
+   if (product_over(kMaxSize, {a->streams, a->state_stride})) return fail(VADC_AMD_EINVAL, "gated_delta: a tensor spans over 2^40 elements");
    return VADC_AMD_OK;
+}
+
+const void *ahead(const void *p, int64_t elements, int64_t w) { return p ? (const char *)p + elements * w : nullptr; }
+
+// ---- slices: of rows, sequences or streams, as many as one launch takes; launches of one stream follow each other, so that all slices may use one workspace
+int64_t rows_per_launch(const vadc_amd_linear_args &a) { return std::max<int64_t>(1, kMaxBlocks / ((a.out_features + 15) / 16)); }
+int64_t sequences_per_launch(const vadc_amd_group_norm_args &a) { return std::max<int64_t>(1, kMaxBlocks / a.groups); }
+int64_t streams_per_launch(const vadc_amd_gated_delta_args &a)
+{
+   const int64_t most = kMaxBlocks / (a.heads * ((a.value_dim + 15) / 16));
+   return std::max<int64_t>(1, a.steps > 1 ? std::min(most, 8192 / a.heads) : most);      // many steps: a slice's workspace has a block of each head at once
 }
 
 }  // namespace
@@ -121,9 +140,15 @@ extern "C" int vadc_amd_linear(const vadc_amd_linear_args *a, void *hip_stream)
 {
    if (int rc = check_linear(a)) return rc;
    if (a->rows == 0 || a->out_features == 0) return VADC_AMD_OK;
+   const int64_t w = width(a->dtype);
    OnDevice d;
    if (int rc = d.enter(a->device, "linear")) return rc;
-   vadc::ops::launch_linear(*a, (hipStream_t)hip_stream);
+   for (int64_t from = 0, most = rows_per_launch(*a); from < a->rows; from += most) {
+      vadc_amd_linear_args s = *a;
+      s.rows = std::min(most, a->rows - from);
+      s.x = ahead(a->x, from * a->x_stride, w); s.residual = ahead(a->residual, from * a->residual_stride, w); s.out = (void *)ahead(a->out, from * a->out_stride, w);
+      vadc::ops::launch_linear(s, (hipStream_t)hip_stream);
+   }
    return d.left("linear");
 }
 
@@ -131,7 +156,9 @@ extern "C" int64_t vadc_amd_group_norm_workspace(const vadc_amd_group_norm_args 
 {
    if (int rc = check_norm(a)) return rc;
    if (a->sequences == 0 || a->positions == 0 || a->channels == 0) return 0;
-   return vadc::ops::group_norm_workspace(*a);
+   vadc_amd_group_norm_args s = *a;
+   s.sequences = std::min(a->sequences, sequences_per_launch(*a));
+   return vadc::ops::group_norm_workspace(s);
 }
 
 extern "C" int vadc_amd_group_norm(const vadc_amd_group_norm_args *a, void *hip_stream)
@@ -144,12 +171,18 @@ extern "C" int vadc_amd_group_norm(const vadc_amd_group_norm_args *a, void *hip_
    const int64_t w = width(a->dtype);
    if (!aligned(a->x, w) || !aligned(a->weight, w) || !aligned(a->bias, w) || !aligned(a->gate, w) || !aligned(a->out, w) || !aligned(a->lengths, 4))
       return fail(VADC_AMD_EINVAL, "group_norm: a tensor is not aligned to its element");
-   const int64_t need = vadc::ops::group_norm_workspace(*a);
+   const int64_t need = vadc_amd_group_norm_workspace(a);
    if (need && (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16)))
       return fail(VADC_AMD_EINVAL, "group_norm: the workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
    OnDevice d;
    if (int rc = d.enter(a->device, "group_norm")) return rc;
-   vadc::ops::launch_group_norm(*a, (hipStream_t)hip_stream);
+   for (int64_t from = 0, most = sequences_per_launch(*a); from < a->sequences; from += most) {
+      vadc_amd_group_norm_args s = *a;
+      s.sequences = std::min(most, a->sequences - from);
+      s.x = ahead(a->x, from * a->x_stride[0], w); s.gate = ahead(a->gate, from * a->gate_stride[0], w); s.out = (void *)ahead(a->out, from * a->out_stride[0], w);
+      s.lengths = (const int32_t *)ahead(a->lengths, from, 4);
+      vadc::ops::launch_group_norm(s, (hipStream_t)hip_stream);
+   }
    return d.left("group_norm");
 }
 
@@ -157,7 +190,9 @@ extern "C" int64_t vadc_amd_gated_delta_workspace(const vadc_amd_gated_delta_arg
 {
    if (int rc = check_delta(a)) return rc;
    if (a->streams == 0 || a->steps == 0 || a->heads == 0 || a->value_dim == 0) return 0;
-   return vadc::ops::gated_delta_workspace(*a);
+   vadc_amd_gated_delta_args s = *a;
+   s.streams = std::min(a->streams, streams_per_launch(*a));
+   return vadc::ops::gated_delta_workspace(s);
 }
 
 extern "C" int vadc_amd_gated_delta(const vadc_amd_gated_delta_args *a, void *hip_stream)
@@ -171,11 +206,19 @@ extern "C" int vadc_amd_gated_delta(const vadc_amd_gated_delta_args *a, void *hi
    const int64_t w = width(a->dtype);
    if (!aligned(a->q, w) || !aligned(a->k, w) || !aligned(a->v, w) || !aligned(a->out, w) || !aligned(a->log_decay, 4) || !aligned(a->beta, 4) || !aligned(a->state, 4) || !aligned(a->lengths, 4))
       return fail(VADC_AMD_EINVAL, "gated_delta: a tensor is not aligned to its element");
-   const int64_t need = vadc::ops::gated_delta_workspace(*a);
+   const int64_t need = vadc_amd_gated_delta_workspace(a);
    if (need && (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16)))
       return fail(VADC_AMD_EINVAL, "gated_delta: the workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
    OnDevice d;
    if (int rc = d.enter(a->device, "gated_delta")) return rc;
-   vadc::ops::launch_gated_delta(*a, (hipStream_t)hip_stream);
+   for (int64_t from = 0, most = streams_per_launch(*a); from < a->streams; from += most) {
+      vadc_amd_gated_delta_args s = *a;
+      s.streams = std::min(most, a->streams - from);
+      s.q = ahead(a->q, from * a->q_stride[0], w); s.k = ahead(a->k, from * a->k_stride[0], w); s.v = ahead(a->v, from * a->v_stride[0], w);
+      s.out = (void *)ahead(a->out, from * a->out_stride[0], w);
+      s.log_decay = a->log_decay + from * a->decay_stride[0]; s.beta = a->beta + from * a->beta_stride[0]; s.state = a->state + from * a->state_stride;
+      s.lengths = (const int32_t *)ahead(a->lengths, from, 4);
+      vadc::ops::launch_gated_delta(s, (hipStream_t)hip_stream);
+   }
    return d.left("gated_delta");
 }
