@@ -2,8 +2,12 @@
 #include "ops_internal.h"
 #include "ops_prims.h"
 
+#include <algorithm>
+
 namespace vadc {
 namespace ops {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
 
 // The epilogue of 4 consecutive output features of one row: bias, residual, activation in float32, one rounding at the end.
 template <typename T>
@@ -34,61 +38,275 @@ __device__ __forceinline__ void finish4(const vadc_amd_linear_args &a, int64_t r
    else for (int i = 0; i < left; ++i) out[col + i] = (T)y[i];
 }
 
-// 64 x 64 outputs per workgroup of four waves, float32 matrix instructions on operands converted to float32 on their way into LDS.  The weight is the A operand,
-// so that a lane's four accumulators are four consecutive features of one row.
-constexpr int kPitch = 36;       // floats per LDS row of 32: 16-byte aligned, and eight consecutive rows start in different banks
-template <typename T>
-__global__ __launch_bounds__(256) void k_linear(const vadc_amd_linear_args a)
+// ---- operands in LDS: rows of 128 bytes (KT elements of k), eight 16-byte pieces, the piece index mixed with the row so that the rows of a fragment lie in different banks
+__device__ __forceinline__ int piece_at(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) << 4); }
+template <typename T> struct Tile { static constexpr int k = 128 / (int)sizeof(T); };      // 64 elements of 16 bits, 32 of 32
+
+// one product step: 16 k's of a 32 x 32 tile (float32: in three bfloat16 parts, ops_prims.h)
+template <typename T> struct Frag;
+template <> struct Frag<__bf16> { b8 v; };
+template <> struct Frag<_Float16> { h8 v; };
+template <> struct Frag<float> { b8 p[3]; };
+template <typename T> __device__ __forceinline__ Frag<T> load_frag(const char *tile, int row, int step, int half)
 {
-   __shared__ float sx[64 * kPitch], sw[64 * kPitch];
-   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-   const int64_t tiles_n = (a.out_features + 63) / 64;
-   const int64_t row0 = (blockIdx.x / tiles_n) * 64, col0 = (blockIdx.x % tiles_n) * 64;
-   const int r = tid >> 2, c = (tid & 3) * 8;                        // a thread stages 8 consecutive k of one row of each operand
-   const T *px = (const T *)a.x + (row0 + r) * a.x_stride, *pw = (const T *)a.weight + (col0 + r) * a.weight_stride;
-   const bool okx = row0 + r < a.rows, okw = col0 + r < a.out_features;
-   f4 acc[2][2] = {};
-   const int wr = (wave & 1) * 32, wc = (wave >> 1) * 32;
-   for (int64_t k = 0; k < a.in_features; k += 32) {
-      float fx[8] = {}, fw[8] = {};
-      const int64_t left = a.in_features - (k + c);
-      if (left >= 8) {
-         if (okx) load_f32<T, 8>(px + k + c, fx);
-         if (okw) load_f32<T, 8>(pw + k + c, fw);
-      } else {
-         for (int i = 0; i < left; ++i) {
-            if (okx) fx[i] = (float)px[k + c + i];
-            if (okw) fw[i] = (float)pw[k + c + i];
-         }
+   Frag<T> f;
+   if constexpr (sizeof(T) == 2) f.v = *reinterpret_cast<const decltype(f.v) *>(tile + piece_at(row, 2 * step + half));
+   else {
+      const f4 lo = *reinterpret_cast<const f4 *>(tile + piece_at(row, 4 * step + 2 * half)), hi = *reinterpret_cast<const f4 *>(tile + piece_at(row, 4 * step + 2 * half + 1));
+      const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      split8<float>(x, f.p);
+   }
+   return f;
+}
+__device__ __forceinline__ f16v product(const Frag<__bf16> &a, const Frag<__bf16> &b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0); }
+__device__ __forceinline__ f16v product(const Frag<_Float16> &a, const Frag<_Float16> &b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.v, b.v, c, 0, 0, 0); }
+__device__ __forceinline__ f16v product(const Frag<float> &a, const Frag<float> &b, f16v c)
+{
+#pragma unroll
+   for (int o = 2; o >= 0; --o)
+#pragma unroll
+      for (int i = 0; i <= o; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[i], b.p[o - i], c, 0, 0, 0);
+   return c;
+}
+
+// 1024 bytes (eight LDS rows) from global memory straight into LDS, 16 bytes a lane, no registers between.  The caller waits with vm_wait before a barrier; M0 is written and
+// read in one statement.
+__device__ __forceinline__ void dma(uint32_t lds, uint32_t offset, const void *base)
+{
+   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(offset), "s"(base) : "memory");
+}
+template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+
+// BM rows x BN features per workgroup, WR x WC waves of (BM / WR) x (BN / WC) outputs in 32 x 32 tiles.  The weight is the A operand: a lane's accumulators are groups of four
+// consecutive features of one row.  STAGES tiles of k are in LDS or on their way there: with DMA (16-byte aligned rows) a wave waits for the oldest with a counted vmcnt -- an operation
+// the count does not know of can only make it wait longer -- and one barrier a tile lets everybody read it and the next one overwrite the last; without, tiles pass through registers.
+template <typename T, int BM, int BN, int WR, int WC, int STAGES, bool DMA>
+__global__ __launch_bounds__(64 * WR * WC) void k_linear_tile(const vadc_amd_linear_args a)
+{
+   constexpr int WAVES = WR * WC, KT = Tile<T>::k, TM = BM / WR / 32, TN = BN / WC / 32, BYTES = (BM + BN) * 128, PIECES = (BM + BN) / 8 / WAVES;
+   static_assert((BM + BN) / 8 % WAVES == 0 && (BM / 8) % PIECES == 0, "a wave's pieces lie in one operand");
+   __shared__ __attribute__((aligned(16))) char lds[STAGES * BYTES];
+   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+   const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.out_features + BN - 1) / BN;
+   // launch order -> tile: the workgroups of one XCD (every eighth) take consecutive tiles, which go down eight row tiles before the next feature tile: their operands stay in its L2
+   int64_t id;
+   {
+      const unsigned n = (unsigned)(tiles_m * tiles_n), x = blockIdx.x % 8, q = n / 8, r = n % 8;
+      id = (int64_t)(x * q + min(x, r) + blockIdx.x / 8);
+   }
+   const int64_t group = id / (8 * tiles_n), first = group * 8, high = min((int64_t)8, tiles_m - first), in = id - group * 8 * tiles_n;
+   const int64_t row0 = (first + in % high) * BM, col0 = (in / high) * BN;
+   const int wr = wave % WR * (BM / WR), wc = wave / WR * (BN / WC);
+   f16v acc[TN][TM];
+#pragma unroll
+   for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int j = 0; j < TM; ++j) acc[i][j] = (f16v)(0.0f);
+
+   // this wave's pieces of eight LDS rows: rows 8 PIECES wave .. of x's tile, then of the weight's
+   const bool of_x = wave * PIECES < BM / 8;
+   const int64_t stride = of_x ? a.x_stride : a.weight_stride, top = of_x ? row0 : col0, last = (of_x ? a.rows : a.out_features) - 1;
+   const T *src = (const T *)(of_x ? a.x : a.weight) + top * stride;
+   const int at = wave * PIECES * 8 - (of_x ? 0 : BM);                // first row in its operand
+   const auto row_of = [&](int p) { return (int)min((int64_t)(at + 8 * p + (lane >> 3)), last - top); };      // rows behind the last are copies of it: their outputs are dropped
+   const auto piece_of = [&](int p) { return (lane & 7) ^ (((at + 8 * p + (lane >> 3)) >> 1) & 7); };
+   const int64_t whole = a.in_features / KT;                          // full tiles of k
+   uint32_t offset[PIECES];
+   if constexpr (DMA)
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) offset[p] = (uint32_t)(row_of(p) * (int)(stride * sizeof(T)) + 16 * piece_of(p));
+   const auto issue = [&](int64_t kt) {
+      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (uint32_t)(kt % STAGES) * BYTES + wave * PIECES * 1024;
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) dma(to + p * 1024, offset[p], src + kt * KT);
+   };
+   T held[DMA ? 1 : PIECES][16 / sizeof(T)];
+   constexpr int PER = 16 / (int)sizeof(T);
+   const auto fetch = [&](int64_t kt, auto &h) {                      // through registers: any alignment, zeros behind the last k
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+         const int64_t k = kt * KT + piece_of(p) * PER, left = a.in_features - k;
+         const T *from = src + row_of(p) * stride + k;
+         if (left >= PER) {
+            const Pack<T, PER> u = *reinterpret_cast<const Pack<T, PER> *>(from);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) h[p][i] = u.v[i];
+         } else
+#pragma unroll
+            for (int i = 0; i < PER; ++i) h[p][i] = i < left ? from[i] : (T)0.0f;
       }
-      __syncthreads();
+   };
+   const auto place = [&](int stage, const auto &h) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { sx[r * kPitch + c + i] = fx[i]; sw[r * kPitch + c + i] = fw[i]; }
-      __syncthreads();
+      for (int p = 0; p < PIECES; ++p) {
+         Pack<T, PER> u;
 #pragma unroll
-      for (int kk = 0; kk < 32; kk += 4) {
-         float fa[2], fb[2];
+         for (int i = 0; i < PER; ++i) u.v[i] = h[p][i];
+         __builtin_memcpy(__builtin_assume_aligned(lds + stage * BYTES + (wave * PIECES + p) * 1024 + lane * 16, 16), &u, 16);
+      }
+   };
+   const auto compute = [&](int stage) {
+      const char *sx = lds + stage * BYTES, *sw = sx + BM * 128;
 #pragma unroll
-         for (int i = 0; i < 2; ++i) {
-            fa[i] = sw[(wc + 16 * i + (lane & 15)) * kPitch + kk + (lane >> 4)];
-            fb[i] = sx[(wr + 16 * i + (lane & 15)) * kPitch + kk + (lane >> 4)];
+      for (int s = 0; s < KT / 16; ++s) {
+         Frag<T> fa[TN], fb[TM];
+#pragma unroll
+         for (int i = 0; i < TN; ++i) fa[i] = load_frag<T>(sw, wc + 32 * i + (lane & 31), s, lane >> 5);
+#pragma unroll
+         for (int j = 0; j < TM; ++j) fb[j] = load_frag<T>(sx, wr + 32 * j + (lane & 31), s, lane >> 5);
+#pragma unroll
+         for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) acc[i][j] = product(fa[i], fb[j], acc[i][j]);
+      }
+   };
+
+   if constexpr (DMA) {
+      const int64_t ahead = min(whole, (int64_t)(STAGES - 1));
+      for (int64_t kt = 0; kt < ahead; ++kt) issue(kt);
+      if (a.in_features % KT) {                                       // the part of a tile at the end comes first, through registers, into the stage that is free
+         T part[PIECES][PER];
+         fetch(whole, part);
+         place(STAGES - 1, part);
+         lds_barrier();
+         compute(STAGES - 1);
+      }
+      for (int64_t kt = 0; kt < whole; ++kt) {
+         if (whole - kt >= STAGES - 1) vm_wait<PIECES * (STAGES - 2)>(); else vm_wait<0>();
+         lds_barrier();
+         if (kt + STAGES - 1 < whole) issue(kt + STAGES - 1);
+         compute((int)(kt % STAGES));
+      }
+   } else {
+      const int64_t all = (a.in_features + KT - 1) / KT;
+      if (all) { fetch(0, held); place(0, held); }
+      for (int64_t kt = 0; kt < all; ++kt) {
+         if (kt + 1 < all) fetch(kt + 1, held);
+         lds_barrier();
+         compute((int)(kt & 1));
+         if (kt + 1 < all) place((int)((kt + 1) & 1), held);          // its readers are behind the barrier above
+      }
+   }
+   if constexpr (sizeof(T) == 4) {
+      // An infinity times a part that is zero makes a NaN, and a value whose first part rounds to infinity one too: a wave that finds one does its outputs again, on the float32 pipe, straight
+      // from memory.  Every NaN of the definition ends here as well and stays one.
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+         for (int j = 0; j < TM; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) nan |= acc[i][j][e] != acc[i][j][e];
+      if (__any(nan)) {
+         const float *px[TM], *pw[TN];
+#pragma unroll
+         for (int j = 0; j < TM; ++j) px[j] = (const float *)a.x + min(row0 + wr + 32 * j + (lane & 31), a.rows - 1) * a.x_stride;
+#pragma unroll
+         for (int i = 0; i < TN; ++i) pw[i] = (const float *)a.weight + min(col0 + wc + 32 * i + (lane & 31), a.out_features - 1) * a.weight_stride;
+#pragma unroll
+         for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) acc[i][j] = (f16v)(0.0f);
+         for (int64_t k = lane >> 5; k - (lane >> 5) < a.in_features; k += 2) {
+            const bool in = k < a.in_features;
+#pragma unroll
+            for (int i = 0; i < TN; ++i)
+#pragma unroll
+               for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? pw[i][k] : 0.0f, in ? px[j][k] : 0.0f, acc[i][j], 0, 0, 0);
          }
-#pragma unroll
-         for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fa[i], fb[j], acc[i][j], 0, 0, 0);
       }
    }
 #pragma unroll
-   for (int i = 0; i < 2; ++i)
+   for (int j = 0; j < TM; ++j)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) finish4<T>(a, row0 + wr + 16 * j + (lane & 15), col0 + wc + 16 * i + (lane >> 4) * 4, acc[i][j]);
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+         for (int g = 0; g < 4; ++g)
+            finish4<T>(a, row0 + wr + 32 * j + (lane & 31), col0 + wc + 32 * i + 8 * g + 4 * (lane >> 5),
+                       f4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]});
 }
 
+// ---- few rows: the weight goes once through registers, nothing is shared -------------------------------------------------------------------------------
+// A workgroup does 16 features of up to 16 TM rows; its eight waves take every eighth 64 k's and add up in LDS in a fixed order.  A lane reads 32 (float32: 64) consecutive bytes of its
+// row, so that the four lanes of a row read a run: the k's of an operand fragment may come in any order that both operands share.
+template <typename T, int TM>
+__global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_args a)
+{
+   constexpr int WAVES = 8;
+   __shared__ __attribute__((aligned(16))) f4 part[WAVES][TM][64];
+   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, l4 = lane >> 4;
+   const int64_t tiles_n = (a.out_features + 15) / 16, row0 = blockIdx.x / tiles_n * (16 * TM), col0 = blockIdx.x % tiles_n * 16;
+   const T *pw = (const T *)a.weight + min(col0 + l15, a.out_features - 1) * a.weight_stride, *px[TM];
+#pragma unroll
+   for (int j = 0; j < TM; ++j) px[j] = (const T *)a.x + min(row0 + 16 * j + l15, a.rows - 1) * a.x_stride;
+   f4 acc[TM];
+#pragma unroll
+   for (int j = 0; j < TM; ++j) acc[j] = (f4)(0.0f);
+   const auto load16 = [&](const T *p, int64_t k, T (&x)[16]) {
+      const int64_t left = a.in_features - k;
+      if (left >= 16) {
+         const Pack<T, 16> u = *reinterpret_cast<const Pack<T, 16> *>(p + k);
+#pragma unroll
+         for (int i = 0; i < 16; ++i) x[i] = u.v[i];
+      } else
+#pragma unroll
+         for (int i = 0; i < 16; ++i) x[i] = i < left ? p[k + i] : (T)0.0f;
+   };
+   for (int64_t k = 64 * wave; k < a.in_features; k += 64 * WAVES) {
+      T w[16], x[TM][16];
+      load16(pw, k + 16 * l4, w);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) load16(px[j], k + 16 * l4, x[j]);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+         if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int s = 0; s < 16; ++s) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[s], x[j][s], acc[j], 0, 0, 0);
+         } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+               Frag<T> fa, fb;
+#pragma unroll
+               for (int i = 0; i < 8; ++i) { fa.v[i] = w[8 * s + i]; fb.v[i] = x[j][8 * s + i]; }
+               if constexpr (__is_same(T, __bf16)) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa.v, fb.v, acc[j], 0, 0, 0);
+               else acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa.v, fb.v, acc[j], 0, 0, 0);
+            }
+         }
+      }
+   }
+#pragma unroll
+   for (int j = 0; j < TM; ++j) part[wave][j][lane] = acc[j];
+   __syncthreads();
+   for (int j = wave; j < TM; j += WAVES) {
+      f4 sum = part[0][j][lane];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) sum += part[w][j][lane];
+      finish4<T>(a, row0 + 16 * j + l15, col0 + 4 * l4, sum);
+   }
+}
+
+// ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
+template <typename T, int BM, int BN, int WR, int WC, int STAGES> static void launch_tile(const vadc_amd_linear_args &a, hipStream_t s, bool dma)
+{
+   const dim3 grid((unsigned)(((a.rows + BM - 1) / BM) * ((a.out_features + BN - 1) / BN)));
+   if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, STAGES, true>), grid, dim3(64 * WR * WC), 0, s, a);
+   else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, 2, false>), grid, dim3(64 * WR * WC), 0, s, a);
+}
+template <typename T, int TM> static void launch_narrow(const vadc_amd_linear_args &a, hipStream_t s)
+{
+   hipLaunchKernelGGL((k_linear_narrow<T, TM>), dim3((unsigned)(((a.rows + 16 * TM - 1) / (16 * TM)) * ((a.out_features + 15) / 16))), dim3(512), 0, s, a);
+}
 template <typename T> static void launch(const vadc_amd_linear_args &a, hipStream_t s)
 {
-   const int64_t tiles = ((a.rows + 63) / 64) * ((a.out_features + 63) / 64);
-   hipLaunchKernelGGL(k_linear<T>, dim3((unsigned)tiles), dim3(256), 0, s, a);
+   if (a.rows <= 16) return launch_narrow<T, 1>(a, s);
+   if (a.rows <= 64) return launch_narrow<T, 4>(a, s);
+   constexpr int64_t per = 16 / sizeof(T);
+   const bool dma = ((uintptr_t)a.x | (uintptr_t)a.weight) % 16 == 0 && a.x_stride % per == 0 && a.weight_stride % per == 0 &&
+                    std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) < (int64_t(1) << 31) / 256;      // a tile's rows within 32-bit offsets
+   const auto tiles = [&](int64_t t) { return ((a.rows + t - 1) / t) * ((a.out_features + t - 1) / t); };
+   if constexpr (sizeof(T) == 2) if (tiles(256) >= 200) return launch_tile<T, 256, 256, 4, 2, 2>(a, s, dma);
+   if (tiles(128) >= 200) return launch_tile<T, 128, 128, 2, 2, 2>(a, s, dma);
+   launch_tile<T, 64, 64, 2, 2, 4>(a, s, dma);
 }
 
 void launch_linear(const vadc_amd_linear_args &a, hipStream_t s)
