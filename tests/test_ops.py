@@ -152,10 +152,40 @@ def test_entry_points_take_nothing_to_do_and_refuse_a_host_without_a_device():
 
 def test_overlapping_outputs_are_refused():
     x, w = t(4, 8), t(8, 8)
-    with pytest.raises(ValueError, match="overlaps"):
-        ops._apart("linear", "out", x[1:], x=x)
-    with pytest.raises(ValueError, match="overlaps"):
-        ops._same_or_apart("linear", x[1:], residual=x[:3])
-    ops._same_or_apart("linear", x, residual=x)
-    ops._apart("linear", "out", x[:2], x=x[2:], weight=w)
+
+    def spans(*ts):
+        return tuple(ops._span(ops._Layout(*ops._layout(a))) for a in ts)
+
+    with pytest.raises(ValueError, match="overlaps x"):
+        ops._apart("linear", spans(x, x[1:]), x[1:], (("x", x),))
+    with pytest.raises(ValueError, match="overlaps residual"):
+        ops._apart("linear", spans(x[:3], x[1:]), x[1:], (("residual", x[:3]),), ("residual",))
+    with pytest.raises(ValueError, match="overlaps residual"):               # the same memory in another order
+        ops._apart("linear", spans(w, w.T), w.T, (("residual", w),), ("residual",))
+    ops._apart("linear", spans(x, x), x, (("residual", x),), ("residual",))
+    ops._apart("linear", spans(x[2:], w, x[:2]), x[:2], (("x", x[2:]), ("weight", w)))
     assert issubclass(VadcAmdError, RuntimeError) and C.sizeof(C.c_void_p) == 8
+
+
+@pytest.mark.parametrize("out, error", [
+    (t(4).expand(3, 4), "on top"),
+    (torch.zeros(20).as_strided((3, 4), (2, 1)), "on top"),
+])
+def test_an_output_with_entries_on_top_of_each_other_is_refused(out, error):
+    with pytest.raises(ValueError, match=error):
+        ops.linear(t(3, 5), t(4, 5), out=out)
+    with pytest.raises(ValueError, match=error):
+        ops.group_norm(t(3, 4), 2, out=out)
+
+
+def test_rows_at_one_distance():
+    def rows(a):
+        return ops._rows("linear", "x", ops._Layout(*ops._layout(a)))
+
+    assert rows(t(6, 5)) == 5 and rows(t(5)) == 5 and rows(t(2, 3, 5)) == 5 and rows(t(6, 9)[:, :5]) == 9
+    assert rows(t(2, 1, 3, 9)[..., 2:5]) == 9 and rows(t(1, 4, 9)[:, ::2]) == 18 and rows(t(7, 2, 5)[:, 0]) == 10
+    for bad in (t(2, 6, 5)[:, ::2], t(2, 3, 5).transpose(0, 1), t(4, 6, 5)[:, :3]):
+        if bad.stride(0) == bad.shape[1] * bad.stride(1):
+            continue
+        with pytest.raises(ValueError, match="rows"):
+            rows(bad)

@@ -11,8 +11,9 @@ argument raises ValueError or TypeError before the device is touched, a failure 
 """
 from __future__ import annotations
 
+import functools
 import struct
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -31,108 +32,164 @@ _DELTA = struct.Struct("=9Qq6q12q4qqf3i")
 Tensor = torch.Tensor
 
 
-def _call(fn, packed: bytes, device: int):
-    rc = fn(packed, torch._C._cuda_getCurrentRawStream(device))
-    if rc != 0:
+# A call's checks go by its tensors' layouts (shape, strides, type, device) alone, so each set of layouts is checked once and what the checks found is kept: the fields behind the
+# pointers, the workspace's size, the bytes that each tensor spans.  A step of one stream is a matter of microseconds, and checking it is half of them.
+class _Plan(NamedTuple):
+    fields: tuple            # of the struct, behind its pointers (and its workspace)
+    shape: tuple             # of the output
+    device: int
+    spans: tuple             # bytes from each tensor's first to its last element, in the order of the layouts; the output's is last
+    workspace: int
+    empty: bool              # nothing to do
+
+
+_KEPT = 1024                 # plans, the least recently used go first
+
+
+class _Layout(NamedTuple):
+    shape: torch.Size
+    stride: tuple
+    dtype: torch.dtype
+    device: torch.device
+
+
+def _layout(t: Optional[Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+
+
+def _layouts(*ls):
+    return [None if v is None else _Layout(*v) for v in ls]
+
+
+def _check(rc: int) -> int:
+    if rc < 0:
         raise VadcAmdError(rc, _lib.load().vadc_amd_last_error().decode())
-
-
-def _bytes(fn, packed: bytes) -> int:
-    n = fn(packed)
-    if n < 0:
-        raise VadcAmdError(n, _lib.load().vadc_amd_last_error().decode())
-    return n
+    return rc
 
 
 def _no_grad(what: str, *ts: Optional[Tensor]):
-    if torch.is_grad_enabled():
-        for t in ts:
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or with tensors that ask for none")
-
-
-def _device(what: str, first: Tensor, *ts: Optional[Tensor]) -> int:
-    d = first.device
     for t in ts:
-        if t is not None and t.device != d:
-            raise ValueError(f"{what}: tensors on {d} and on {t.device}")
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or with tensors that ask for none")
+
+
+def _same_device(what: str, *ls: Optional[_Layout]) -> int:
+    d = ls[0].device
+    for v in ls:
+        if v is not None and v.device != d:
+            raise ValueError(f"{what}: tensors on {d} and on {v.device}")
     if d.type != "cuda":
         raise ValueError(f"{what}: tensors must be on a gfx950 device, not on {d} (vadc_amd has no CPU fallback)")
     return d.index
 
 
 def _activation(what: str, name: str) -> int:
-    try:
-        return ACTIVATIONS[name]
-    except (KeyError, TypeError):
-        raise ValueError(f"{what}: activation {name!r} is none of {', '.join(ACTIVATIONS)}") from None
+    if name not in ACTIVATIONS:
+        raise ValueError(f"{what}: activation {name!r} is none of {', '.join(ACTIVATIONS)}")
+    return ACTIVATIONS[name]
 
 
-def _dtype(what: str, first: Tensor, *ts: Optional[Tensor]) -> int:
-    dt = first.dtype
-    code = _DTYPES.get(dt)
-    if code is None:
+def _same_dtype(what: str, *ls: Optional[_Layout]) -> int:
+    dt = ls[0].dtype
+    if dt not in _DTYPES:
         raise TypeError(f"{what}: {dt} is none of float32, float16, bfloat16")
-    for t in ts:
-        if t is not None and t.dtype != dt:
-            raise TypeError(f"{what}: tensors of {dt} and of {t.dtype}")
-    return code
+    for v in ls:
+        if v is not None and v.dtype != dt:
+            raise TypeError(f"{what}: tensors of {dt} and of {v.dtype}")
+    return _DTYPES[dt]
 
 
-def _floats(what: str, name: str, t: Tensor):
-    if t.dtype != torch.float32:
-        raise TypeError(f"{what}: {name} must be float32, not {t.dtype}")
+def _float32(what: str, **ls: _Layout):
+    for name, v in ls.items():
+        if v.dtype != torch.float32:
+            raise TypeError(f"{what}: {name} must be float32, not {v.dtype}")
 
 
-def _inner(what: str, **ts: Optional[Tensor]):
-    for name, t in ts.items():
-        if t is not None and t.shape[-1] > 1 and t.stride(-1) != 1:
+def _shaped(what: str, shape: tuple, **ls: Optional[_Layout]):
+    for name, v in ls.items():
+        if v is not None and tuple(v.shape) != tuple(shape):
+            raise ValueError(f"{what}: {name} {tuple(v.shape)} is not {list(shape)}")
+
+
+def _inner(what: str, **ls: Optional[_Layout]):
+    for name, v in ls.items():
+        if v is not None and v.shape[-1] > 1 and v.stride[-1] != 1:
             raise ValueError(f"{what}: the last dimension of {name} must be contiguous")
 
 
-def _span(t: Tensor):
-    lo = t.data_ptr()
-    return lo, lo + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else lo
+def _distinct(what: str, v: Optional[_Layout]):
+    """no two entries of an output at one place: taken by falling stride, each dimension steps over all that the smaller ones span"""
+    if v is not None and 0 not in v.shape:
+        reach = 1
+        for stride, n in sorted(zip(v.stride, v.shape)):
+            if n > 1:
+                if stride < reach:
+                    raise ValueError(f"{what}: entries of out lie on top of each other (strides {v.stride})")
+                reach = stride * (n - 1) + reach
 
 
-def _apart(what: str, name: str, out: Tensor, **ts: Optional[Tensor]):
-    lo, hi = _span(out)
-    for other, t in ts.items():
+def _lengths(what: str, v: Optional[_Layout], n: int):
+    if v is not None:
+        if v.dtype != torch.int32:
+            raise TypeError(f"{what}: lengths must be int32, not {v.dtype}")
+        if tuple(v.shape) != (n,) or (n > 1 and v.stride[0] != 1):
+            raise ValueError(f"{what}: lengths must be a contiguous tensor of {n}")
+
+
+def _span(v: Optional[_Layout]) -> int:
+    if v is None or 0 in v.shape:
+        return 0
+    return (sum((n - 1) * s for n, s in zip(v.shape, v.stride)) + 1) * v.dtype.itemsize
+
+
+def _apart(what: str, spans: tuple, out: Tensor, ts: tuple, same: tuple = ()):
+    """out overlaps none of `ts` (named, in the order of the plan's spans); those in `same` may be out itself, entry for entry"""
+    lo = out.data_ptr()
+    hi = lo + spans[-1]
+    for (name, t), span in zip(ts, spans):
         if t is not None:
-            a, b = _span(t)
-            if a < hi and lo < b:
-                raise ValueError(f"{what}: {name} overlaps {other}")
+            at = t.data_ptr()
+            if at < hi and lo < at + span and not (name in same and at == lo and t.stride() == out.stride()):
+                raise ValueError(f"{what}: out overlaps {name}")
 
 
-def _same_or_apart(what: str, out: Tensor, **ts: Optional[Tensor]):
-    for name, t in ts.items():
-        if t is not None and not (t.data_ptr() == out.data_ptr() and t.stride() == out.stride()):
-            _apart(what, "out", out, **{name: t})
+def _rows(what: str, name: str, v: Optional[_Layout]):
+    """a tensor [..., n] as rows at one distance: that distance"""
+    if v is None:
+        return 0
+    distance = count = None
+    for n, stride in zip(reversed(v.shape[:-1]), reversed(v.stride[:-1])):
+        if n == 1:
+            continue
+        if distance is None:
+            distance, count = stride, n
+        elif stride == distance * count:
+            count *= n
+        else:
+            raise ValueError(f"{what}: the leading dimensions of {name} are not rows at one distance (strides {v.stride})")
+    return v.shape[-1] if distance is None else distance
 
 
-def _lengths(what: str, lengths: Optional[Tensor], n: int):
-    if lengths is None:
-        return
-    if lengths.dtype != torch.int32:
-        raise TypeError(f"{what}: lengths must be int32, not {lengths.dtype}")
-    if lengths.dim() != 1 or lengths.shape[0] != n or not lengths.is_contiguous():
-        raise ValueError(f"{what}: lengths must be a contiguous tensor of {n}")
-
-
-def _ptr(t: Optional[Tensor]) -> int:
-    return 0 if t is None else t.data_ptr()
-
-
-def _rows(t: Tensor):
-    """a tensor [..., n] as rows [m, n] without a copy, or None"""
-    if t.dim() == 2:
-        return t
-    if t.dim() == 1:
-        return t[None]
-    try:
-        return t.view(-1, t.shape[-1])
-    except RuntimeError:
-        return None
+@functools.lru_cache(_KEPT)
+def _plan_linear(x, weight, bias, residual, out, activation, residual_first) -> _Plan:
+    x, weight, bias, residual, out = _layouts(x, weight, bias, residual, out)
+    if len(weight.shape) != 2 or len(x.shape) < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
+    n, k = weight.shape
+    shape = tuple(x.shape[:-1]) + (n,)
+    _shaped("linear", (n,), bias=bias)
+    _shaped("linear", shape, residual=residual, out=out)
+    act = _activation("linear", activation)
+    dtype = _same_dtype("linear", x, weight, bias, residual, out)
+    _inner("linear", x=x, weight=weight, bias=bias, residual=residual, out=out)
+    _distinct("linear", out)
+    m = 1
+    for d in shape[:-1]:
+        m *= d
+    empty = m == 0 or n == 0
+    strides = (0, 0, 0, 0) if empty else (_rows("linear", "x", x) if k else 0, weight.stride[0], _rows("linear", "residual", residual), _rows("linear", "out", out) if out else n)
+    device = _same_device("linear", x, weight, bias, residual, out)
+    return _Plan((m, k, n, *strides, dtype, act, bool(residual_first), device), shape, device, tuple(map(_span, (x, weight, bias, residual, out))), 0, empty)
 
 
 def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation: str = "none", residual: Optional[Tensor] = None,
@@ -141,36 +198,46 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
 
     x [..., in], weight [out, in], bias [out], residual [..., out]; returns [..., out] (in `out`, if given, which may be the residual).  Leading dimensions must make up rows at one
     distance.  activation: none, relu, silu, gelu (with erf), sigmoid."""
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
-        raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
-    n, k = weight.shape
-    shape = x.shape[:-1] + (n,)
-    if bias is not None and bias.shape != (n,):
-        raise ValueError(f"linear: bias {tuple(bias.shape)} is not [{n}]")
-    if residual is not None and residual.shape != shape:
-        raise ValueError(f"linear: residual {tuple(residual.shape)} is not {tuple(shape)}")
-    if out is not None and out.shape != shape:
-        raise ValueError(f"linear: out {tuple(out.shape)} is not {tuple(shape)}")
-    act = _activation("linear", activation)
-    dtype = _dtype("linear", x, weight, bias, residual, out)
-    _inner("linear", x=x, weight=weight, bias=bias, residual=residual, out=out)
-    _no_grad("linear", x, weight, bias, residual, out)
-    device = _device("linear", x, weight, bias, residual, out)
+    plan = _plan_linear(_layout(x), _layout(weight), _layout(bias), _layout(residual), _layout(out), activation, residual_first)
+    if torch.is_grad_enabled():
+        _no_grad("linear", x, weight, bias, residual, out)
     if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(plan.shape)
     else:
-        _apart("linear", "out", out, x=x, weight=weight, bias=bias)
-        _same_or_apart("linear", out, residual=residual)
-    if out.numel() == 0:
-        return out
-    xr, rr, yr = _rows(x) if k else x.new_empty((out.numel() // n, 0)), residual if residual is None else _rows(residual), _rows(out)
-    if xr is None or yr is None or (rr is None and residual is not None):
-        raise ValueError("linear: the leading dimensions of a tensor are not rows at one distance")
-    m = yr.shape[0]
-    _call(_lib.load().vadc_amd_linear, _LINEAR.pack(
-        xr.data_ptr(), weight.data_ptr(), _ptr(bias), _ptr(rr), yr.data_ptr(), m, k, n, xr.stride(0), weight.stride(0), 0 if rr is None else rr.stride(0), yr.stride(0),
-        dtype, act, bool(residual_first), device), device)
+        _apart("linear", plan.spans, out, (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)), ("residual",))
+    if not plan.empty:
+        _check(_lib.load().vadc_amd_linear(_LINEAR.pack(
+            x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(), *plan.fields),
+            torch._C._cuda_getCurrentRawStream(plan.device)))
     return out
+
+
+@functools.lru_cache(_KEPT)
+def _plan_norm(x, groups, weight, bias, eps, activation, gate, lengths, out) -> _Plan:
+    x, weight, bias, gate, lengths, out = _layouts(x, weight, bias, gate, lengths, out)
+    if len(x.shape) not in (2, 3):
+        raise ValueError(f"group_norm: x {tuple(x.shape)} is neither [sequences, positions, channels] nor [tokens, channels]")
+    n, l, c = x.shape if len(x.shape) == 3 else (x.shape[0], 1, x.shape[1])
+    if groups < 1 or c % groups:
+        raise ValueError(f"group_norm: {c} channels do not divide into {groups} groups")
+    if not 0 <= eps < float("inf"):
+        raise ValueError(f"group_norm: eps {eps} must be finite and not negative")
+    _shaped("group_norm", (c,), weight=weight, bias=bias)
+    _shaped("group_norm", x.shape, gate=gate, out=out)
+    _lengths("group_norm", lengths, n)
+    act = _activation("group_norm", activation)
+    dtype = _same_dtype("group_norm", x, weight, bias, gate, out)
+    _inner("group_norm", x=x, weight=weight, bias=bias, gate=gate, out=out)
+    _distinct("group_norm", out)
+    device = _same_device("group_norm", x, weight, bias, gate, lengths, out)
+    empty = 0 in x.shape
+
+    def strides(v):
+        return (0, 0) if v is None else (v.stride[0], v.stride[1]) if len(v.shape) == 3 else (v.stride[0], c)
+
+    fields = (n, l, c, groups, *strides(x), *strides(gate), *(strides(out) if out else (l * c, c)), dtype, act, device, eps)
+    space = 0 if empty else _check(_lib.load().vadc_amd_group_norm_workspace(_NORM.pack(*(0,) * 8, *fields)))
+    return _Plan(fields, tuple(x.shape), device, tuple(map(_span, (x, weight, bias, gate, lengths, out))), space, empty)
 
 
 def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5, activation: str = "none",
@@ -179,45 +246,53 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
 
     x [sequences, positions, channels], or [tokens, channels] (each token a sequence of one position); gate like x; weight, bias [channels].  lengths [sequences] (int32): sequence n
     has its first lengths[n] positions only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given).  `out` may be x or gate."""
-    if x.dim() not in (2, 3):
-        raise ValueError(f"group_norm: x {tuple(x.shape)} is neither [sequences, positions, channels] nor [tokens, channels]")
-    n, l, c = x.shape if x.dim() == 3 else (x.shape[0], 1, x.shape[1])
-    if groups < 1 or c % groups:
-        raise ValueError(f"group_norm: {c} channels do not divide into {groups} groups")
-    if not 0 <= eps < float("inf"):
-        raise ValueError(f"group_norm: eps {eps} must be finite and not negative")
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and t.shape != (c,):
-            raise ValueError(f"group_norm: {name} {tuple(t.shape)} is not [{c}]")
-    for name, t in (("gate", gate), ("out", out)):
-        if t is not None and t.shape != x.shape:
-            raise ValueError(f"group_norm: {name} {tuple(t.shape)} is not {tuple(x.shape)}")
-    _lengths("group_norm", lengths, n)
-    act = _activation("group_norm", activation)
-    dtype = _dtype("group_norm", x, weight, bias, gate, out)
-    _inner("group_norm", x=x, weight=weight, bias=bias, gate=gate, out=out)
-    _no_grad("group_norm", x, weight, bias, gate, out)
-    device = _device("group_norm", x, weight, bias, gate, lengths, out)
+    plan = _plan_norm(_layout(x), groups, _layout(weight), _layout(bias), eps, activation, _layout(gate), _layout(lengths), _layout(out))
+    if torch.is_grad_enabled():
+        _no_grad("group_norm", x, weight, bias, gate, out)
     if out is None:
-        out = (torch.empty if lengths is None else torch.zeros)(x.shape, dtype=x.dtype, device=x.device)
+        out = x.new_empty(plan.shape) if lengths is None else x.new_zeros(plan.shape)
     else:
-        _apart("group_norm", "out", out, weight=weight, bias=bias, lengths=lengths)
-        _same_or_apart("group_norm", out, x=x, gate=gate)
-    if out.numel() == 0:
-        return out
-
-    def strides(t):
-        return (0, 0) if t is None else (t.stride(0), t.stride(1)) if t.dim() == 3 else (t.stride(0), 0)
-
-    L = _lib.load()
-    sizes = (n, l, c, groups, *strides(x), *strides(gate), *strides(out), dtype, act, device, eps)
-    pointers = (x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(gate), out.data_ptr(), _ptr(lengths))
-    space, need = None, 0
-    if l > 1:                                        # a single position never needs any
-        need = _bytes(L.vadc_amd_group_norm_workspace, _NORM.pack(*pointers, 0, 0, *sizes))
-        space = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _call(L.vadc_amd_group_norm, _NORM.pack(*pointers, _ptr(space), need, *sizes), device)
+        _apart("group_norm", plan.spans, out, (("x", x), ("weight", weight), ("bias", bias), ("gate", gate), ("lengths", lengths)), ("x", "gate"))
+    if not plan.empty:
+        space = torch.empty(plan.workspace, dtype=torch.uint8, device=x.device) if plan.workspace else None
+        _check(_lib.load().vadc_amd_group_norm(_NORM.pack(
+            x.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if gate is None else gate.data_ptr(), out.data_ptr(),
+            0 if lengths is None else lengths.data_ptr(), 0 if space is None else space.data_ptr(), plan.workspace, *plan.fields),
+            torch._C._cuda_getCurrentRawStream(plan.device)))
     return out
+
+
+@functools.lru_cache(_KEPT)
+def _plan_delta(q, k, v, log_decay, beta, state, scale, normalize, lengths, out) -> _Plan:
+    q, k, v, log_decay, beta, state, lengths, out = _layouts(q, k, v, log_decay, beta, state, lengths, out)
+    if len(q.shape) != 4 or k.shape != q.shape or len(v.shape) != 4 or v.shape[:2] != q.shape[:2]:
+        raise ValueError(f"gated_delta: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
+    b, t, hk, dk = q.shape
+    h, dv = v.shape[2:]
+    if hk < 1 or h % hk:
+        raise ValueError(f"gated_delta: {h} heads are no multiple of {hk} key heads")
+    if not 1 <= dk <= 256:
+        raise ValueError(f"gated_delta: key_dim {dk} is not in 1 ... 256")
+    _shaped("gated_delta", (b, t, h), log_decay=log_decay, beta=beta)
+    _shaped("gated_delta", (b, h, dk, dv), state=state)
+    _shaped("gated_delta", v.shape, out=out)
+    _lengths("gated_delta", lengths, b)
+    dtype = _same_dtype("gated_delta", q, k, v, out)
+    _float32("gated_delta", log_decay=log_decay, beta=beta, state=state)
+    _inner("gated_delta", q=q, k=k, v=v, log_decay=log_decay, beta=beta, out=out)
+    _distinct("gated_delta", out)
+    part = dk * dv
+    if 0 not in state.shape and any(n > 1 and have != want for n, have, want in zip(state.shape[1:], state.stride[1:], (part, dv, 1))):
+        raise ValueError("gated_delta: each stream's part of state must be contiguous")
+    scale = dk ** -0.5 if scale is None else float(scale)
+    if not abs(scale) < float("inf"):
+        raise ValueError("gated_delta: scale must be finite")
+    device = _same_device("gated_delta", q, k, v, log_decay, beta, state, lengths, out)
+    empty = 0 in v.shape
+    fields = (b, t, hk, h, dk, dv, *q.stride[:3], *k.stride[:3], *v.stride[:3], *(out.stride[:3] if out else (t * h * dv, h * dv, dv)), *log_decay.stride[:2], *beta.stride[:2],
+              state.stride[0] if b > 1 else h * part, scale, bool(normalize), dtype, device)
+    space = 0 if empty else _check(_lib.load().vadc_amd_gated_delta_workspace(_DELTA.pack(*(0,) * 10, *fields)))
+    return _Plan(fields, tuple(v.shape), device, tuple(map(_span, (q, k, v, log_decay, beta, state, lengths, out))), space, empty)
 
 
 def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor, state: Tensor, scale: Optional[float] = None, normalize: bool = False,
@@ -227,46 +302,18 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor
     q, k [streams, steps, key_heads, key_dim], v [streams, steps, heads, value_dim], log_decay, beta [streams, steps, heads] (float32), state [streams, heads, key_dim, value_dim]
     (float32), which is UPDATED in place; returns [streams, steps, heads, value_dim].  heads is a multiple of key_heads (consecutive heads share a key head); key_dim is 256 at most.
     scale: 1 / sqrt(key_dim) by default.  normalize: q and k are brought to unit length (x / sqrt(sum x^2 + 1e-6)).  lengths [streams] (int32): stream b has its first lengths[b] steps
-    only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given); a stream of no steps keeps its state."""
-    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2]:
-        raise ValueError(f"gated_delta: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
-    b, t, hk, dk = q.shape
-    h, dv = v.shape[2:]
-    if hk < 1 or h % hk:
-        raise ValueError(f"gated_delta: {h} heads are no multiple of {hk} key heads")
-    if not 1 <= dk <= 256:
-        raise ValueError(f"gated_delta: key_dim {dk} is not in 1 ... 256")
-    if log_decay.shape != (b, t, h) or beta.shape != (b, t, h):
-        raise ValueError(f"gated_delta: log_decay {tuple(log_decay.shape)} and beta {tuple(beta.shape)} must be [{b}, {t}, {h}]")
-    if state.shape != (b, h, dk, dv):
-        raise ValueError(f"gated_delta: state {tuple(state.shape)} is not [{b}, {h}, {dk}, {dv}]")
-    if out is not None and out.shape != v.shape:
-        raise ValueError(f"gated_delta: out {tuple(out.shape)} is not {tuple(v.shape)}")
-    _lengths("gated_delta", lengths, b)
-    dtype = _dtype("gated_delta", q, k, v, out)
-    _floats("gated_delta", "log_decay", log_decay)
-    _floats("gated_delta", "beta", beta)
-    _floats("gated_delta", "state", state)
-    _inner("gated_delta", q=q, k=k, v=v, log_decay=log_decay, beta=beta, out=out)
-    if not state.is_contiguous() and not state[0].is_contiguous():
-        raise ValueError("gated_delta: each stream's part of state must be contiguous")
-    if scale is None:
-        scale = dk ** -0.5
-    _no_grad("gated_delta", q, k, v, log_decay, beta, state, out)
-    device = _device("gated_delta", q, k, v, log_decay, beta, state, lengths, out)
+    only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given); a stream of no steps keeps its state.  A value that is not finite makes NaN of
+    what it reaches: its column of the state and of the outputs from its step on (a key or gate: every column of its head; a query: its own outputs)."""
+    plan = _plan_delta(_layout(q), _layout(k), _layout(v), _layout(log_decay), _layout(beta), _layout(state), scale, normalize, _layout(lengths), _layout(out))
+    if torch.is_grad_enabled():
+        _no_grad("gated_delta", q, k, v, log_decay, beta, state, out)
     if out is None:
-        out = (torch.empty if lengths is None else torch.zeros)(v.shape, dtype=v.dtype, device=v.device)
+        out = v.new_empty(plan.shape) if lengths is None else v.new_zeros(plan.shape)
     else:
-        _apart("gated_delta", "out", out, q=q, k=k, v=v, log_decay=log_decay, beta=beta, state=state, lengths=lengths)
-    if out.numel() == 0:
-        return out
-    L = _lib.load()
-    sizes = (b, t, hk, h, dk, dv, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *log_decay.stride()[:2], *beta.stride()[:2], state.stride(0),
-             scale, bool(normalize), dtype, device)
-    pointers = (q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), out.data_ptr(), _ptr(lengths))
-    space, need = None, 0
-    if t > 1:                                        # a single step never needs any
-        need = _bytes(L.vadc_amd_gated_delta_workspace, _DELTA.pack(*pointers, 0, 0, *sizes))
-        space = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _call(L.vadc_amd_gated_delta, _DELTA.pack(*pointers, _ptr(space), need, *sizes), device)
+        _apart("gated_delta", plan.spans, out, (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("state", state), ("lengths", lengths)))
+    if not plan.empty:
+        space = torch.empty(plan.workspace, dtype=torch.uint8, device=v.device) if plan.workspace else None
+        _check(_lib.load().vadc_amd_gated_delta(_DELTA.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), out.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+            0 if space is None else space.data_ptr(), plan.workspace, *plan.fields), torch._C._cuda_getCurrentRawStream(plan.device)))
     return out
