@@ -113,22 +113,65 @@ constexpr int kTiles = 6;                                            // 16 x 32 
 struct __align__(16) BlockData {
    b8 t[kTiles][3][64], p[kTiles][3][64];                            // operand order: a lane's eight columns of its row
    float c1[kBlock], beta[kBlock], c2[kBlock], c3[kBlock];           // beta a rk, beta, a rq, e^(G_63 - G) rk
-   float end[4];                                                     // a_63
+   float end[4];                                                     // a_63, four times
 };
 __device__ __forceinline__ int tile_of(int mt, int ks) { return mt < 2 ? mt : 2 * mt - 2 + ks; }
 // LDS rows of KD bfloat16 in 16-byte pieces; the piece index is mixed with the row so that 16 rows' pieces of one column lie in 16 different places of the 256 bytes of banks
 template <int KD> __device__ __forceinline__ int place(int row, int piece) { return row * KD + 8 * (KD == 64 ? piece ^ ((row >> 1) & 7) : piece ^ (row & 15)); }
 
-template <typename T> __device__ __forceinline__ void load8(const T *p, int left, T (&x)[8])      // elements at and behind `left` are zero
+// Eight elements of a row from c on, in two halves: the load, which always goes out and is always inside the row (kd >= 8), and, where the value is used, what does not count: elements
+// behind the row's kd, and everything where `keep` is false.  A load under a branch or with its value touched at once would be waited for on the spot.
+template <typename T> struct Raw8 { uint32_t w[2 * sizeof(T)]; };
+template <typename T> __device__ __forceinline__ Raw8<T> load8(const T *row, int c, int kd)
 {
-   if (left >= 8) {
-      const Pack<T, 8> u = *reinterpret_cast<const Pack<T, 8> *>(p);
+   const Pack<uint32_t, 2 * (int)sizeof(T)> u = *reinterpret_cast<const Pack<uint32_t, 2 * (int)sizeof(T)> *>(row + min(c, kd - 8));
+   Raw8<T> r;
+   __builtin_memcpy(&r, &u, sizeof(r));
+   return r;
+}
+template <typename T> __device__ __forceinline__ void trim8(Raw8<T> &r, int c, int kd, bool keep)
+{
+   constexpr int W = 2 * (int)sizeof(T);
+   {
+      const int back = c + 8 - kd;                                   // elements the load was moved back by: the row's last ones come down to the front
+      const bool moved = back > 0 && back < 8;
+      if (kd & 7) {
+         const int n = 8 - (kd & 7);
+         uint32_t v[W];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = u.v[i];
-   } else {
+         for (int i = 0; i < W; ++i) v[i] = r.w[i];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = i < left ? p[i] : (T)0.0f;
+         for (int bit = 0; bit < 3; ++bit)
+            if (n >> bit & 1) {
+               const int by = sizeof(T) == 4 ? 1 << bit : bit ? 1 << (bit - 1) : 0;      // words
+#pragma unroll
+               for (int i = 0; i < W; ++i) {
+                  if (by) v[i] = i + by < W ? v[i + by] : 0u;
+                  else v[i] = v[i] >> 16 | (i + 1 < W ? v[i + 1] << 16 : 0u);
+               }
+            }
+#pragma unroll
+         for (int i = 0; i < W; ++i) r.w[i] = moved ? v[i] : r.w[i];
+      }
+      const bool in = keep && c < kd;
+#pragma unroll
+      for (int i = 0; i < W; ++i) r.w[i] = in ? r.w[i] : 0u;
    }
+}
+template <typename T> __device__ __forceinline__ void value8(Raw8<T> r, int c, int kd, bool keep, bool partial, T (&x)[8])
+{
+   if (partial) trim8<T>(r, c, kd, keep);
+   __builtin_memcpy(x, &r, sizeof(r));
+}
+template <typename T> __device__ __forceinline__ uint32_t load1(const T *p)
+{
+   if constexpr (sizeof(T) == 2) return *reinterpret_cast<const uint16_t *>(p);
+   else return *reinterpret_cast<const uint32_t *>(p);
+}
+template <typename T> __device__ __forceinline__ T value1(uint32_t w)
+{
+   if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)w);
+   else return __builtin_bit_cast(T, w);
 }
 
 struct Segment { int64_t from, blocks; };                            // the blocks from step `from` on that one pair of launches does
@@ -141,11 +184,12 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
    __shared__ __attribute__((aligned(16))) float sa[kBlock * PITCH], sp[kBlock * PITCH], st[kBlock * PITCH];
    __shared__ double sg[kBlock];
    __shared__ float sbeta[kBlock], srk[kBlock], srq[kBlock];
-   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, l4 = lane >> 4;
+   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, l4 = lane >> 4;
    const int64_t block = blockIdx.x % seg.blocks, head = blockIdx.x / seg.blocks % a.heads, stream = blockIdx.x / seg.blocks / a.heads;
    const int64_t t0 = seg.from + block * kBlock;
    const int live = (int)min((int64_t)kBlock, live_steps(a, stream) - t0), kd = (int)a.key_dim;
    if (live <= 0) return;
+   const bool partial = live < kBlock || kd < KD;
    const int64_t kh = head / (a.heads / a.key_heads);
    const T *q = (const T *)a.q + stream * a.q_stride[0] + t0 * a.q_stride[1] + kh * a.q_stride[2], *k = (const T *)a.k + stream * a.k_stride[0] + t0 * a.k_stride[1] + kh * a.k_stride[2];
    BlockData &out = ((BlockData *)a.workspace)[blockIdx.x];
@@ -155,10 +199,10 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
       T x[KD / 32][8];
 #pragma unroll
       for (int s = 0; s < KD / 32; ++s) {
-         const int c = 8 * ((tid & 3) + 4 * s), left = row < live ? kd - c : 0;
+         const int c = 8 * ((tid & 3) + 4 * s);
          T y[8];
-         load8(k + row * a.k_stride[1] + c, left, x[s]);
-         load8(q + row * a.q_stride[1] + c, a.normalize ? left : 0, y);
+         value8<T>(load8(k + min(row, live - 1) * a.k_stride[1], c, kd), c, kd, row < live, partial, x[s]);
+         value8<T>(load8(q + min(row, live - 1) * a.q_stride[1], c, kd), c, kd, row < live, partial, y);
 #pragma unroll
          for (int i = 0; i < 8; ++i) {
             const float f = (float)x[s][i], g = (float)y[i];
@@ -201,7 +245,7 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
 #pragma unroll
       for (int s = 0; s < KD / 32; ++s) {
          T y[8];
-         load8(q + row * a.q_stride[1] + 32 * s + 8 * l4, row < live ? kd - (32 * s + 8 * l4) : 0, y);
+         value8<T>(load8(q + min(row, live - 1) * a.q_stride[1], 32 * s + 8 * l4, kd), 32 * s + 8 * l4, kd, row < live, partial, y);
          split8<T>(y, fq[s]);
 #pragma unroll
          for (int n = 0; n < NT; ++n) fk[s][n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(row, 4 * s + l4)]);
@@ -289,7 +333,7 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
       out.c1[lane] = sbeta[lane] * g * srk[lane];
       out.c2[lane] = g * srq[lane];
       out.c3[lane] = expf((float)(sg[kBlock - 1] - sg[lane])) * srk[lane];
-      if (lane == 0) out.end[0] = expf((float)sg[kBlock - 1]);
+      if (lane < 4) out.end[lane] = expf((float)sg[kBlock - 1]);
    }
 }
 
@@ -302,9 +346,10 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
    constexpr int NT = Parts<T>::n, KS = KD / 32, ST = KD / 64, COLS = 32;
    __shared__ __attribute__((aligned(16))) __bf16 ss[3][COLS * KD], skt[NT][KD * kBlock], sr[3][COLS * kBlock], su[3][COLS * kBlock], sw[3][COLS * kBlock];
    __shared__ int spoison[COLS];
-   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, l4 = lane >> 4, mt = wave & 3, nt = wave >> 2;
-   const int64_t tiles = (a.value_dim + COLS - 1) / COLS;
-   const int64_t tile = blockIdx.x % tiles, head = blockIdx.x / tiles % a.heads, stream = blockIdx.x / tiles / a.heads;
+   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, l4 = lane >> 4, mt = wave & 3, nt = wave >> 2;
+   // the workgroups of one state, which read the same k, q, T and P, lie eight apart: on one XCD, behind one L2
+   const unsigned tiles = (unsigned)((a.value_dim + COLS - 1) / COLS), all = gridDim.x / tiles, group = blockIdx.x / (8 * tiles), in = blockIdx.x - group * 8 * tiles, wide = min(8u, all - 8 * group);
+   const int64_t tile = in / wide, which = 8 * group + in % wide, head = which % a.heads, stream = which / a.heads;
    const int64_t steps = live_steps(a, stream) - seg.from;
    if (steps <= 0) return;
    const int blocks = (int)min(seg.blocks, (steps + kBlock - 1) / kBlock), kd = (int)a.key_dim;
@@ -328,36 +373,48 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
    if (tid < COLS) spoison[tid] = kBlock;
    bool dead = false;
 
-   T xk[KS][8], xq[KS][8], xt[8][ST], xv[4];
-   const auto fetch = [&](int b) {                                   // block b's rows of k, q, v for this lane
-      const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock), row = 16 * mt + l15;
+   constexpr bool PAIR = ST == 2 && sizeof(T) == 2;                  // a lane's two columns of k in one word
+   Raw8<T> xk[KS], xq[KS];
+   uint32_t xt[8][PAIR ? 1 : ST], xv[4];
+   const T *pk = k + (16 * mt + l15) * a.k_stride[1], *pq = q + (16 * mt + l15) * a.q_stride[1], *pv = v + (16 * mt + 4 * l4) * a.v_stride[1] - (there ? 0 : col);
+   const auto fetch = [&](int b) {                                   // block b's rows of k, q, v for this lane; rows behind the last are copies of it
+      const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock), back = min(0, live - 1 - (16 * mt + l15));
       const int64_t t = (int64_t)b * kBlock;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-         const int c = 32 * s + 8 * l4, left = row < live ? kd - c : 0;
-         load8(k + (t + row) * a.k_stride[1] + c, left, xk[s]);
-         load8(q + (t + row) * a.q_stride[1] + c, left, xq[s]);
+         xk[s] = load8(pk + (t + back) * a.k_stride[1], 32 * s + 8 * l4, kd);
+         xq[s] = load8(pq + (t + back) * a.q_stride[1], 32 * s + 8 * l4, kd);
       }
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
+      for (int r = 0; r < 8; ++r) {
+         const T *from = k + (t + min(8 * wave + r, live - 1)) * a.k_stride[1] + min(ST * lane, kd - ST);
+         if constexpr (PAIR) xt[r][0] = reinterpret_cast<const Pack<uint32_t, 1> *>(from)->v[0];
+         else
 #pragma unroll
-         for (int e = 0; e < ST; ++e) xt[r][e] = 8 * wave + r < live && ST * lane + e < kd ? k[(t + 8 * wave + r) * a.k_stride[1] + ST * lane + e] : (T)0.0f;
+            for (int e = 0; e < ST; ++e) xt[r][e] = load1(from + e);
+      }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) xv[r] = there && 16 * mt + 4 * l4 + r < live ? v[(t + 16 * mt + 4 * l4 + r) * a.v_stride[1]] : (T)0.0f;
+      for (int r = 0; r < 4; ++r) xv[r] = load1(pv + (t + r + min(0, live - 1 - (16 * mt + 4 * l4 + r))) * a.v_stride[1]);
    };
+   // T, P and the factors of a block are fetched behind the last use of the block before: each has the better part of a block to arrive
+   const auto rows4 = [&](const float *f) { return *reinterpret_cast<const f4 *>(f + 16 * mt + 4 * l4); };
+   const auto tiles2 = [&](const b8 (&from)[kTiles][3][64], b8 (&to)[2][3]) {
+#pragma unroll
+      for (int n = 0; n < 3; ++n) {
+         to[0][n] = from[tile_of(mt, 0)][n][lane];
+         to[1][n] = from[tile_of(mt, mt >= 2)][n][lane];             // rows 0 .. 31 have one tile
+      }
+   };
+   b8 ft[2][3], fp[2][3];
+   f4 c1 = rows4(data->c1), beta = rows4(data->beta), c2 = rows4(data->c2), c3 = rows4(data->c3);
+   float end = data->end[lane & 3];                                  // a vector load: a scalar one would be waited for at the next barrier, with the LDS
+   tiles2(data->t, ft);
+   tiles2(data->p, fp);
    fetch(0);
    for (int b = 0; b < blocks; ++b) {
-      const BlockData &d = data[b];
+      const BlockData &next = data[min(b + 1, blocks - 1)];
       const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock);
-      b8 ft[2][3], fp[2][3];
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-         if (s == 0 || mt >= 2)
-#pragma unroll
-            for (int n = 0; n < 3; ++n) { ft[s][n] = d.t[tile_of(mt, s)][n][lane]; fp[s][n] = d.p[tile_of(mt, s)][n][lane]; }
-      const f4 c1 = *reinterpret_cast<const f4 *>(&d.c1[16 * mt + 4 * l4]), beta = *reinterpret_cast<const f4 *>(&d.beta[16 * mt + 4 * l4]);
-      const f4 c2 = *reinterpret_cast<const f4 *>(&d.c2[16 * mt + 4 * l4]), c3 = *reinterpret_cast<const f4 *>(&d.c3[16 * mt + 4 * l4]);
-      const float end = d.end[0];
+      const bool partial = live < kBlock || kd < KD;
 #pragma unroll
       for (int i = 0; i < ST; ++i) {
          b4 p[3];
@@ -365,23 +422,43 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
 #pragma unroll
          for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&ss[n][place<KD>(col, 8 * i + 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
       }
+      if (partial) {                                                 // the one place where what lies behind the rows' and columns' ends is dropped
+#pragma unroll
+         for (int s = 0; s < KS; ++s) {
+            trim8<T>(xk[s], 32 * s + 8 * l4, kd, 16 * mt + l15 < live);
+            trim8<T>(xq[s], 32 * s + 8 * l4, kd, 16 * mt + l15 < live);
+         }
+#pragma unroll
+         for (int r = 0; r < 8; ++r) {
+            const bool in = 8 * wave + r < live, moved = ST == 2 && ST * lane == kd - 1;       // an odd row's last element: its load was moved back by one
+            if constexpr (PAIR) xt[r][0] = !in || 2 * lane >= kd ? 0u : moved ? xt[r][0] >> 16 : xt[r][0];
+            else {
+               if constexpr (ST == 2) { xt[r][0] = moved ? xt[r][ST - 1] : xt[r][0]; xt[r][ST - 1] = in && 2 * lane + 1 < kd ? xt[r][ST - 1] : 0u; }
+               xt[r][0] = in && ST * lane < kd ? xt[r][0] : 0u;
+            }
+         }
+      }
       lds_barrier();
       f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-         b8 fs[3], f[NT];
+         b8 fs[3], fk[NT], fq[NT];
+         T e[8];
 #pragma unroll
          for (int n = 0; n < 3; ++n) fs[n] = *reinterpret_cast<const b8 *>(&ss[n][place<KD>(col, 4 * s + l4)]);
-         split8<T>(xk[s], f);
-         x = mfma_parts<NT, 3>(f, fs, x);
-         split8<T>(xq[s], f);
-         y = mfma_parts<NT, 3>(f, fs, y);
+         __builtin_memcpy(e, &xk[s], sizeof(e));
+         split8<T>(e, fk);
+         __builtin_memcpy(e, &xq[s], sizeof(e));
+         split8<T>(e, fq);
+         mfma_parts2<NT, 3>(fk, fs, x, fq, fs, y);
       }
 #pragma unroll
       for (int e = 0; e < ST; ++e) {                                 // k^T: read behind the last barrier of this block, last read before its first
          T c[8];
 #pragma unroll
-         for (int r = 0; r < 8; ++r) c[r] = xt[r][e];
+         for (int r = 0; r < 8; ++r) {
+            c[r] = value1<T>(PAIR ? xt[r][0] >> 16 * e : xt[r][PAIR ? 0 : e]);
+         }
          b8 p[NT];
          split8<T>(c, p);
 #pragma unroll
@@ -390,10 +467,11 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
       f4 r;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-         r[i] = beta[i] * (float)xv[i] - c1[i] * x[i];
+         r[i] = beta[i] * (there && 16 * mt + 4 * l4 + i < live ? (float)value1<T>(xv[i]) : 0.0f) - c1[i] * x[i];
          if (!(fabsf(r[i]) < INFINITY)) { r[i] = 0.0f; atomicMin(&spoison[col], 16 * mt + 4 * l4 + i); }
       }
-      if (b + 1 < blocks) fetch(b + 1);
+      c1 = rows4(next.c1); beta = rows4(next.beta);
+      fetch(min(b + 1, blocks - 1));
       b4 p[3];
       split4(r, p);
 #pragma unroll
@@ -401,14 +479,19 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
       lds_barrier();
       const int poison = dead ? 0 : spoison[col];
       f4 u = {0, 0, 0, 0};
+      {
+         b8 f[2][3];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-         if (s == 0 || mt >= 2) {
-            b8 f[3];
+         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int n = 0; n < 3; ++n) f[n] = *reinterpret_cast<const b8 *>(&sr[n][place<kBlock>(col, 4 * s + l4)]);
-            u = mfma_parts<3, 3>(ft[s], f, u);
-         }
+            for (int n = 0; n < 3; ++n) f[s][n] = *reinterpret_cast<const b8 *>(&sr[n][place<kBlock>(col, 4 * s + l4)]);
+         if (mt >= 2) {
+            f4 u2 = {0, 0, 0, 0};
+            mfma_parts2<3, 3>(ft[0], f[0], u, ft[1], f[1], u2);
+            u += u2;
+         } else u = mfma_parts<3, 3>(ft[0], f[0], u);
+      }
+      tiles2(next.t, ft);
       split4(u, p);
 #pragma unroll
       for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&su[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
@@ -417,31 +500,42 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
       for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&sw[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
       lds_barrier();
       if (tid < COLS) spoison[tid] = kBlock;
-      b8 fw[2][3];
+      c3 = rows4(next.c3);
+      {  // two chains of products at a time: the rows of S this wave holds, or one of them beside the outputs
+         b8 fw[2][3];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
+         for (int s = 0; s < 2; ++s)
 #pragma unroll
-         for (int n = 0; n < 3; ++n) fw[s][n] = *reinterpret_cast<const b8 *>(&sw[n][place<kBlock>(col, 4 * s + l4)]);
+            for (int n = 0; n < 3; ++n) fw[s][n] = *reinterpret_cast<const b8 *>(&sw[n][place<kBlock>(col, 4 * s + l4)]);
 #pragma unroll
-      for (int i = 0; i < ST; ++i) {
-         S[i] *= end;
+         for (int i = 0; i < ST; ++i) S[i] *= end;
+         end = next.end[lane & 3];
 #pragma unroll
          for (int s = 0; s < 2; ++s) {
-            b8 f[NT];
+            b8 f[ST][NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) f[n] = *reinterpret_cast<const b8 *>(&skt[n][place<kBlock>(64 * i + 16 * mt + l15, 4 * s + l4)]);
-            S[i] = mfma_parts<NT, 3>(f, fw[s], S[i]);
+            for (int i = 0; i < ST; ++i)
+#pragma unroll
+               for (int n = 0; n < NT; ++n) f[i][n] = *reinterpret_cast<const b8 *>(&skt[n][place<kBlock>(64 * i + 16 * mt + l15, 4 * s + l4)]);
+            if constexpr (ST == 2) mfma_parts2<NT, 3>(f[0], fw[s], S[0], f[1], fw[s], S[1]);
+            else S[0] = mfma_parts<NT, 3>(f[0], fw[s], S[0]);
          }
       }
-      y *= c2;
+      {
+         b8 f[2][3];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-         if (s == 0 || mt >= 2) {
-            b8 f[3];
+         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int n = 0; n < 3; ++n) f[n] = *reinterpret_cast<const b8 *>(&su[n][place<kBlock>(col, 4 * s + l4)]);
-            y = mfma_parts<3, 3>(fp[s], f, y);
-         }
+            for (int n = 0; n < 3; ++n) f[s][n] = *reinterpret_cast<const b8 *>(&su[n][place<kBlock>(col, 4 * s + l4)]);
+         y *= c2;
+         if (mt >= 2) {
+            f4 y2 = {0, 0, 0, 0};
+            mfma_parts2<3, 3>(fp[0], f[0], y, fp[1], f[1], y2);
+            y += y2;
+         } else y = mfma_parts<3, 3>(fp[0], f[0], y);
+      }
+      c2 = rows4(next.c2);
+      tiles2(next.p, fp);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
          const int row = 16 * mt + 4 * l4 + i;
@@ -459,8 +553,8 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
 }
 
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
-// Blocks from 16 steps on, for keys of up to 128; the workspace holds as many blocks as stay in the last-level cache between the two launches, longer calls go out in segments of steps
-static bool in_blocks(const vadc_amd_gated_delta_args &a) { return a.steps >= 16 && a.key_dim <= 128; }
+// Blocks from 16 steps on, for keys of 8 to 128; the workspace holds as many blocks as stay in the last-level cache between the two launches, longer calls go out in segments of steps
+static bool in_blocks(const vadc_amd_gated_delta_args &a) { return a.steps >= 16 && a.key_dim >= 8 && a.key_dim <= 128; }
 static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
 {
    const int64_t blocks = (a.steps + kBlock - 1) / kBlock, most = std::max<int64_t>(1, 4096 / (a.streams * a.heads));

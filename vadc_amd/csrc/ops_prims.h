@@ -85,6 +85,18 @@ template <int NA, int NB> __device__ __forceinline__ f4 mfma_parts(const b8 (&a)
          if (o - i >= 0 && o - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[o - i], acc, 0, 0, 0);
    return acc;
 }
+// two of them at once, product by product: the matrix pipe has the other's while one's result is under way
+template <int NA, int NB> __device__ __forceinline__ void mfma_parts2(const b8 (&a)[NA], const b8 (&b)[NB], f4 &x, const b8 (&c)[NA], const b8 (&d)[NB], f4 &y)
+{
+#pragma unroll
+   for (int o = 2; o >= 0; --o)
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+         if (o - i >= 0 && o - i < NB) {
+            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[o - i], x, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c[i], d[o - i], y, 0, 0, 0);
+         }
+}
 
 // LDS is ready for the other waves and theirs for this one; global loads stay in flight (__syncthreads would wait for them)
 __device__ __forceinline__ void lds_barrier()
