@@ -113,8 +113,9 @@ constexpr int kTiles = 6;                                            // 16 x 32 
 struct __align__(16) BlockData {
    b8 t[kTiles][3][64], p[kTiles][3][64];                            // operand order: a lane's eight columns of its row
    float c1[kBlock], beta[kBlock], c2[kBlock], c3[kBlock];           // beta a rk, beta, a rq, e^(G_63 - G) rk
-   float end[4];                                                     // a_63, four times
+   float end[32];                                                    // a_63, four times; the rest keeps the next block on a line of its own
 };
+static_assert(sizeof(BlockData) % 128 == 0, "a block's tiles start on a cache line");
 __device__ __forceinline__ int tile_of(int mt, int ks) { return mt < 2 ? mt : 2 * mt - 2 + ks; }
 // LDS rows of KD bfloat16 in 16-byte pieces; the piece index is mixed with the row so that 16 rows' pieces of one column lie in 16 different places of the 256 bytes of banks
 template <int KD> __device__ __forceinline__ int place(int row, int piece) { return row * KD + 8 * (KD == 64 ? piece ^ ((row >> 1) & 7) : piece ^ (row & 15)); }
@@ -172,6 +173,48 @@ template <typename T> __device__ __forceinline__ T value1(uint32_t w)
 {
    if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)w);
    else return __builtin_bit_cast(T, w);
+}
+// two neighbours of a row, likewise
+template <typename T> struct Raw2 { uint32_t w[sizeof(T) / 2]; };
+template <typename T> __device__ __forceinline__ Raw2<T> load2(const T *row, int c, int kd)
+{
+   const Pack<uint32_t, (int)sizeof(T) / 2> u = *reinterpret_cast<const Pack<uint32_t, (int)sizeof(T) / 2> *>(row + min(c, kd - 2));
+   Raw2<T> r;
+   __builtin_memcpy(&r, &u, sizeof(r));
+   return r;
+}
+template <typename T> __device__ __forceinline__ void trim2(Raw2<T> &r, int c, int kd, bool keep)
+{
+   const bool moved = c == kd - 1;                                   // an odd row's last element: its load was moved back by one
+   if constexpr (sizeof(T) == 2) r.w[0] = !keep || c >= kd ? 0u : moved ? r.w[0] >> 16 : r.w[0];
+   else {
+      r.w[0] = !keep || c >= kd ? 0u : moved ? r.w[1] : r.w[0];
+      r.w[1] = keep && c + 1 < kd ? r.w[1] : 0u;
+   }
+}
+template <typename T> __device__ __forceinline__ void split2(const Raw2<T> &r, uint32_t (&p)[Parts<T>::n])
+{
+   if constexpr (Parts<T>::n == 1) p[0] = r.w[0];
+   else {
+      float rest[2] = {(float)value1<T>(r.w[0]), (float)value1<T>(sizeof(T) == 2 ? r.w[0] >> 16 : r.w[sizeof(T) / 2 - 1])};
+#pragma unroll
+      for (int k = 0; k < Parts<T>::n; ++k) {
+         const __bf16 x = (__bf16)rest[0], y = (__bf16)rest[1];
+         p[k] = (uint32_t)__builtin_bit_cast(uint16_t, x) | (uint32_t)__builtin_bit_cast(uint16_t, y) << 16;
+         rest[0] -= (float)x; rest[1] -= (float)y;
+      }
+   }
+}
+// The A fragment of k^T from rows of k in LDS: 16 columns from c0 on, this lane's 8 rows from row on.  The transposing read hands lane i of 16 the i-th column of the 4 x 16 elements
+// whose rows lanes 4 m .. 4 m + 3 point at.
+template <int KD> __device__ __forceinline__ b8 load_transposed(const __bf16 *rows, int row, int c0, int l15)
+{
+   typedef short s4 __attribute__((ext_vector_type(4)));
+   typedef __attribute__((address_space(3))) s4 *lds_s4;
+   const int c = c0 + 4 * (l15 & 3);
+   const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(rows + place<KD>(row + (l15 >> 2), c >> 3) + (c & 7)));
+   const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(rows + place<KD>(row + 4 + (l15 >> 2), c >> 3) + (c & 7)));
+   return __builtin_bit_cast(b8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
 struct Segment { int64_t from, blocks; };                            // the blocks from step `from` on that one pair of launches does
@@ -338,13 +381,13 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
 }
 
 // A workgroup of eight waves walks the blocks of one stream and head with 32 columns of S: wave (mt, nt) does rows 16 mt .. of the block's products and rows 16 mt .., 16 mt + 64 .. of S,
-// columns 16 nt ...  Operands whose k runs along memory rows (k, q, T, P) come straight from global memory in operand order, a block ahead; S, r, u and the scaled u pass
-// through LDS in three parts, written as four consecutive k's from the accumulators; k^T is staged by columns.  Three barriers a block.
+// columns 16 nt ...  k and q go through registers into LDS in their parts, a block ahead, each row read once as a run; T and P come from global memory in operand order; S, r, u and the
+// scaled u pass through LDS in three parts, written as four consecutive k's from the accumulators; k^T is k's rows through the transposing LDS read.  Three barriers a block.
 template <typename T, int KD>
 __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_args a, const Segment seg)
 {
    constexpr int NT = Parts<T>::n, KS = KD / 32, ST = KD / 64, COLS = 32;
-   __shared__ __attribute__((aligned(16))) __bf16 ss[3][COLS * KD], skt[NT][KD * kBlock], sr[3][COLS * kBlock], su[3][COLS * kBlock], sw[3][COLS * kBlock];
+   __shared__ __attribute__((aligned(16))) __bf16 sk[NT][kBlock * KD], sq[NT][kBlock * KD], ss[3][COLS * KD], sr[3][COLS * kBlock], su[3][COLS * kBlock], sw[3][COLS * kBlock];
    __shared__ int spoison[COLS];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, l4 = lane >> 4, mt = wave & 3, nt = wave >> 2;
    // the workgroups of one state, which read the same k, q, T and P, lie eight apart: on one XCD, behind one L2
@@ -373,25 +416,20 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
    if (tid < COLS) spoison[tid] = kBlock;
    bool dead = false;
 
-   constexpr bool PAIR = ST == 2 && sizeof(T) == 2;                  // a lane's two columns of k in one word
-   Raw8<T> xk[KS], xq[KS];
-   uint32_t xt[8][PAIR ? 1 : ST], xv[4];
-   const T *pk = k + (16 * mt + l15) * a.k_stride[1], *pq = q + (16 * mt + l15) * a.q_stride[1], *pv = v + (16 * mt + 4 * l4) * a.v_stride[1] - (there ? 0 : col);
-   const auto fetch = [&](int b) {                                   // block b's rows of k, q, v for this lane; rows behind the last are copies of it
-      const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock), back = min(0, live - 1 - (16 * mt + l15));
+   // this lane's part of the wave's eight rows of k and q: two columns of every PER-th row from row0 on
+   constexpr int PER = 128 / KD, LOADS = 8 / PER;
+   const int row0 = 8 * wave + lane / (KD / 2), c2k = 2 * (lane % (KD / 2));
+   Raw2<T> xk[LOADS], xq[LOADS];
+   uint32_t xv[4];
+   const T *pv = v + (16 * mt + 4 * l4) * a.v_stride[1] - (there ? 0 : col);
+   const auto fetch = [&](int b) {                                   // block b's k, q, v; rows behind the last are copies of it
+      const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock);
       const int64_t t = (int64_t)b * kBlock;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-         xk[s] = load8(pk + (t + back) * a.k_stride[1], 32 * s + 8 * l4, kd);
-         xq[s] = load8(pq + (t + back) * a.q_stride[1], 32 * s + 8 * l4, kd);
-      }
-#pragma unroll
-      for (int r = 0; r < 8; ++r) {
-         const T *from = k + (t + min(8 * wave + r, live - 1)) * a.k_stride[1] + min(ST * lane, kd - ST);
-         if constexpr (PAIR) xt[r][0] = reinterpret_cast<const Pack<uint32_t, 1> *>(from)->v[0];
-         else
-#pragma unroll
-            for (int e = 0; e < ST; ++e) xt[r][e] = load1(from + e);
+      for (int i = 0; i < LOADS; ++i) {
+         const int64_t row = t + min(row0 + PER * i, live - 1);
+         xk[i] = load2(k + row * a.k_stride[1], c2k, kd);
+         xq[i] = load2(q + row * a.q_stride[1], c2k, kd);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) xv[r] = load1(pv + (t + r + min(0, live - 1 - (16 * mt + 4 * l4 + r))) * a.v_stride[1]);
@@ -422,47 +460,31 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
 #pragma unroll
          for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&ss[n][place<KD>(col, 8 * i + 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
       }
-      if (partial) {                                                 // the one place where what lies behind the rows' and columns' ends is dropped
 #pragma unroll
-         for (int s = 0; s < KS; ++s) {
-            trim8<T>(xk[s], 32 * s + 8 * l4, kd, 16 * mt + l15 < live);
-            trim8<T>(xq[s], 32 * s + 8 * l4, kd, 16 * mt + l15 < live);
-         }
+      for (int i = 0; i < LOADS; ++i) {
+         const int row = row0 + PER * i, at = place<KD>(row, c2k >> 3) + (c2k & 7);
+         if (partial) { trim2<T>(xk[i], c2k, kd, row < live); trim2<T>(xq[i], c2k, kd, row < live); }
+         uint32_t p[NT];
+         split2<T>(xk[i], p);
 #pragma unroll
-         for (int r = 0; r < 8; ++r) {
-            const bool in = 8 * wave + r < live, moved = ST == 2 && ST * lane == kd - 1;       // an odd row's last element: its load was moved back by one
-            if constexpr (PAIR) xt[r][0] = !in || 2 * lane >= kd ? 0u : moved ? xt[r][0] >> 16 : xt[r][0];
-            else {
-               if constexpr (ST == 2) { xt[r][0] = moved ? xt[r][ST - 1] : xt[r][0]; xt[r][ST - 1] = in && 2 * lane + 1 < kd ? xt[r][ST - 1] : 0u; }
-               xt[r][0] = in && ST * lane < kd ? xt[r][0] : 0u;
-            }
-         }
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<uint32_t *>(&sk[n][at]) = p[n];
+         split2<T>(xq[i], p);
+#pragma unroll
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<uint32_t *>(&sq[n][at]) = p[n];
       }
       lds_barrier();
       f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
          b8 fs[3], fk[NT], fq[NT];
-         T e[8];
 #pragma unroll
          for (int n = 0; n < 3; ++n) fs[n] = *reinterpret_cast<const b8 *>(&ss[n][place<KD>(col, 4 * s + l4)]);
-         __builtin_memcpy(e, &xk[s], sizeof(e));
-         split8<T>(e, fk);
-         __builtin_memcpy(e, &xq[s], sizeof(e));
-         split8<T>(e, fq);
-         mfma_parts2<NT, 3>(fk, fs, x, fq, fs, y);
-      }
 #pragma unroll
-      for (int e = 0; e < ST; ++e) {                                 // k^T: read behind the last barrier of this block, last read before its first
-         T c[8];
-#pragma unroll
-         for (int r = 0; r < 8; ++r) {
-            c[r] = value1<T>(PAIR ? xt[r][0] >> 16 * e : xt[r][PAIR ? 0 : e]);
+         for (int n = 0; n < NT; ++n) {
+            fk[n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(16 * mt + l15, 4 * s + l4)]);
+            fq[n] = *reinterpret_cast<const b8 *>(&sq[n][place<KD>(16 * mt + l15, 4 * s + l4)]);
          }
-         b8 p[NT];
-         split8<T>(c, p);
-#pragma unroll
-         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&skt[n][place<kBlock>(ST * lane + e, wave)]) = p[n];
+         mfma_parts2<NT, 3>(fk, fs, x, fq, fs, y);
       }
       f4 r;
 #pragma unroll
@@ -492,6 +514,13 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
          } else u = mfma_parts<3, 3>(ft[0], f[0], u);
       }
       tiles2(next.t, ft);
+      b8 kt[2][ST][NT];                                              // k^T, before the next block's k may take its place
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+         for (int i = 0; i < ST; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) kt[s][i][n] = load_transposed<KD>(sk[n], 32 * s + 8 * l4, 64 * i + 16 * mt, l15);
       split4(u, p);
 #pragma unroll
       for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&su[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
@@ -512,13 +541,8 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
          end = next.end[lane & 3];
 #pragma unroll
          for (int s = 0; s < 2; ++s) {
-            b8 f[ST][NT];
-#pragma unroll
-            for (int i = 0; i < ST; ++i)
-#pragma unroll
-               for (int n = 0; n < NT; ++n) f[i][n] = *reinterpret_cast<const b8 *>(&skt[n][place<kBlock>(64 * i + 16 * mt + l15, 4 * s + l4)]);
-            if constexpr (ST == 2) mfma_parts2<NT, 3>(f[0], fw[s], S[0], f[1], fw[s], S[1]);
-            else S[0] = mfma_parts<NT, 3>(f[0], fw[s], S[0]);
+            if constexpr (ST == 2) mfma_parts2<NT, 3>(kt[s][0], fw[s], S[0], kt[s][ST - 1], fw[s], S[ST - 1]);
+            else S[0] = mfma_parts<NT, 3>(kt[s][0], fw[s], S[0]);
          }
       }
       {
