@@ -111,7 +111,7 @@ template <typename T, int VEC, int ROWS> static void launch_step(const vadc_amd_
 constexpr int kBlock = 64;
 constexpr int kTiles = 6;                                            // 16 x 32 tiles of a lower triangle: rows 0, 16 need columns 0 .. 31 only
 struct __align__(16) BlockData {
-   b8 t[kTiles][3][64], p[kTiles][3][64];                            // operand order: a lane's eight columns of its row
+   b8 t[kTiles][3][64], p[kTiles][3][64];                            // operand order, in three parts: lane (l4, l15) has row l15, columns 4 l4 .. and 16 + 4 l4 .. of the tile
    float c1[kBlock], beta[kBlock], c2[kBlock], c3[kBlock];           // beta a rk, beta, a rq, e^(G_63 - G) rk
    float end[32];                                                    // a_63, four times; the rest keeps the next block on a line of its own
 };
@@ -159,10 +159,12 @@ template <typename T> __device__ __forceinline__ void trim8(Raw8<T> &r, int c, i
       for (int i = 0; i < W; ++i) r.w[i] = in ? r.w[i] : 0u;
    }
 }
-template <typename T> __device__ __forceinline__ void value8(Raw8<T> r, int c, int kd, bool keep, bool partial, T (&x)[8])
+// its parts, through memory of the value's own type
+template <typename T> __device__ __forceinline__ void split_raw(const Raw8<T> &r, b8 (&p)[Parts<T>::n])
 {
-   if (partial) trim8<T>(r, c, kd, keep);
-   __builtin_memcpy(x, &r, sizeof(r));
+   T x[8];
+   __builtin_memcpy(x, &r, sizeof(x));
+   split8<T>(x, p);
 }
 template <typename T> __device__ __forceinline__ uint32_t load1(const T *p)
 {
@@ -173,37 +175,6 @@ template <typename T> __device__ __forceinline__ T value1(uint32_t w)
 {
    if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)w);
    else return __builtin_bit_cast(T, w);
-}
-// two neighbours of a row, likewise
-template <typename T> struct Raw2 { uint32_t w[sizeof(T) / 2]; };
-template <typename T> __device__ __forceinline__ Raw2<T> load2(const T *row, int c, int kd)
-{
-   const Pack<uint32_t, (int)sizeof(T) / 2> u = *reinterpret_cast<const Pack<uint32_t, (int)sizeof(T) / 2> *>(row + min(c, kd - 2));
-   Raw2<T> r;
-   __builtin_memcpy(&r, &u, sizeof(r));
-   return r;
-}
-template <typename T> __device__ __forceinline__ void trim2(Raw2<T> &r, int c, int kd, bool keep)
-{
-   const bool moved = c == kd - 1;                                   // an odd row's last element: its load was moved back by one
-   if constexpr (sizeof(T) == 2) r.w[0] = !keep || c >= kd ? 0u : moved ? r.w[0] >> 16 : r.w[0];
-   else {
-      r.w[0] = !keep || c >= kd ? 0u : moved ? r.w[1] : r.w[0];
-      r.w[1] = keep && c + 1 < kd ? r.w[1] : 0u;
-   }
-}
-template <typename T> __device__ __forceinline__ void split2(const Raw2<T> &r, uint32_t (&p)[Parts<T>::n])
-{
-   if constexpr (Parts<T>::n == 1) p[0] = r.w[0];
-   else {
-      float rest[2] = {(float)value1<T>(r.w[0]), (float)value1<T>(sizeof(T) == 2 ? r.w[0] >> 16 : r.w[sizeof(T) / 2 - 1])};
-#pragma unroll
-      for (int k = 0; k < Parts<T>::n; ++k) {
-         const __bf16 x = (__bf16)rest[0], y = (__bf16)rest[1];
-         p[k] = (uint32_t)__builtin_bit_cast(uint16_t, x) | (uint32_t)__builtin_bit_cast(uint16_t, y) << 16;
-         rest[0] -= (float)x; rest[1] -= (float)y;
-      }
-   }
 }
 // The A fragment of k^T from rows of k in LDS: 16 columns from c0 on, this lane's 8 rows from row on.  The transposing read hands lane i of 16 the i-th column of the 4 x 16 elements
 // whose rows lanes 4 m .. 4 m + 3 point at.
@@ -217,14 +188,31 @@ template <int KD> __device__ __forceinline__ b8 load_transposed(const __bf16 *ro
    return __builtin_bit_cast(b8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// the tiles of rows 16 mt .. from the sixteen-column pieces a lane holds of its row
+__device__ __forceinline__ void store_rows(b8 (&to)[kTiles][3][64], const f4 (&x)[4], int mt, int lane)
+{
+#pragma unroll
+   for (int s = 0; s < 2; ++s)
+      if (s == 0 || mt >= 2) {
+         b4 lo[3], hi[3];
+         split4(x[2 * s], lo);
+         split4(x[2 * s + 1], hi);
+#pragma unroll
+         for (int n = 0; n < 3; ++n) to[tile_of(mt, s)][n][lane] = __builtin_shufflevector(lo[n], hi[n], 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+}
+
 struct Segment { int64_t from, blocks; };                            // the blocks from step `from` on that one pair of launches does
 
+// One workgroup of four waves per block.  Everything is computed transposed -- k.k and q.k as (column, row), T through T[i][j] = -(sum_m T[i][m] A[m][j]) T[j][j] -- because an accumulator
+// then holds four consecutive columns of a lane's row: what the scan wants as an operand (its k order is the same permutation of the columns on both sides), so that P and T go from
+// registers to memory.  The inverse runs on the float32 pipe, whose operand is the accumulator as it is.
 template <typename T, int KD>
 __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta_args a, const Segment seg)
 {
-   constexpr int NT = Parts<T>::n, PITCH = kBlock + 4;
+   constexpr int NT = Parts<T>::n, PITCH = kBlock + 4, KS = KD / 32;
    __shared__ __attribute__((aligned(16))) __bf16 sk[NT][kBlock * KD];
-   __shared__ __attribute__((aligned(16))) float sa[kBlock * PITCH], sp[kBlock * PITCH], st[kBlock * PITCH];
+   __shared__ __attribute__((aligned(16))) float sat[kBlock * PITCH], std_[kBlock * 20];      // A transposed; the diagonal blocks of T, each transposed
    __shared__ double sg[kBlock];
    __shared__ float sbeta[kBlock], srk[kBlock], srq[kBlock];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, l4 = lane >> 4;
@@ -236,147 +224,149 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
    const int64_t kh = head / (a.heads / a.key_heads);
    const T *q = (const T *)a.q + stream * a.q_stride[0] + t0 * a.q_stride[1] + kh * a.q_stride[2], *k = (const T *)a.k + stream * a.k_stride[0] + t0 * a.k_stride[1] + kh * a.k_stride[2];
    BlockData &out = ((BlockData *)a.workspace)[blockIdx.x];
-   {  // k into LDS in its parts, lengths of k and q: four threads a row
+   const int mine = 16 * wave + l15;                                 // the row of the block that this lane holds of the wave's sixteen
+   Raw8<T> xk[KS], xq[KS];
+   {  // rows of q in operand order; k into LDS in its parts, four threads a row
       const int row = tid >> 2;
-      float kk = 0.0f, qq = 0.0f, odd = 0.0f;
-      T x[KD / 32][8];
+      const T *from = k + min(row, live - 1) * a.k_stride[1];
 #pragma unroll
-      for (int s = 0; s < KD / 32; ++s) {
-         const int c = 8 * ((tid & 3) + 4 * s);
-         T y[8];
-         value8<T>(load8(k + min(row, live - 1) * a.k_stride[1], c, kd), c, kd, row < live, partial, x[s]);
-         value8<T>(load8(q + min(row, live - 1) * a.q_stride[1], c, kd), c, kd, row < live, partial, y);
+      for (int s = 0; s < KS; ++s) xk[s] = load8(from, 8 * ((tid & 3) + 4 * s), kd);
+      const T *fromq = q + min(mine, live - 1) * a.q_stride[1];
 #pragma unroll
-         for (int i = 0; i < 8; ++i) {
-            const float f = (float)x[s][i], g = (float)y[i];
-            kk = fmaf(f, f, kk); qq = fmaf(g, g, qq); odd = fmaf(f, 0.0f, odd);
-         }
-      }
-      kk = sum_lanes(kk, 4); qq = sum_lanes(qq, 4); odd = sum_lanes(odd, 4);
-#pragma unroll
-      for (int s = 0; s < KD / 32; ++s) {
-         if (odd != 0.0f)                                            // NaN: an element is not finite
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[s][i] = (T)0.0f;
-         b8 p[NT];
-         split8<T>(x[s], p);
-#pragma unroll
-         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&sk[n][place<KD>(row, (tid & 3) + 4 * s)]) = p[n];
-      }
-      if ((tid & 3) == 0) {
-         srk[row] = a.normalize ? 1.0f / sqrtf((odd != 0.0f ? 1.0f : kk) + 1e-6f) : 1.0f;
-         srq[row] = a.normalize ? a.scale / sqrtf(qq + 1e-6f) : a.scale;
-      }
+      for (int s = 0; s < KS; ++s) xq[s] = load8(fromq, 32 * s + 8 * l4, kd);
    }
-   if (wave == 0) {  // G in 64 bits: differences of neighbours far down the block keep their digits.  e^-200 is zero in float32, as e^-inf is
-      const int64_t t = t0 + lane;
-      float g = lane < live ? a.log_decay[stream * a.decay_stride[0] + t * a.decay_stride[1] + head] : 0.0f;
-      float beta = lane < live ? a.beta[stream * a.beta_stride[0] + t * a.beta_stride[1] + head] : 0.0f;
+   if (wave == 0) {  // G in 64 bits and in powers of two: differences of neighbours far down the block keep their digits.  e^-200 is zero in float32, as e^-inf is
+      const int64_t t = t0 + min(lane, live - 1);
+      float g = a.log_decay[stream * a.decay_stride[0] + t * a.decay_stride[1] + head], beta = a.beta[stream * a.beta_stride[0] + t * a.beta_stride[1] + head];
+      if (lane >= live) g = beta = 0.0f;
       const bool bad = !(g < INFINITY) || !(fabsf(beta) < INFINITY);
       g = bad ? 0.0f : fmaxf(g, -200.0f);
-      double sum = g;
+      double sum = g * 1.4426950408889634;
 #pragma unroll
       for (int d = 1; d < 64; d <<= 1) { const double o = __shfl_up(sum, d); sum += lane >= d ? o : 0.0; }
       sg[lane] = sum;
       sbeta[lane] = bad ? 0.0f : beta;
       out.beta[lane] = bad ? NAN : beta;
    }
-   __syncthreads();
-   {  // wave w: rows 16 w .. of k.k and q.k, tiles at and below the diagonal
-      b8 fk[KD / 32][NT], fq[KD / 32][NT];
-      const int row = 16 * wave + l15;
+   {
+      const int row = tid >> 2;
+      float kk = 0.0f, odd = 0.0f;
 #pragma unroll
-      for (int s = 0; s < KD / 32; ++s) {
-         T y[8];
-         value8<T>(load8(q + min(row, live - 1) * a.q_stride[1], 32 * s + 8 * l4, kd), 32 * s + 8 * l4, kd, row < live, partial, y);
-         split8<T>(y, fq[s]);
+      for (int s = 0; s < KS; ++s) {
+         if (partial) trim8<T>(xk[s], 8 * ((tid & 3) + 4 * s), kd, row < live);
+         T x[8];
+         __builtin_memcpy(x, &xk[s], sizeof(x));
 #pragma unroll
-         for (int n = 0; n < NT; ++n) fk[s][n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(row, 4 * s + l4)]);
+         for (int i = 0; i < 8; ++i) { const float f = (float)x[i]; kk = fmaf(f, f, kk); odd = fmaf(f, 0.0f, odd); }
       }
-      for (int nt = 0; nt <= wave; ++nt) {
-         f4 ck = {0, 0, 0, 0}, cq = {0, 0, 0, 0};
+      kk = sum_lanes(kk, 4); odd = sum_lanes(odd, 4);
 #pragma unroll
-         for (int s = 0; s < KD / 32; ++s) {
-            b8 fb[NT];
+      for (int s = 0; s < KS; ++s) {
+         if (odd != 0.0f) xk[s] = Raw8<T>{};                         // NaN: an element is not finite
+         b8 p[NT];
+         split_raw<T>(xk[s], p);
 #pragma unroll
-            for (int n = 0; n < NT; ++n) fb[n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(16 * nt + l15, 4 * s + l4)]);
-            ck = mfma_parts<NT, NT>(fk[s], fb, ck);
-            cq = mfma_parts<NT, NT>(fq[s], fb, cq);
-         }
-         const int j = 16 * nt + l15;
-#pragma unroll
-         for (int r = 0; r < 4; ++r) {
-            const int i = 16 * wave + 4 * l4 + r;
-            const float e = j <= i ? expf((float)(sg[i] - sg[j])) * srk[j] : 0.0f;
-            sa[i * PITCH + j] = j < i ? sbeta[i] * srk[i] * e * ck[r] : 0.0f;
-            sp[i * PITCH + j] = j <= i ? srq[i] * e * cq[r] : 0.0f;
-         }
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&sk[n][place<KD>(row, (tid & 3) + 4 * s)]) = p[n];
       }
+      if ((tid & 3) == 0) srk[row] = a.normalize ? 1.0f / sqrtf((odd != 0.0f ? 1.0f : kk) + 1e-6f) : 1.0f;
+      float qq = 0.0f;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+         if (partial) trim8<T>(xq[s], 32 * s + 8 * l4, kd, mine < live);
+         T x[8];
+         __builtin_memcpy(x, &xq[s], sizeof(x));
+#pragma unroll
+         for (int i = 0; i < 8; ++i) { const float f = (float)x[i]; qq = fmaf(f, f, qq); }
+      }
+      qq += __shfl_xor(qq, 16); qq += __shfl_xor(qq, 32);
+      if (l4 == 0) srq[mine] = a.normalize ? a.scale / sqrtf(qq + 1e-6f) : a.scale;
    }
    __syncthreads();
-   {  // the diagonal blocks of T by substitution, a wave each: lane = column (the four quarters of the wave do the same)
+   const double gi = sg[mine];
+   {
+      b8 fk[KS][NT], fq[KS][NT];
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+         split_raw<T>(xq[s], fq[s]);
+#pragma unroll
+         for (int n = 0; n < NT; ++n) fk[s][n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(mine, 4 * s + l4)]);
+      }
+      const float rowk = sbeta[mine] * srk[mine], rowq = srq[mine];
+      f4 p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {                                  // columns 16 j ..
+         p[j] = (f4)(0.0f);
+         if (j > wave) continue;
+         f4 ck = {0, 0, 0, 0}, cq = {0, 0, 0, 0};
+#pragma unroll
+         for (int s = 0; s < KS; ++s) {
+            b8 fa[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) fa[n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(16 * j + l15, 4 * s + l4)]);
+            mfma_parts2<NT, NT>(fa, fk[s], ck, fa, fq[s], cq);
+         }
+#pragma unroll
+         for (int r = 0; r < 4; ++r) {
+            const int c = 16 * j + 4 * l4 + r;
+            const float e = c <= mine ? __builtin_amdgcn_exp2f((float)(gi - sg[c])) * srk[c] : 0.0f;
+            sat[c * PITCH + mine] = c < mine ? rowk * e * ck[r] : 0.0f;
+            p[j][r] = c <= mine ? rowq * e * cq[r] : 0.0f;
+         }
+      }
+      store_rows(out.p, p, wave, lane);
+   }
+   __syncthreads();
+   {  // T[w][w] by substitution: lane = column (the four quarters of the wave do the same); row i of the transposed A holds what row i of T gives to the rows below
       float t[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-         float c = i == l15 ? 1.0f : 0.0f;
+      for (int i = 0; i < 16; ++i) t[i] = i == l15 ? 1.0f : 0.0f;
 #pragma unroll
-         for (int m4 = 0; m4 < i; m4 += 4) {
-            const f4 row = *reinterpret_cast<const f4 *>(&sa[(16 * wave + i) * PITCH + 16 * wave + m4]);
+      for (int i = 0; i < 15; ++i) {
+#pragma unroll
+         for (int m4 = (i + 1) & ~3; m4 < 16; m4 += 4) {
+            const f4 col = *reinterpret_cast<const f4 *>(&sat[(16 * wave + i) * PITCH + 16 * wave + m4]);
 #pragma unroll
             for (int m = 0; m < 4; ++m)
-               if (m4 + m < i) c = fmaf(-row[m], t[m4 + m], c);
+               if (m4 + m > i) t[m4 + m] = fmaf(-col[m], t[i], t[m4 + m]);
          }
-         t[i] = c;
       }
       if (lane < 16)
 #pragma unroll
-         for (int i = 0; i < 16; ++i) st[(16 * wave + i) * PITCH + 16 * wave + l15] = t[i];
+         for (int i = 0; i < 16; i += 4) *reinterpret_cast<f4 *>(&std_[mine * 20 + i]) = f4{t[i], t[i + 1], t[i + 2], t[i + 3]};
    }
    __syncthreads();
-   {  // T[i][j] = -T[i][i] sum_m A[i][m] T[m][j], wave = block column j, on the float32 pipe; a result's four rows per lane are the four k's of the next product's B operand
+   {  // wave = block row
       f4 t[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-         if (i < wave) continue;
-         if (i == wave) {
+      for (int j = 3; j >= 0; --j) {
+         t[j] = (f4)(0.0f);
+         if (j > wave) continue;
+         if (j == wave) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) t[i][r] = st[(16 * i + 4 * l4 + r) * PITCH + 16 * i + l15];
+            for (int r = 0; r < 4; ++r) t[j][r] = std_[(16 * j + 4 * l4 + r) * 20 + l15];
             continue;
          }
          f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
 #pragma unroll
-         for (int m = 0; m < i; ++m) {
-            if (m < wave) continue;
-            const f4 f = *reinterpret_cast<const f4 *>(&sa[(16 * i + l15) * PITCH + 16 * m + 4 * l4]);
+         for (int m = j + 1; m < 4; ++m) {
+            if (m > wave) continue;
+            const f4 f = *reinterpret_cast<const f4 *>(&sat[(16 * j + l15) * PITCH + 16 * m + 4 * l4]);
 #pragma unroll
             for (int s = 0; s < 4; ++s) x = __builtin_amdgcn_mfma_f32_16x16x4f32(f[s], t[m][s], x, 0, 0, 0);
          }
-         const f4 f = *reinterpret_cast<const f4 *>(&st[(16 * i + l15) * PITCH + 16 * i + 4 * l4]);
+         const f4 f = *reinterpret_cast<const f4 *>(&std_[(16 * j + l15) * 20 + 4 * l4]);
 #pragma unroll
          for (int s = 0; s < 4; ++s) y = __builtin_amdgcn_mfma_f32_16x16x4f32(f[s], x[s], y, 0, 0, 0);
-#pragma unroll
-         for (int r = 0; r < 4; ++r) { t[i][r] = -y[r]; st[(16 * i + 4 * l4 + r) * PITCH + 16 * wave + l15] = -y[r]; }
+         t[j] = -y;
       }
-   }
-   __syncthreads();
-   for (int w = wave; w < 2 * kTiles; w += 4) {
-      const int tile = w % kTiles, mt = tile < 2 ? tile : 2 + (tile - 2) / 2, ks = tile < 2 ? 0 : (tile - 2) % 2;
-      const int i = 16 * mt + l15, j = 32 * ks + 8 * l4;
-      const float *src = (w < kTiles ? st : sp) + i * PITCH + j;
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = j + e <= i ? src[e] : 0.0f;     // tiles above the diagonal were never written
-      b8 p[3];
-      split8<float>(x, p);
-#pragma unroll
-      for (int n = 0; n < 3; ++n) (w < kTiles ? out.t : out.p)[tile][n][lane] = p[n];
+      store_rows(out.t, t, wave, lane);
    }
    if (wave == 0) {
-      const float g = expf((float)sg[lane]);
+      const float g = __builtin_amdgcn_exp2f((float)sg[lane]);
       out.c1[lane] = sbeta[lane] * g * srk[lane];
       out.c2[lane] = g * srq[lane];
-      out.c3[lane] = expf((float)(sg[kBlock - 1] - sg[lane])) * srk[lane];
-      if (lane < 4) out.end[lane] = expf((float)sg[kBlock - 1]);
+      out.c3[lane] = __builtin_amdgcn_exp2f((float)(sg[kBlock - 1] - sg[lane])) * srk[lane];
+      if (lane < 4) out.end[lane] = __builtin_amdgcn_exp2f((float)sg[kBlock - 1]);
    }
 }
 
@@ -416,10 +406,10 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
    if (tid < COLS) spoison[tid] = kBlock;
    bool dead = false;
 
-   // this lane's part of the wave's eight rows of k and q: two columns of every PER-th row from row0 on
-   constexpr int PER = 128 / KD, LOADS = 8 / PER;
-   const int row0 = 8 * wave + lane / (KD / 2), c2k = 2 * (lane % (KD / 2));
-   Raw2<T> xk[LOADS], xq[LOADS];
+   // this lane's part of the wave's eight rows of k and q: one piece of eight columns in every PER-th row from row0 on
+   constexpr int PER = 512 / KD, LOADS = 8 / PER;
+   const int row0 = 8 * wave + lane / (KD / 8), piece = lane % (KD / 8);
+   Raw8<T> xk[LOADS], xq[LOADS];
    uint32_t xv[4];
    const T *pv = v + (16 * mt + 4 * l4) * a.v_stride[1] - (there ? 0 : col);
    const auto fetch = [&](int b) {                                   // block b's k, q, v; rows behind the last are copies of it
@@ -428,8 +418,8 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
          const int64_t row = t + min(row0 + PER * i, live - 1);
-         xk[i] = load2(k + row * a.k_stride[1], c2k, kd);
-         xq[i] = load2(q + row * a.q_stride[1], c2k, kd);
+         xk[i] = load8(k + row * a.k_stride[1], 8 * piece, kd);
+         xq[i] = load8(q + row * a.q_stride[1], 8 * piece, kd);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) xv[r] = load1(pv + (t + r + min(0, live - 1 - (16 * mt + 4 * l4 + r))) * a.v_stride[1]);
@@ -442,6 +432,10 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
          to[0][n] = from[tile_of(mt, 0)][n][lane];
          to[1][n] = from[tile_of(mt, mt >= 2)][n][lane];             // rows 0 .. 31 have one tile
       }
+   };
+   const auto rows8 = [&](const __bf16 *from, int s) {                // of this lane's column, in the order of T's and P's columns
+      const b4 lo = *reinterpret_cast<const b4 *>(from + place<kBlock>(col, 4 * s + (l4 >> 1)) + 4 * (l4 & 1)), hi = *reinterpret_cast<const b4 *>(from + place<kBlock>(col, 4 * s + 2 + (l4 >> 1)) + 4 * (l4 & 1));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
    };
    b8 ft[2][3], fp[2][3];
    f4 c1 = rows4(data->c1), beta = rows4(data->beta), c2 = rows4(data->c2), c3 = rows4(data->c3);
@@ -462,15 +456,15 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
       }
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-         const int row = row0 + PER * i, at = place<KD>(row, c2k >> 3) + (c2k & 7);
-         if (partial) { trim2<T>(xk[i], c2k, kd, row < live); trim2<T>(xq[i], c2k, kd, row < live); }
-         uint32_t p[NT];
-         split2<T>(xk[i], p);
+         const int row = row0 + PER * i;
+         if (partial) { trim8<T>(xk[i], 8 * piece, kd, row < live); trim8<T>(xq[i], 8 * piece, kd, row < live); }
+         b8 p[NT];
+         split_raw<T>(xk[i], p);
 #pragma unroll
-         for (int n = 0; n < NT; ++n) *reinterpret_cast<uint32_t *>(&sk[n][at]) = p[n];
-         split2<T>(xq[i], p);
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&sk[n][place<KD>(row, piece)]) = p[n];
+         split_raw<T>(xq[i], p);
 #pragma unroll
-         for (int n = 0; n < NT; ++n) *reinterpret_cast<uint32_t *>(&sq[n][at]) = p[n];
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&sq[n][place<KD>(row, piece)]) = p[n];
       }
       lds_barrier();
       f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
@@ -506,7 +500,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
 #pragma unroll
          for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int n = 0; n < 3; ++n) f[s][n] = *reinterpret_cast<const b8 *>(&sr[n][place<kBlock>(col, 4 * s + l4)]);
+            for (int n = 0; n < 3; ++n) f[s][n] = rows8(sr[n], s);
          if (mt >= 2) {
             f4 u2 = {0, 0, 0, 0};
             mfma_parts2<3, 3>(ft[0], f[0], u, ft[1], f[1], u2);
@@ -550,7 +544,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
 #pragma unroll
          for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int n = 0; n < 3; ++n) f[s][n] = *reinterpret_cast<const b8 *>(&su[n][place<kBlock>(col, 4 * s + l4)]);
+            for (int n = 0; n < 3; ++n) f[s][n] = rows8(su[n], s);
          y *= c2;
          if (mt >= 2) {
             f4 y2 = {0, 0, 0, 0};
