@@ -117,8 +117,14 @@ struct __align__(16) BlockData {
 };
 static_assert(sizeof(BlockData) % 128 == 0, "a block's tiles start on a cache line");
 __device__ __forceinline__ int tile_of(int mt, int ks) { return mt < 2 ? mt : 2 * mt - 2 + ks; }
-// LDS rows of KD bfloat16 in 16-byte pieces; the piece index is mixed with the row so that 16 rows' pieces of one column lie in 16 different places of the 256 bytes of banks
-template <int KD> __device__ __forceinline__ int place(int row, int piece) { return row * KD + 8 * (KD == 64 ? piece ^ ((row >> 1) & 7) : piece ^ (row & 15)); }
+// LDS rows of KD bfloat16 in 16-byte pieces, the piece index mixed with the row: 16 rows' pieces of one column (an operand) and two neighbouring pieces of 4 rows and of the 4 rows
+// eight further (a transposing read) lie in different places of the 256 bytes of banks
+template <int KD> __device__ __forceinline__ int place(int row, int piece)
+{
+   const int x = row >> 1;
+   const int mix = KD == 64 ? (x & 1) << 1 | (x & 4) | (x >> 1 & 1) : (row & 3) << 1 | (row & 8) | (row >> 2 & 1);
+   return row * KD + 8 * (piece ^ mix);
+}
 
 // Eight elements of a row from c on, in two halves: the load, which always goes out and is always inside the row (kd >= 8), and, where the value is used, what does not count: elements
 // behind the row's kd, and everything where `keep` is false.  A load under a branch or with its value touched at once would be waited for on the spot.
@@ -166,15 +172,43 @@ template <typename T> __device__ __forceinline__ void split_raw(const Raw8<T> &r
    __builtin_memcpy(x, &r, sizeof(x));
    split8<T>(x, p);
 }
-template <typename T> __device__ __forceinline__ uint32_t load1(const T *p)
+template <typename T> struct Raw4 { uint32_t w[sizeof(T)]; };
+template <typename T> __device__ __forceinline__ Raw4<T> load4(const T *p)
 {
-   if constexpr (sizeof(T) == 2) return *reinterpret_cast<const uint16_t *>(p);
-   else return *reinterpret_cast<const uint32_t *>(p);
+   const Pack<uint32_t, (int)sizeof(T)> u = *reinterpret_cast<const Pack<uint32_t, (int)sizeof(T)> *>(p);
+   Raw4<T> r;
+   __builtin_memcpy(&r, &u, sizeof(r));
+   return r;
 }
-template <typename T> __device__ __forceinline__ T value1(uint32_t w)
+template <typename T> __device__ __forceinline__ f4 values4(const Raw4<T> &r)
 {
-   if constexpr (sizeof(T) == 2) return __builtin_bit_cast(T, (uint16_t)w);
-   else return __builtin_bit_cast(T, w);
+   T x[4];
+   __builtin_memcpy(x, &r, sizeof(x));
+   return f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+}
+// the values behind the first `back`, moved to the front; zeros follow
+__device__ __forceinline__ f4 trim4(f4 x, int back)
+{
+   const f4 one = {x[1], x[2], x[3], 0.0f};
+   x = back & 1 ? one : x;
+   const f4 two = {x[2], x[3], 0.0f, 0.0f}, none = {0.0f, 0.0f, 0.0f, 0.0f};
+   x = back & 2 ? two : x;
+   return back >= 4 ? none : x;
+}
+// four lanes' four values, rows for columns: lane i of the four hands its j-th value to lane j
+template <int CTRL> __device__ __forceinline__ void swap_lanes(float &keep, float &give, bool second)
+{
+   const int got = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, second ? keep : give), CTRL, 0xf, 0xf, true);
+   keep = second ? __builtin_bit_cast(float, got) : keep;
+   give = second ? give : __builtin_bit_cast(float, got);
+}
+__device__ __forceinline__ void transpose4(f4 &x, int lane)
+{
+   constexpr int kNeighbour = 0xb1, kOpposite = 0x4e;                // quad_perm [1,0,3,2] and [2,3,0,1]
+   float a = x[0], b = x[1], c = x[2], d = x[3];
+   swap_lanes<kNeighbour>(a, b, lane & 1); swap_lanes<kNeighbour>(c, d, lane & 1);
+   swap_lanes<kOpposite>(a, c, lane & 2); swap_lanes<kOpposite>(b, d, lane & 2);
+   x = f4{a, b, c, d};
 }
 // The A fragment of k^T from rows of k in LDS: 16 columns from c0 on, this lane's 8 rows from row on.  The transposing read hands lane i of 16 the i-th column of the 4 x 16 elements
 // whose rows lanes 4 m .. 4 m + 3 point at.
@@ -391,8 +425,8 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
    const int64_t column = tile * COLS + col;
    const bool there = column < a.value_dim;
    const T *q = (const T *)a.q + stream * a.q_stride[0] + seg.from * a.q_stride[1] + kh * a.q_stride[2], *k = (const T *)a.k + stream * a.k_stride[0] + seg.from * a.k_stride[1] + kh * a.k_stride[2];
-   const T *v = (const T *)a.v + stream * a.v_stride[0] + seg.from * a.v_stride[1] + head * a.v_stride[2] + column;
-   T *o = (T *)a.out + stream * a.out_stride[0] + seg.from * a.out_stride[1] + head * a.out_stride[2] + column;
+   const T *v = (const T *)a.v + stream * a.v_stride[0] + seg.from * a.v_stride[1] + head * a.v_stride[2] + tile * COLS;
+   T *o = (T *)a.out + stream * a.out_stride[0] + seg.from * a.out_stride[1] + head * a.out_stride[2] + tile * COLS;
    const BlockData *data = (const BlockData *)a.workspace + (stream * a.heads + head) * seg.blocks;
    float *state = a.state + stream * a.state_stride + head * a.key_dim * a.value_dim + column;
    f4 S[ST];
@@ -410,8 +444,9 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
    constexpr int PER = 512 / KD, LOADS = 8 / PER;
    const int row0 = 8 * wave + lane / (KD / 8), piece = lane % (KD / 8);
    Raw8<T> xk[LOADS], xq[LOADS];
-   uint32_t xv[4];
-   const T *pv = v + (16 * mt + 4 * l4) * a.v_stride[1] - (there ? 0 : col);
+   // v and out: four columns of one row per lane, turned to one column of four rows (transpose4); a group of columns that ends behind the last is read from further left
+   const int vrow = 16 * mt + 4 * l4 + (l15 & 3), vcol = 16 * nt + (l15 & 12), width = (int)min((int64_t)COLS, a.value_dim - tile * COLS), vback = max(0, vcol + 4 - width);
+   Raw4<T> xv;
    const auto fetch = [&](int b) {                                   // block b's k, q, v; rows behind the last are copies of it
       const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock);
       const int64_t t = (int64_t)b * kBlock;
@@ -421,8 +456,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
          xk[i] = load8(k + row * a.k_stride[1], 8 * piece, kd);
          xq[i] = load8(q + row * a.q_stride[1], 8 * piece, kd);
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) xv[r] = load1(pv + (t + r + min(0, live - 1 - (16 * mt + 4 * l4 + r))) * a.v_stride[1]);
+      xv = load4(v + (t + min(vrow, live - 1)) * a.v_stride[1] + vcol - vback);
    };
    // T, P and the factors of a block are fetched behind the last use of the block before: each has the better part of a block to arrive
    const auto rows4 = [&](const float *f) { return *reinterpret_cast<const f4 *>(f + 16 * mt + 4 * l4); };
@@ -438,11 +472,20 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
    };
    b8 ft[2][3], fp[2][3];
-   f4 c1 = rows4(data->c1), beta = rows4(data->beta), c2 = rows4(data->c2), c3 = rows4(data->c3);
-   float end = data->end[lane & 3];                                  // a vector load: a scalar one would be waited for at the next barrier, with the LDS
-   tiles2(data->t, ft);
-   tiles2(data->p, fp);
+   // the first block's, in the order in which the loop fetches the next one's: the compiler's counts of what is still under way hold for both then
+   const auto in_order = [] { asm volatile("" ::: "memory"); };
+   f4 c1 = rows4(data->c1), beta = rows4(data->beta);
+   in_order();
    fetch(0);
+   in_order();
+   tiles2(data->t, ft);
+   in_order();
+   f4 c3 = rows4(data->c3);
+   float end = data->end[lane & 3];                                  // a vector load: a scalar one would be waited for at the next barrier, with the LDS
+   f4 c2 = rows4(data->c2);
+   in_order();
+   tiles2(data->p, fp);
+   in_order();
    for (int b = 0; b < blocks; ++b) {
       const BlockData &next = data[min(b + 1, blocks - 1)];
       const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock);
@@ -480,12 +523,17 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
          }
          mfma_parts2<NT, 3>(fk, fs, x, fq, fs, y);
       }
-      f4 r;
+      f4 r = values4<T>(xv);
+      if (live < kBlock || width < COLS) r = trim4(r, vrow < live ? vback : 4);
+      transpose4(r, l15);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-         r[i] = beta[i] * (there && 16 * mt + 4 * l4 + i < live ? (float)value1<T>(xv[i]) : 0.0f) - c1[i] * x[i];
-         if (!(fabsf(r[i]) < INFINITY)) { r[i] = 0.0f; atomicMin(&spoison[col], 16 * mt + 4 * l4 + i); }
+         r[i] = beta[i] * r[i] - c1[i] * x[i];
       }
+      if (!(fabsf(r[0]) + fabsf(r[1]) + fabsf(r[2]) + fabsf(r[3]) < INFINITY))
+#pragma unroll
+         for (int i = 3; i >= 0; --i)
+            if (!(fabsf(r[i]) < INFINITY)) { r[i] = 0.0f; atomicMin(&spoison[col], 16 * mt + 4 * l4 + i); }
       c1 = rows4(next.c1); beta = rows4(next.beta);
       fetch(min(b + 1, blocks - 1));
       b4 p[3];
@@ -555,9 +603,16 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
       c2 = rows4(next.c2);
       tiles2(next.p, fp);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-         const int row = 16 * mt + 4 * l4 + i;
-         if (there && row < live) o[((int64_t)b * kBlock + row) * a.out_stride[1]] = (T)(row < poison ? y[i] : NAN);
+      for (int i = 0; i < 4; ++i) y[i] = 16 * mt + 4 * l4 + i < poison ? y[i] : NAN;
+      transpose4(y, l15);
+      if (vrow < live) {
+         T *to = o + ((int64_t)b * kBlock + vrow) * a.out_stride[1] + vcol;
+         const float f[4] = {y[0], y[1], y[2], y[3]};
+         if (!vback) store_f32<T, 4>(to, f);
+         else
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+               if (vcol + i < width) to[i] = (T)f[i];
       }
       dead = dead || poison < kBlock;
    }
@@ -571,8 +626,8 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
 }
 
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
-// Blocks from 16 steps on, for keys of 8 to 128; the workspace holds as many blocks as stay in the last-level cache between the two launches, longer calls go out in segments of steps
-static bool in_blocks(const vadc_amd_gated_delta_args &a) { return a.steps >= 16 && a.key_dim >= 8 && a.key_dim <= 128; }
+// Blocks from 16 steps on, for keys of 8 to 128 and values of 4 and more; the workspace holds as many blocks as stay in the last-level cache between the two launches, longer calls go out in segments of steps
+static bool in_blocks(const vadc_amd_gated_delta_args &a) { return a.steps >= 16 && a.key_dim >= 8 && a.key_dim <= 128 && a.value_dim >= 4; }
 static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
 {
    const int64_t blocks = (a.steps + kBlock - 1) / kBlock, most = std::max<int64_t>(1, 4096 / (a.streams * a.heads));
