@@ -111,7 +111,7 @@ template <typename T, int VEC, int ROWS> static void launch_step(const vadc_amd_
 constexpr int kBlock = 64;
 constexpr int kTiles = 6;                                            // 16 x 32 tiles of a lower triangle: rows 0, 16 need columns 0 .. 31 only
 struct __align__(16) BlockData {
-   b8 t[kTiles][3][64], p[kTiles][3][64];                            // operand order, in three parts: lane (l4, l15) has row l15, columns 4 l4 .. and 16 + 4 l4 .. of the tile
+   p8 t[kTiles][3][64], p[kTiles][3][64];                            // operand order, in three parts: lane (l4, l15) has row l15, columns 4 l4 .. and 16 + 4 l4 .. of the tile
    float c1[kBlock], beta[kBlock], c2[kBlock], c3[kBlock];           // beta a rk, beta, a rq, e^(G_63 - G) rk
    float end[32];                                                    // a_63, four times; the rest keeps the next block on a line of its own
 };
@@ -126,12 +126,12 @@ template <int KD> __device__ __forceinline__ int place(int row, int piece)
    return row * KD + 8 * (piece ^ mix);
 }
 
-// Eight elements of a row from c on, in two halves: the load, which always goes out and is always inside the row (kd >= 8), and, where the value is used, what does not count: elements
-// behind the row's kd, and everything where `keep` is false.  A load under a branch or with its value touched at once would be waited for on the spot.
+// Eight elements of a row from c on, in two halves: the load from min(c, kd - 8), which always goes out and is always inside the row, and, where the value is used, what does not count:
+// elements behind the row's kd, and everything where `keep` is false.  A load under a branch or with its value touched at once would be waited for on the spot.
 template <typename T> struct Raw8 { uint32_t w[2 * sizeof(T)]; };
-template <typename T> __device__ __forceinline__ Raw8<T> load8(const T *row, int c, int kd)
+template <typename T> __device__ __forceinline__ Raw8<T> load8(const T *p)
 {
-   const Pack<uint32_t, 2 * (int)sizeof(T)> u = *reinterpret_cast<const Pack<uint32_t, 2 * (int)sizeof(T)> *>(row + min(c, kd - 8));
+   const Pack<uint32_t, 2 * (int)sizeof(T)> u = *reinterpret_cast<const Pack<uint32_t, 2 * (int)sizeof(T)> *>(p);
    Raw8<T> r;
    __builtin_memcpy(&r, &u, sizeof(r));
    return r;
@@ -166,7 +166,7 @@ template <typename T> __device__ __forceinline__ void trim8(Raw8<T> &r, int c, i
    }
 }
 // its parts, through memory of the value's own type
-template <typename T> __device__ __forceinline__ void split_raw(const Raw8<T> &r, b8 (&p)[Parts<T>::n])
+template <typename T> __device__ __forceinline__ void split_raw(const Raw8<T> &r, p8 (&p)[Parts<T>::n])
 {
    T x[8];
    __builtin_memcpy(x, &r, sizeof(x));
@@ -212,27 +212,27 @@ __device__ __forceinline__ void transpose4(f4 &x, int lane)
 }
 // The A fragment of k^T from rows of k in LDS: 16 columns from c0 on, this lane's 8 rows from row on.  The transposing read hands lane i of 16 the i-th column of the 4 x 16 elements
 // whose rows lanes 4 m .. 4 m + 3 point at.
-template <int KD> __device__ __forceinline__ b8 load_transposed(const __bf16 *rows, int row, int c0, int l15)
+template <int KD> __device__ __forceinline__ p8 load_transposed(const __bf16 *rows, int row, int c0, int l15)
 {
    typedef short s4 __attribute__((ext_vector_type(4)));
    typedef __attribute__((address_space(3))) s4 *lds_s4;
    const int c = c0 + 4 * (l15 & 3);
    const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(rows + place<KD>(row + (l15 >> 2), c >> 3) + (c & 7)));
    const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(rows + place<KD>(row + 4 + (l15 >> 2), c >> 3) + (c & 7)));
-   return __builtin_bit_cast(b8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+   return join(__builtin_bit_cast(p4, lo), __builtin_bit_cast(p4, hi));
 }
 
 // the tiles of rows 16 mt .. from the sixteen-column pieces a lane holds of its row
-__device__ __forceinline__ void store_rows(b8 (&to)[kTiles][3][64], const f4 (&x)[4], int mt, int lane)
+__device__ __forceinline__ void store_rows(p8 (&to)[kTiles][3][64], const f4 (&x)[4], int mt, int lane)
 {
 #pragma unroll
    for (int s = 0; s < 2; ++s)
       if (s == 0 || mt >= 2) {
-         b4 lo[3], hi[3];
+         p4 lo[3], hi[3];
          split4(x[2 * s], lo);
          split4(x[2 * s + 1], hi);
 #pragma unroll
-         for (int n = 0; n < 3; ++n) to[tile_of(mt, s)][n][lane] = __builtin_shufflevector(lo[n], hi[n], 0, 1, 2, 3, 4, 5, 6, 7);
+         for (int n = 0; n < 3; ++n) to[tile_of(mt, s)][n][lane] = join(lo[n], hi[n]);
       }
 }
 
@@ -264,10 +264,10 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
       const int row = tid >> 2;
       const T *from = k + min(row, live - 1) * a.k_stride[1];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) xk[s] = load8(from, 8 * ((tid & 3) + 4 * s), kd);
+      for (int s = 0; s < KS; ++s) xk[s] = load8(from + min(8 * ((tid & 3) + 4 * s), kd - 8));
       const T *fromq = q + min(mine, live - 1) * a.q_stride[1];
 #pragma unroll
-      for (int s = 0; s < KS; ++s) xq[s] = load8(fromq, 32 * s + 8 * l4, kd);
+      for (int s = 0; s < KS; ++s) xq[s] = load8(fromq + min(32 * s + 8 * l4, kd - 8));
    }
    if (wave == 0) {  // G in 64 bits and in powers of two: differences of neighbours far down the block keep their digits.  e^-200 is zero in float32, as e^-inf is
       const int64_t t = t0 + min(lane, live - 1);
@@ -297,10 +297,10 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
          if (odd != 0.0f) xk[s] = Raw8<T>{};                         // NaN: an element is not finite
-         b8 p[NT];
+         p8 p[NT];
          split_raw<T>(xk[s], p);
 #pragma unroll
-         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&sk[n][place<KD>(row, (tid & 3) + 4 * s)]) = p[n];
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<p8 *>(&sk[n][place<KD>(row, (tid & 3) + 4 * s)]) = p[n];
       }
       if ((tid & 3) == 0) srk[row] = a.normalize ? 1.0f / sqrtf((odd != 0.0f ? 1.0f : kk) + 1e-6f) : 1.0f;
       float qq = 0.0f;
@@ -318,12 +318,12 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
    __syncthreads();
    const double gi = sg[mine];
    {
-      b8 fk[KS][NT], fq[KS][NT];
+      p8 fk[KS][NT], fq[KS][NT];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
          split_raw<T>(xq[s], fq[s]);
 #pragma unroll
-         for (int n = 0; n < NT; ++n) fk[s][n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(mine, 4 * s + l4)]);
+         for (int n = 0; n < NT; ++n) fk[s][n] = *reinterpret_cast<const p8 *>(&sk[n][place<KD>(mine, 4 * s + l4)]);
       }
       const float rowk = sbeta[mine] * srk[mine], rowq = srq[mine];
       f4 p[4];
@@ -334,9 +334,9 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
          f4 ck = {0, 0, 0, 0}, cq = {0, 0, 0, 0};
 #pragma unroll
          for (int s = 0; s < KS; ++s) {
-            b8 fa[NT];
+            p8 fa[NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) fa[n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(16 * j + l15, 4 * s + l4)]);
+            for (int n = 0; n < NT; ++n) fa[n] = *reinterpret_cast<const p8 *>(&sk[n][place<KD>(16 * j + l15, 4 * s + l4)]);
             mfma_parts2<NT, NT>(fa, fk[s], ck, fa, fq[s], cq);
          }
 #pragma unroll
@@ -447,20 +447,30 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
    // v and out: four columns of one row per lane, turned to one column of four rows (transpose4); a group of columns that ends behind the last is read from further left
    const int vrow = 16 * mt + 4 * l4 + (l15 & 3), vcol = 16 * nt + (l15 & 12), width = (int)min((int64_t)COLS, a.value_dim - tile * COLS), vback = max(0, vcol + 4 - width);
    Raw4<T> xv;
-   const auto fetch = [&](int b) {                                   // block b's k, q, v; rows behind the last are copies of it
-      const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock);
-      const int64_t t = (int64_t)b * kBlock;
+   int64_t atk[LOADS], atq[LOADS], atv;                              // from a block's first row
+   const auto aim = [&](int live) {                                  // rows behind the last are copies of it
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
-         const int64_t row = t + min(row0 + PER * i, live - 1);
-         xk[i] = load8(k + row * a.k_stride[1], 8 * piece, kd);
-         xq[i] = load8(q + row * a.q_stride[1], 8 * piece, kd);
+         const int64_t row = min(row0 + PER * i, live - 1);
+         atk[i] = row * a.k_stride[1] + min(8 * piece, kd - 8);
+         atq[i] = row * a.q_stride[1] + min(8 * piece, kd - 8);
       }
-      xv = load4(v + (t + min(vrow, live - 1)) * a.v_stride[1] + vcol - vback);
+      atv = min(vrow, live - 1) * a.v_stride[1] + vcol - vback;
+   };
+   aim(kBlock);
+   const auto fetch = [&](int b) {                                   // block b's k, q, v
+      const int64_t t = (int64_t)b * kBlock;
+      if (steps - t < kBlock) aim((int)(steps - t));                 // the last one
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+         xk[i] = load8(k + t * a.k_stride[1] + atk[i]);
+         xq[i] = load8(q + t * a.q_stride[1] + atq[i]);
+      }
+      xv = load4(v + t * a.v_stride[1] + atv);
    };
    // T, P and the factors of a block are fetched behind the last use of the block before: each has the better part of a block to arrive
    const auto rows4 = [&](const float *f) { return *reinterpret_cast<const f4 *>(f + 16 * mt + 4 * l4); };
-   const auto tiles2 = [&](const b8 (&from)[kTiles][3][64], b8 (&to)[2][3]) {
+   const auto tiles2 = [&](const p8 (&from)[kTiles][3][64], p8 (&to)[2][3]) {
 #pragma unroll
       for (int n = 0; n < 3; ++n) {
          to[0][n] = from[tile_of(mt, 0)][n][lane];
@@ -468,10 +478,10 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
       }
    };
    const auto rows8 = [&](const __bf16 *from, int s) {                // of this lane's column, in the order of T's and P's columns
-      const b4 lo = *reinterpret_cast<const b4 *>(from + place<kBlock>(col, 4 * s + (l4 >> 1)) + 4 * (l4 & 1)), hi = *reinterpret_cast<const b4 *>(from + place<kBlock>(col, 4 * s + 2 + (l4 >> 1)) + 4 * (l4 & 1));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      const p4 lo = *reinterpret_cast<const p4 *>(from + place<kBlock>(col, 4 * s + (l4 >> 1)) + 4 * (l4 & 1)), hi = *reinterpret_cast<const p4 *>(from + place<kBlock>(col, 4 * s + 2 + (l4 >> 1)) + 4 * (l4 & 1));
+      return join(lo, hi);
    };
-   b8 ft[2][3], fp[2][3];
+   p8 ft[2][3], fp[2][3];
    // the first block's, in the order in which the loop fetches the next one's: the compiler's counts of what is still under way hold for both then
    const auto in_order = [] { asm volatile("" ::: "memory"); };
    f4 c1 = rows4(data->c1), beta = rows4(data->beta);
@@ -492,34 +502,34 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
       const bool partial = live < kBlock || kd < KD;
 #pragma unroll
       for (int i = 0; i < ST; ++i) {
-         b4 p[3];
+         p4 p[3];
          split4(S[i], p);
 #pragma unroll
-         for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&ss[n][place<KD>(col, 8 * i + 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+         for (int n = 0; n < 3; ++n) *reinterpret_cast<p4 *>(&ss[n][place<KD>(col, 8 * i + 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
       }
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
          const int row = row0 + PER * i;
          if (partial) { trim8<T>(xk[i], 8 * piece, kd, row < live); trim8<T>(xq[i], 8 * piece, kd, row < live); }
-         b8 p[NT];
+         p8 p[NT];
          split_raw<T>(xk[i], p);
 #pragma unroll
-         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&sk[n][place<KD>(row, piece)]) = p[n];
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<p8 *>(&sk[n][place<KD>(row, piece)]) = p[n];
          split_raw<T>(xq[i], p);
 #pragma unroll
-         for (int n = 0; n < NT; ++n) *reinterpret_cast<b8 *>(&sq[n][place<KD>(row, piece)]) = p[n];
+         for (int n = 0; n < NT; ++n) *reinterpret_cast<p8 *>(&sq[n][place<KD>(row, piece)]) = p[n];
       }
       lds_barrier();
       f4 x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-         b8 fs[3], fk[NT], fq[NT];
+         p8 fs[3], fk[NT], fq[NT];
 #pragma unroll
-         for (int n = 0; n < 3; ++n) fs[n] = *reinterpret_cast<const b8 *>(&ss[n][place<KD>(col, 4 * s + l4)]);
+         for (int n = 0; n < 3; ++n) fs[n] = *reinterpret_cast<const p8 *>(&ss[n][place<KD>(col, 4 * s + l4)]);
 #pragma unroll
          for (int n = 0; n < NT; ++n) {
-            fk[n] = *reinterpret_cast<const b8 *>(&sk[n][place<KD>(16 * mt + l15, 4 * s + l4)]);
-            fq[n] = *reinterpret_cast<const b8 *>(&sq[n][place<KD>(16 * mt + l15, 4 * s + l4)]);
+            fk[n] = *reinterpret_cast<const p8 *>(&sk[n][place<KD>(16 * mt + l15, 4 * s + l4)]);
+            fq[n] = *reinterpret_cast<const p8 *>(&sq[n][place<KD>(16 * mt + l15, 4 * s + l4)]);
          }
          mfma_parts2<NT, 3>(fk, fs, x, fq, fs, y);
       }
@@ -536,15 +546,15 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
             if (!(fabsf(r[i]) < INFINITY)) { r[i] = 0.0f; atomicMin(&spoison[col], 16 * mt + 4 * l4 + i); }
       c1 = rows4(next.c1); beta = rows4(next.beta);
       fetch(min(b + 1, blocks - 1));
-      b4 p[3];
+      p4 p[3];
       split4(r, p);
 #pragma unroll
-      for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&sr[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+      for (int n = 0; n < 3; ++n) *reinterpret_cast<p4 *>(&sr[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
       lds_barrier();
       const int poison = dead ? 0 : spoison[col];
       f4 u = {0, 0, 0, 0};
       {
-         b8 f[2][3];
+         p8 f[2][3];
 #pragma unroll
          for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -556,7 +566,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
          } else u = mfma_parts<3, 3>(ft[0], f[0], u);
       }
       tiles2(next.t, ft);
-      b8 kt[2][ST][NT];                                              // k^T, before the next block's k may take its place
+      p8 kt[2][ST][NT];                                              // k^T, before the next block's k may take its place
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -565,19 +575,19 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
             for (int n = 0; n < NT; ++n) kt[s][i][n] = load_transposed<KD>(sk[n], 32 * s + 8 * l4, 64 * i + 16 * mt, l15);
       split4(u, p);
 #pragma unroll
-      for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&su[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+      for (int n = 0; n < 3; ++n) *reinterpret_cast<p4 *>(&su[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
       split4(c3 * u, p);
 #pragma unroll
-      for (int n = 0; n < 3; ++n) *reinterpret_cast<b4 *>(&sw[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+      for (int n = 0; n < 3; ++n) *reinterpret_cast<p4 *>(&sw[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
       lds_barrier();
       if (tid < COLS) spoison[tid] = kBlock;
       c3 = rows4(next.c3);
       {  // two chains of products at a time: the rows of S this wave holds, or one of them beside the outputs
-         b8 fw[2][3];
+         p8 fw[2][3];
 #pragma unroll
          for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int n = 0; n < 3; ++n) fw[s][n] = *reinterpret_cast<const b8 *>(&sw[n][place<kBlock>(col, 4 * s + l4)]);
+            for (int n = 0; n < 3; ++n) fw[s][n] = *reinterpret_cast<const p8 *>(&sw[n][place<kBlock>(col, 4 * s + l4)]);
 #pragma unroll
          for (int i = 0; i < ST; ++i) S[i] *= end;
          end = next.end[lane & 3];
@@ -588,7 +598,7 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
          }
       }
       {
-         b8 f[2][3];
+         p8 f[2][3];
 #pragma unroll
          for (int s = 0; s < 2; ++s)
 #pragma unroll

@@ -46,7 +46,7 @@ template <typename T> struct Tile { static constexpr int k = 128 / (int)sizeof(T
 template <typename T> struct Frag;
 template <> struct Frag<__bf16> { b8 v; };
 template <> struct Frag<_Float16> { h8 v; };
-template <> struct Frag<float> { b8 p[3]; };
+template <> struct Frag<float> { p8 p[3]; };
 template <typename T> __device__ __forceinline__ Frag<T> load_frag(const char *tile, int row, int step, int half)
 {
    Frag<T> f;
@@ -65,7 +65,7 @@ __device__ __forceinline__ f16v product(const Frag<float> &a, const Frag<float> 
 #pragma unroll
    for (int o = 2; o >= 0; --o)
 #pragma unroll
-      for (int i = 0; i <= o; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.p[i], b.p[o - i], c, 0, 0, 0);
+      for (int i = 0; i <= o; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a.p[i]), __builtin_bit_cast(b8, b.p[o - i]), c, 0, 0, 0);
    return c;
 }
 

@@ -51,50 +51,61 @@ template <typename T> struct Parts;
 template <> struct Parts<__bf16> { static constexpr int n = 1; };
 template <> struct Parts<_Float16> { static constexpr int n = 2; };
 template <> struct Parts<float> { static constexpr int n = 3; };
-template <typename T> __device__ __forceinline__ void split8(const T (&x)[8], b8 (&p)[Parts<T>::n])
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+typedef u4 p8;                                                       // eight values' one part: an operand.  In whole words: the compiler takes vectors of 16 bits apart
+typedef u2 p4;
+// the next part of two values, packed, taken off them
+__device__ __forceinline__ uint32_t next_part(f2 &rest)
+{
+   const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, b2));
+   rest[0] -= __builtin_bit_cast(float, w << 16);
+   rest[1] -= __builtin_bit_cast(float, w & 0xffff0000u);
+   return w;
+}
+template <typename T> __device__ __forceinline__ void split8(const T (&x)[8], p8 (&p)[Parts<T>::n])
 {
    if constexpr (Parts<T>::n == 1) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) p[0][i] = x[i];
+      __builtin_memcpy(&p[0], x, sizeof(p8));
    } else {
-      float rest[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) rest[i] = (float)x[i];
+      for (int i = 0; i < 4; ++i) {
+         f2 rest = {(float)x[2 * i], (float)x[2 * i + 1]};
 #pragma unroll
-      for (int k = 0; k < Parts<T>::n; ++k)
-#pragma unroll
-         for (int i = 0; i < 8; ++i) { p[k][i] = (__bf16)rest[i]; rest[i] -= (float)p[k][i]; }
+         for (int k = 0; k < Parts<T>::n; ++k) p[k][i] = next_part(rest);
+      }
    }
 }
-typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ void split4(const f4 &x, b4 (&p)[3])
+__device__ __forceinline__ void split4(const f4 &x, p4 (&p)[3])
 {
-   f4 rest = x;
+   f2 lo = {x[0], x[1]}, hi = {x[2], x[3]};
 #pragma unroll
-   for (int k = 0; k < 3; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { p[k][i] = (__bf16)rest[i]; rest[i] -= (float)p[k][i]; }
+   for (int k = 0; k < 3; ++k) p[k] = p4{next_part(lo), next_part(hi)};
 }
+__device__ __forceinline__ p8 join(const p4 &lo, const p4 &hi) { return p8{lo[0], lo[1], hi[0], hi[1]}; }
+__device__ __forceinline__ f4 mfma16(const p8 &a, const p8 &b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0); }
 // acc += a . b over 32 k's, operands in NA and NB parts: the small products first
-template <int NA, int NB> __device__ __forceinline__ f4 mfma_parts(const b8 (&a)[NA], const b8 (&b)[NB], f4 acc)
+template <int NA, int NB> __device__ __forceinline__ f4 mfma_parts(const p8 (&a)[NA], const p8 (&b)[NB], f4 acc)
 {
 #pragma unroll
    for (int o = 2; o >= 0; --o)
 #pragma unroll
       for (int i = 0; i < NA; ++i)
-         if (o - i >= 0 && o - i < NB) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[o - i], acc, 0, 0, 0);
+         if (o - i >= 0 && o - i < NB) acc = mfma16(a[i], b[o - i], acc);
    return acc;
 }
 // two of them at once, product by product: the matrix pipe has the other's while one's result is under way
-template <int NA, int NB> __device__ __forceinline__ void mfma_parts2(const b8 (&a)[NA], const b8 (&b)[NB], f4 &x, const b8 (&c)[NA], const b8 (&d)[NB], f4 &y)
+template <int NA, int NB> __device__ __forceinline__ void mfma_parts2(const p8 (&a)[NA], const p8 (&b)[NB], f4 &x, const p8 (&c)[NA], const p8 (&d)[NB], f4 &y)
 {
 #pragma unroll
    for (int o = 2; o >= 0; --o)
 #pragma unroll
       for (int i = 0; i < NA; ++i)
          if (o - i >= 0 && o - i < NB) {
-            x = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[o - i], x, 0, 0, 0);
-            y = __builtin_amdgcn_mfma_f32_16x16x32_bf16(c[i], d[o - i], y, 0, 0, 0);
+            x = mfma16(a[i], b[o - i], x);
+            y = mfma16(c[i], d[o - i], y);
          }
 }
 
