@@ -404,13 +404,13 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
    }
 }
 
-// A workgroup of eight waves walks the blocks of one stream and head with 32 columns of S: wave (mt, nt) does rows 16 mt .. of the block's products and rows 16 mt .., 16 mt + 64 .. of S,
+// A workgroup of four or eight waves walks the blocks of one stream and head with 16 or 32 columns of S: wave (mt, nt) does rows 16 mt .. of the block's products and rows 16 mt .., 16 mt + 64 .. of S,
 // columns 16 nt ...  k and q go through registers into LDS in their parts, a block ahead, each row read once as a run; T and P come from global memory in operand order; S, r, u and the
 // scaled u pass through LDS in three parts, written as four consecutive k's from the accumulators; k^T is k's rows through the transposing LDS read.  Three barriers a block.
-template <typename T, int KD>
-__global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_args a, const Segment seg)
+template <typename T, int KD, int COLS>
+__global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_delta_args a, const Segment seg)
 {
-   constexpr int NT = Parts<T>::n, KS = KD / 32, ST = KD / 64, COLS = 32;
+   constexpr int NT = Parts<T>::n, KS = KD / 32, ST = KD / 64, WAVES = COLS / 4;
    __shared__ __attribute__((aligned(16))) __bf16 sk[NT][kBlock * KD], sq[NT][kBlock * KD], ss[3][COLS * KD], sr[3][COLS * kBlock], su[3][COLS * kBlock], sw[3][COLS * kBlock];
    __shared__ int spoison[COLS];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, l4 = lane >> 4, mt = wave & 3, nt = wave >> 2;
@@ -440,9 +440,9 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
    if (tid < COLS) spoison[tid] = kBlock;
    bool dead = false;
 
-   // this lane's part of the wave's eight rows of k and q: one piece of eight columns in every PER-th row from row0 on
-   constexpr int PER = 512 / KD, LOADS = 8 / PER;
-   const int row0 = 8 * wave + lane / (KD / 8), piece = lane % (KD / 8);
+   // this lane's part of the wave's rows of k and q: one piece of eight columns in every PER-th row from row0 on
+   constexpr int PER = 512 / KD, LOADS = kBlock / WAVES / PER;
+   const int row0 = kBlock / WAVES * wave + lane / (KD / 8), piece = lane % (KD / 8);
    Raw8<T> xk[LOADS], xq[LOADS];
    // v and out: four columns of one row per lane, turned to one column of four rows (transpose4); a group of columns that ends behind the last is read from further left
    const int vrow = 16 * mt + 4 * l4 + (l15 & 3), vcol = 16 * nt + (l15 & 12), width = (int)min((int64_t)COLS, a.value_dim - tile * COLS), vback = max(0, vcol + 4 - width);
@@ -638,6 +638,10 @@ __global__ __launch_bounds__(512) void k_delta_scan(const vadc_amd_gated_delta_a
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
 // Blocks from 16 steps on, for keys of 8 to 128 and values of 4 and more; the workspace holds as many blocks as stay in the last-level cache between the two launches, longer calls go out in segments of steps
 static bool in_blocks(const vadc_amd_gated_delta_args &a) { return a.steps >= 16 && a.key_dim >= 8 && a.key_dim <= 128 && a.value_dim >= 4; }
+// Columns of S per workgroup: with keys of up to 64, 16 -- several workgroups a CU, one computes while another waits at its barriers (61 streams of up to 333 steps, 6 heads of 48 x 80,
+// float32: 70.6 us a launch against 81.3 with 32) --; with longer keys, where staging k and q again for every 16 columns costs more than that gains, 32 (2 x 4096 steps, 32 heads of
+// 128 x 128, bfloat16: 244 us against 269 with 16)
+template <int KD> constexpr int scan_columns() { return KD == 64 ? 16 : 32; }
 static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
 {
    const int64_t blocks = (a.steps + kBlock - 1) / kBlock, most = std::max<int64_t>(1, 4096 / (a.streams * a.heads));
@@ -645,11 +649,12 @@ static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
 }
 template <typename T, int KD> static void launch_blocks(const vadc_amd_gated_delta_args &a, hipStream_t s)
 {
-   const int64_t step = segment_blocks(a), tiles = (a.value_dim + 31) / 32;
+   constexpr int cols = scan_columns<KD>();
+   const int64_t step = segment_blocks(a), tiles = (a.value_dim + cols - 1) / cols;
    for (Segment seg = {0, 0}; seg.from < a.steps; seg.from += step * kBlock) {
       seg.blocks = std::min(step, (a.steps - seg.from + kBlock - 1) / kBlock);
       hipLaunchKernelGGL((k_delta_blocks<T, KD>), dim3((unsigned)(a.streams * a.heads * seg.blocks)), dim3(256), 0, s, a, seg);
-      hipLaunchKernelGGL((k_delta_scan<T, KD>), dim3((unsigned)(a.streams * a.heads * tiles)), dim3(512), 0, s, a, seg);
+      hipLaunchKernelGGL((k_delta_scan<T, KD, cols>), dim3((unsigned)(a.streams * a.heads * tiles)), dim3(16 * cols), 0, s, a, seg);
    }
 }
 
