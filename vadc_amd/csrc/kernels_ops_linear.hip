@@ -9,33 +9,49 @@ namespace ops {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
-// The epilogue of 4 consecutive output features of one row: bias, residual, activation in float32, one rounding at the end.
-template <typename T>
-__device__ __forceinline__ void finish4(const vadc_amd_linear_args &a, int64_t row, int64_t col, const f4 &acc)
+// The epilogue of N consecutive output features of one row: bias, residual, activation in float32, one rounding at the end.  `left` features are left in the row.
+template <typename T, int N> __device__ __forceinline__ void load_bias(const vadc_amd_linear_args &a, int64_t col, float (&b)[N])
+{
+#pragma unroll
+   for (int i = 0; i < N; ++i) b[i] = 0.0f;
+   const int64_t left = a.out_features - col;
+   if (!a.bias || left <= 0) return;
+   const T *bias = (const T *)a.bias + col;
+   if (left >= N) load_f32<T, N>(bias, b);
+   else
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+         if (i < left) b[i] = (float)bias[i];
+}
+template <typename T, int N>
+__device__ __forceinline__ void finish(const vadc_amd_linear_args &a, int64_t row, int64_t col, float (&y)[N], const float (&b)[N])
 {
    const int64_t left = a.out_features - col;
    if (row >= a.rows || left <= 0) return;
-   const T *bias = (const T *)a.bias, *res = (const T *)a.residual + row * a.residual_stride;
-   T *out = (T *)a.out + row * a.out_stride;
-   float y[4] = {acc[0], acc[1], acc[2], acc[3]}, b[4] = {0, 0, 0, 0}, r[4] = {0, 0, 0, 0};
-   if (left >= 4) {
-      if (a.bias) load_f32<T, 4>(bias + col, b);
-      if (a.residual) load_f32<T, 4>(res + col, r);
-   } else {
-      for (int i = 0; i < left; ++i) {
-         if (a.bias) b[i] = (float)bias[col + i];
-         if (a.residual) r[i] = (float)res[col + i];
-      }
-   }
+   const T *res = (const T *)a.residual + row * a.residual_stride + col;
+   T *out = (T *)a.out + row * a.out_stride + col;
+   float r[N];
 #pragma unroll
-   for (int i = 0; i < 4; ++i) {
-      y[i] += b[i];
-      if (a.residual && a.residual_first) y[i] += r[i];
-      y[i] = activate(y[i], a.activation);
-      if (a.residual && !a.residual_first) y[i] += r[i];
+   for (int i = 0; i < N; ++i) { r[i] = 0.0f; y[i] += b[i]; }
+   if (a.residual) {
+      if (left >= N) load_f32<T, N>(res, r);
+      else
+#pragma unroll
+         for (int i = 0; i < N; ++i)
+            if (i < left) r[i] = (float)res[i];
+      if (a.residual_first)
+#pragma unroll
+         for (int i = 0; i < N; ++i) y[i] += r[i];
    }
-   if (left >= 4) store_f32<T, 4>(out + col, y);
-   else for (int i = 0; i < left; ++i) out[col + i] = (T)y[i];
+   activate_all<N>(y, a.activation);
+   if (a.residual && !a.residual_first)
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] += r[i];
+   if (left >= N) store_f32<T, N>(out, y);
+   else
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+         if (i < left) out[i] = (T)y[i];
 }
 
 // ---- operands in LDS: rows of 128 bytes (KT elements of k), eight 16-byte pieces, the piece index mixed with the row so that the rows of a fragment lie in different banks
@@ -75,6 +91,13 @@ __device__ __forceinline__ void dma(uint32_t lds, uint32_t offset, const void *b
 {
    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" :: "s"(lds), "v"(offset), "s"(base) : "memory");
 }
+// the same for all lanes, and the compiler may know: a scalar register
+__device__ __forceinline__ const void *uniform(const void *p)
+{
+   const uint64_t v = (uint64_t)(uintptr_t)p;
+   const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+   return (const void *)(uintptr_t)((uint64_t)hi << 32 | lo);
+}
 template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
 // BM rows x BN features per workgroup, WR x WC waves of (BM / WR) x (BN / WC) outputs in 32 x 32 tiles.  The weight is the A operand: a lane's accumulators are groups of four
@@ -85,6 +108,7 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_tile(const vadc_amd_lin
 {
    constexpr int WAVES = WR * WC, KT = Tile<T>::k, TM = BM / WR / 32, TN = BN / WC / 32, BYTES = (BM + BN) * 128, PIECES = (BM + BN) / 8 / WAVES;
    static_assert((BM + BN) / 8 % WAVES == 0 && (BM / 8) % PIECES == 0, "a wave's pieces lie in one operand");
+   static_assert(STAGES * BYTES >= WAVES * 32 * (BN / WC) * 4, "the epilogue's part of LDS");
    __shared__ __attribute__((aligned(16))) char lds[STAGES * BYTES];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
    const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.out_features + BN - 1) / BN;
@@ -117,8 +141,9 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_tile(const vadc_amd_lin
       for (int p = 0; p < PIECES; ++p) offset[p] = (uint32_t)(row_of(p) * (int)(stride * sizeof(T)) + 16 * piece_of(p));
    const auto issue = [&](int64_t kt) {
       const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (uint32_t)(kt % STAGES) * BYTES + wave * PIECES * 1024;
+      const void *from = uniform(src + kt * KT);
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) dma(to + p * 1024, offset[p], src + kt * KT);
+      for (int p = 0; p < PIECES; ++p) dma(to + p * 1024, offset[p], from);
    };
    T held[DMA ? 1 : PIECES][16 / sizeof(T)];
    constexpr int PER = 16 / (int)sizeof(T);
@@ -216,14 +241,29 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_tile(const vadc_amd_lin
          }
       }
    }
+   // Out through LDS, 32 rows of the wave's features at a time in float32, so that a row's features leave (and its residuals come) as one run, eight to a lane: a lane's own accumulators lie
+   // in pieces of four features of 32 different rows (8192 x 4096 x 4096 bfloat16 with a residual: 340 us with stores straight from them, EPILOGUE us so)
+   lds_barrier();                                                     // everybody has read the last tile
+   constexpr int FEATS = BN / WC, PP = FEATS / 4, LPR = FEATS / 8, RPI = 64 / LPR;
+   f4 *mine = reinterpret_cast<f4 *>(lds) + wave * 32 * PP;
+   const auto slot = [&](int row, int piece) { return row * PP + (piece ^ (PP == 8 ? (row >> 1) & 7 : row & (PP - 1))); };
+   const int64_t col = col0 + wc + 8 * (lane % LPR);
+   float bias[8];
+   load_bias<T, 8>(a, col, bias);
 #pragma unroll
-   for (int j = 0; j < TM; ++j)
+   for (int j = 0; j < TM; ++j) {
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll
-         for (int g = 0; g < 4; ++g)
-            finish4<T>(a, row0 + wr + 32 * j + (lane & 31), col0 + wc + 32 * i + 8 * g + 4 * (lane >> 5),
-                       f4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]});
+         for (int g = 0; g < 4; ++g) mine[slot(lane & 31, 8 * i + 2 * g + (lane >> 5))] = f4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
+#pragma unroll
+      for (int k = 0; k < 32 / RPI; ++k) {
+         const int row = k * RPI + lane / LPR;
+         const f4 lo = mine[slot(row, 2 * (lane % LPR))], hi = mine[slot(row, 2 * (lane % LPR) + 1)];
+         float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+         finish<T, 8>(a, row0 + wr + 32 * j + row, col, y, bias);
+      }
+   }
 }
 
 // ---- few rows: the weight goes once through registers, nothing is shared -------------------------------------------------------------------------------
@@ -281,7 +321,9 @@ __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_arg
       f4 sum = part[0][j][lane];
 #pragma unroll
       for (int w = 1; w < WAVES; ++w) sum += part[w][j][lane];
-      finish4<T>(a, row0 + 16 * j + l15, col0 + 4 * l4, sum);
+      float y[4] = {sum[0], sum[1], sum[2], sum[3]}, bias[4];
+      load_bias<T, 4>(a, col0 + 4 * l4, bias);
+      finish<T, 4>(a, row0 + 16 * j + l15, col0 + 4 * l4, y, bias);
    }
 }
 

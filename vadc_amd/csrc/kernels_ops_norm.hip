@@ -41,10 +41,12 @@ __device__ __forceinline__ void apply(const vadc_amd_group_norm_args &a, const f
    float y[VEC], g[VEC];
    if (a.gate) load_f32<T, VEC>(gate, g);
 #pragma unroll
-   for (int i = 0; i < VEC; ++i) {
-      y[i] = fmaf((x[i] - mean) * rstd, w[i], b[i]);
-      y[i] = a.gate ? y[i] * activate(g[i], a.activation) : activate(y[i], a.activation);
-   }
+   for (int i = 0; i < VEC; ++i) y[i] = fmaf((x[i] - mean) * rstd, w[i], b[i]);
+   if (a.gate) {
+      activate_all<VEC>(g, a.activation);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) y[i] *= g[i];
+   } else activate_all<VEC>(y, a.activation);
    store_f32<T, VEC>(out, y);
 }
 template <typename T, int VEC>

@@ -28,6 +28,24 @@ __device__ __forceinline__ float activate(float y, int act)
    }
 }
 
+template <int N> __device__ __forceinline__ void activate_all(float (&y)[N], int act)      // one branch for all
+{
+   if (act == kActNone) return;
+   if (act == kActRelu) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = activate(y[i], kActRelu);
+   } else if (act == kActSilu) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = activate(y[i], kActSilu);
+   } else if (act == kActGelu) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = activate(y[i], kActGelu);
+   } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = activate(y[i], kActSigmoid);
+   }
+}
+
 // N consecutive elements; the pointer needs the element's alignment only (gfx950 serves unaligned vector accesses; an aligned address costs no more)
 template <typename T, int N> struct __attribute__((packed)) Pack { T v[N]; };
 template <typename T, int N> __device__ __forceinline__ void load_f32(const T *p, float (&f)[N])
