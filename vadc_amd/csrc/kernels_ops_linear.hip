@@ -100,53 +100,52 @@ __device__ __forceinline__ const void *uniform(const void *p)
 }
 template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
-// BM rows x BN features per workgroup, WR x WC waves of (BM / WR) x (BN / WC) outputs in 32 x 32 tiles.  The weight is the A operand: a lane's accumulators are groups of four
-// consecutive features of one row.  STAGES tiles of k are in LDS or on their way there: with DMA (16-byte aligned rows) a wave waits for the oldest with a counted vmcnt -- an operation
-// the count does not know of can only make it wait longer -- and one barrier a tile lets everybody read it and the next one overwrite the last; without, tiles pass through registers.
+// BM rows x BN features per tile, WR x WC waves of (BM / WR) x (BN / WC) outputs in 32 x 32 tiles.  The weight is the A operand: a lane's accumulators are groups of four consecutive
+// features of one row.  STAGES tiles of k are in LDS or on their way there: with DMA (16-byte aligned rows) a wave waits for the oldest with a counted vmcnt -- an operation the count does
+// not know of can only make it wait longer -- and one barrier a tile lets everybody read it and the next one overwrite the last; without, tiles pass through registers.
+// A workgroup does every gridDim-th output tile; the next one's first tiles of k are fetched before this one's outputs leave, which takes as long as a few tiles of k.
+// Outputs leave through LDS, 32 rows of up to 64 of the wave's features at a time in float32, so that a row's features leave (and its residuals come) as one run, eight to a lane: a
+// lane's own accumulators lie in pieces of four features of 32 different rows (8192 x 4096 x 4096 bfloat16 with a residual: 340 us with stores straight from them, 260 us so).
 template <typename T, int BM, int BN, int WR, int WC, int STAGES, bool DMA>
-__global__ __launch_bounds__(64 * WR * WC) void k_linear_tile(const vadc_amd_linear_args a)
+__global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_tile(const vadc_amd_linear_args a)
 {
-   constexpr int WAVES = WR * WC, KT = Tile<T>::k, TM = BM / WR / 32, TN = BN / WC / 32, BYTES = (BM + BN) * 128, PIECES = (BM + BN) / 8 / WAVES;
+   constexpr int WAVES = WR * WC, KT = Tile<T>::k, TM = BM / WR / 32, TN = BN / WC / 32, BYTES = (BM + BN) * 128, PIECES = (BM + BN) / 8 / WAVES, PER = 16 / (int)sizeof(T);
    static_assert((BM + BN) / 8 % WAVES == 0 && (BM / 8) % PIECES == 0, "a wave's pieces lie in one operand");
-   static_assert(STAGES * BYTES >= WAVES * 32 * (BN / WC) * 4, "the epilogue's part of LDS");
    __shared__ __attribute__((aligned(16))) char lds[STAGES * BYTES];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
    const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.out_features + BN - 1) / BN;
-   // launch order -> tile: the workgroups of one XCD (every eighth) take consecutive tiles, which go down eight row tiles before the next feature tile: their operands stay in its L2
-   int64_t id;
-   {
-      const unsigned n = (unsigned)(tiles_m * tiles_n), x = blockIdx.x % 8, q = n / 8, r = n % 8;
-      id = (int64_t)(x * q + min(x, r) + blockIdx.x / 8);
-   }
-   const int64_t group = id / (8 * tiles_n), first = group * 8, high = min((int64_t)8, tiles_m - first), in = id - group * 8 * tiles_n;
-   const int64_t row0 = (first + in % high) * BM, col0 = (in / high) * BN;
+   const unsigned tiles = (unsigned)(tiles_m * tiles_n);
    const int wr = wave % WR * (BM / WR), wc = wave / WR * (BN / WC);
-   f16v acc[TN][TM];
-#pragma unroll
-   for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int j = 0; j < TM; ++j) acc[i][j] = (f16v)(0.0f);
+   const int64_t whole = a.in_features / KT;                          // full tiles of k
 
    // this wave's pieces of eight LDS rows: rows 8 PIECES wave .. of x's tile, then of the weight's
    const bool of_x = wave * PIECES < BM / 8;
-   const int64_t stride = of_x ? a.x_stride : a.weight_stride, top = of_x ? row0 : col0, last = (of_x ? a.rows : a.out_features) - 1;
-   const T *src = (const T *)(of_x ? a.x : a.weight) + top * stride;
    const int at = wave * PIECES * 8 - (of_x ? 0 : BM);                // first row in its operand
-   const auto row_of = [&](int p) { return (int)min((int64_t)(at + 8 * p + (lane >> 3)), last - top); };      // rows behind the last are copies of it: their outputs are dropped
-   const auto piece_of = [&](int p) { return (lane & 7) ^ (((at + 8 * p + (lane >> 3)) >> 1) & 7); };
-   const int64_t whole = a.in_features / KT;                          // full tiles of k
+   const int64_t stride = of_x ? a.x_stride : a.weight_stride;
+   int64_t row0, col0, last;
+   const T *src;
    uint32_t offset[PIECES];
-   if constexpr (DMA)
+   const auto row_of = [&](int p) { return (int)min((int64_t)(at + 8 * p + (lane >> 3)), last); };      // rows behind the last are copies of it: their outputs are dropped
+   const auto piece_of = [&](int p) { return (lane & 7) ^ (((at + 8 * p + (lane >> 3)) >> 1) & 7); };
+   const auto aim = [&](unsigned index) {
+      // launch order -> tile: the workgroups of one XCD (every eighth) take consecutive tiles, which go down eight row tiles before the next feature tile: their operands stay in its L2
+      const unsigned x = index % 8, q = tiles / 8, r = tiles % 8;
+      const int64_t id = x * q + min(x, r) + index / 8, group = id / (8 * tiles_n), first = group * 8, high = min((int64_t)8, tiles_m - first), in = id - group * 8 * tiles_n;
+      row0 = (first + in % high) * BM;
+      col0 = in / high * BN;
+      const int64_t top = of_x ? row0 : col0;
+      last = (of_x ? a.rows : a.out_features) - 1 - top;
+      src = (const T *)(of_x ? a.x : a.weight) + top * stride;
+      if constexpr (DMA)
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) offset[p] = (uint32_t)(row_of(p) * (int)(stride * sizeof(T)) + 16 * piece_of(p));
-   const auto issue = [&](int64_t kt) {
-      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (uint32_t)(kt % STAGES) * BYTES + wave * PIECES * 1024;
+         for (int p = 0; p < PIECES; ++p) offset[p] = (uint32_t)(row_of(p) * (int)(stride * sizeof(T)) + 16 * piece_of(p));
+   };
+   const auto issue = [&](int64_t kt, int stage) {
+      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (uint32_t)stage * BYTES + wave * PIECES * 1024;
       const void *from = uniform(src + kt * KT);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) dma(to + p * 1024, offset[p], from);
    };
-   T held[DMA ? 1 : PIECES][16 / sizeof(T)];
-   constexpr int PER = 16 / (int)sizeof(T);
    const auto fetch = [&](int64_t kt, auto &h) {                      // through registers: any alignment, zeros behind the last k
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
@@ -163,13 +162,9 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_tile(const vadc_amd_lin
    };
    const auto place = [&](int stage, const auto &h) {
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) {
-         Pack<T, PER> u;
-#pragma unroll
-         for (int i = 0; i < PER; ++i) u.v[i] = h[p][i];
-         __builtin_memcpy(__builtin_assume_aligned(lds + stage * BYTES + (wave * PIECES + p) * 1024 + lane * 16, 16), &u, 16);
-      }
+      for (int p = 0; p < PIECES; ++p) __builtin_memcpy(__builtin_assume_aligned(lds + stage * BYTES + (wave * PIECES + p) * 1024 + lane * 16, 16), &h[p], 16);
    };
+   f16v acc[TN][TM];
    const auto compute = [&](int stage) {
       const char *sx = lds + stage * BYTES, *sw = sx + BM * 128;
 #pragma unroll
@@ -185,84 +180,112 @@ __global__ __launch_bounds__(64 * WR * WC) void k_linear_tile(const vadc_amd_lin
             for (int j = 0; j < TM; ++j) acc[i][j] = product(fa[i], fb[j], acc[i][j]);
       }
    };
+   constexpr int FEATS = BN / WC < 64 ? BN / WC : 64, PP = FEATS / 4, LPR = FEATS / 8, RPI = 64 / LPR;
+   static_assert(BYTES >= WAVES * 32 * FEATS * 4, "the outputs leave through one stage");
+   const auto leave = [&](int stage, int64_t row0, int64_t col0) {
+      f4 *mine = reinterpret_cast<f4 *>(lds + stage * BYTES) + wave * 32 * PP;
+      const auto slot = [&](int row, int piece) { return row * PP + (piece ^ (PP == 8 ? (row >> 1) & 7 : row & (PP - 1))); };
+#pragma unroll
+      for (int h = 0; h < TN * 32 / FEATS; ++h) {
+         const int64_t col = col0 + wc + h * FEATS + 8 * (lane % LPR);
+         float bias[8];
+         load_bias<T, 8>(a, col, bias);
+#pragma unroll
+         for (int j = 0; j < TM; ++j) {
+#pragma unroll
+            for (int i = 0; i < FEATS / 32; ++i)
+#pragma unroll
+               for (int g = 0; g < 4; ++g) {
+                  const f16v &c = acc[h * (FEATS / 32) + i][j];
+                  mine[slot(lane & 31, 8 * i + 2 * g + (lane >> 5))] = f4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
+               }
+#pragma unroll
+            for (int k = 0; k < 32 / RPI; ++k) {
+               const int row = k * RPI + lane / LPR;
+               const f4 lo = mine[slot(row, 2 * (lane % LPR))], hi = mine[slot(row, 2 * (lane % LPR) + 1)];
+               float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+               finish<T, 8>(a, row0 + wr + 32 * j + row, col, y, bias);
+            }
+         }
+      }
+   };
 
-   if constexpr (DMA) {
-      const int64_t ahead = min(whole, (int64_t)(STAGES - 1));
-      for (int64_t kt = 0; kt < ahead; ++kt) issue(kt);
-      if (a.in_features % KT) {                                       // the part of a tile at the end comes first, through registers, into the stage that is free
-         T part[PIECES][PER];
-         fetch(whole, part);
-         place(STAGES - 1, part);
-         lds_barrier();
-         compute(STAGES - 1);
-      }
-      for (int64_t kt = 0; kt < whole; ++kt) {
-         if (whole - kt >= STAGES - 1) vm_wait<PIECES * (STAGES - 2)>(); else vm_wait<0>();
-         lds_barrier();
-         if (kt + STAGES - 1 < whole) issue(kt + STAGES - 1);
-         compute((int)(kt % STAGES));
-      }
-   } else {
-      const int64_t all = (a.in_features + KT - 1) / KT;
-      if (all) { fetch(0, held); place(0, held); }
-      for (int64_t kt = 0; kt < all; ++kt) {
-         if (kt + 1 < all) fetch(kt + 1, held);
-         lds_barrier();
-         compute((int)(kt & 1));
-         if (kt + 1 < all) place((int)((kt + 1) & 1), held);          // its readers are behind the barrier above
-      }
-   }
-   if constexpr (sizeof(T) == 4) {
-      // An infinity times a part that is zero makes a NaN, and a value whose first part rounds to infinity one too: a wave that finds one does its outputs again, on the float32 pipe, straight
-      // from memory.  Every NaN of the definition ends here as well and stays one.
-      bool nan = false;
+   unsigned index = blockIdx.x;
+   aim(index);
+   int stage = 0;                                                     // of the next tile of k
+   const auto step = [](int stage, int by) { const int s = stage + by; return s < STAGES ? s : s - STAGES; };
+   const int ahead = (int)min(whole, (int64_t)(STAGES - 1));
+   if constexpr (DMA)
+      for (int i = 0; i < ahead; ++i) issue(i, step(stage, i));
+   for (;;) {
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll
-         for (int j = 0; j < TM; ++j)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) nan |= acc[i][j][e] != acc[i][j][e];
-      if (__any(nan)) {
-         const float *px[TM], *pw[TN];
-#pragma unroll
-         for (int j = 0; j < TM; ++j) px[j] = (const float *)a.x + min(row0 + wr + 32 * j + (lane & 31), a.rows - 1) * a.x_stride;
-#pragma unroll
-         for (int i = 0; i < TN; ++i) pw[i] = (const float *)a.weight + min(col0 + wc + 32 * i + (lane & 31), a.out_features - 1) * a.weight_stride;
+         for (int j = 0; j < TM; ++j) acc[i][j] = (f16v)(0.0f);
+      if constexpr (DMA) {
+         if (a.in_features % KT) {                                    // the part of a tile at the end comes first, through registers, into the stage that is free
+            T part[PIECES][PER];
+            fetch(whole, part);
+            lds_barrier();
+            place(step(stage, STAGES - 1), part);
+            lds_barrier();
+            compute(step(stage, STAGES - 1));
+         }
+         for (int64_t kt = 0; kt < whole; ++kt) {
+            if (whole - kt >= STAGES - 1) vm_wait<PIECES * (STAGES - 2)>(); else vm_wait<0>();
+            lds_barrier();
+            if (kt + STAGES - 1 < whole) issue(kt + STAGES - 1, step(stage, STAGES - 1));
+            compute(stage);
+            stage = step(stage, 1);
+         }
+      } else {
+         const int64_t all = (a.in_features + KT - 1) / KT;
+         T held[PIECES][PER];
+         if (all) { fetch(0, held); lds_barrier(); place(0, held); }
+         for (int64_t kt = 0; kt < all; ++kt) {
+            if (kt + 1 < all) fetch(kt + 1, held);
+            lds_barrier();
+            compute((int)(kt & 1));
+            if (kt + 1 < all) place((int)((kt + 1) & 1), held);       // its readers are behind the barrier above
+         }
+      }
+      if constexpr (sizeof(T) == 4) {
+         // An infinity times a part that is zero makes a NaN, and a value whose first part rounds to infinity one too: a wave that finds one does its outputs again, on the float32
+         // pipe, straight from memory.  Every NaN of the definition ends here as well and stays one.
+         bool nan = false;
 #pragma unroll
          for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) acc[i][j] = (f16v)(0.0f);
-         for (int64_t k = lane >> 5; k - (lane >> 5) < a.in_features; k += 2) {
-            const bool in = k < a.in_features;
+            for (int j = 0; j < TM; ++j)
+#pragma unroll
+               for (int e = 0; e < 16; ++e) nan |= acc[i][j][e] != acc[i][j][e];
+         if (__any(nan)) {
 #pragma unroll
             for (int i = 0; i < TN; ++i)
 #pragma unroll
-               for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? pw[i][k] : 0.0f, in ? px[j][k] : 0.0f, acc[i][j], 0, 0, 0);
+               for (int j = 0; j < TM; ++j) {
+                  const float *px = (const float *)a.x + min(row0 + wr + 32 * j + (lane & 31), a.rows - 1) * a.x_stride;
+                  const float *pw = (const float *)a.weight + min(col0 + wc + 32 * i + (lane & 31), a.out_features - 1) * a.weight_stride;
+                  acc[i][j] = (f16v)(0.0f);
+#pragma unroll 1
+                  for (int64_t k = lane >> 5; k - (lane >> 5) < a.in_features; k += 2) {
+                     const bool in = k < a.in_features;
+                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? pw[k] : 0.0f, in ? px[k] : 0.0f, acc[i][j], 0, 0, 0);
+                  }
+               }
          }
       }
-   }
-   // Out through LDS, 32 rows of the wave's features at a time in float32, so that a row's features leave (and its residuals come) as one run, eight to a lane: a lane's own accumulators lie
-   // in pieces of four features of 32 different rows (8192 x 4096 x 4096 bfloat16 with a residual: 340 us with stores straight from them, EPILOGUE us so)
-   lds_barrier();                                                     // everybody has read the last tile
-   constexpr int FEATS = BN / WC, PP = FEATS / 4, LPR = FEATS / 8, RPI = 64 / LPR;
-   f4 *mine = reinterpret_cast<f4 *>(lds) + wave * 32 * PP;
-   const auto slot = [&](int row, int piece) { return row * PP + (piece ^ (PP == 8 ? (row >> 1) & 7 : row & (PP - 1))); };
-   const int64_t col = col0 + wc + 8 * (lane % LPR);
-   float bias[8];
-   load_bias<T, 8>(a, col, bias);
-#pragma unroll
-   for (int j = 0; j < TM; ++j) {
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-         for (int g = 0; g < 4; ++g) mine[slot(lane & 31, 8 * i + 2 * g + (lane >> 5))] = f4{acc[i][j][4 * g], acc[i][j][4 * g + 1], acc[i][j][4 * g + 2], acc[i][j][4 * g + 3]};
-#pragma unroll
-      for (int k = 0; k < 32 / RPI; ++k) {
-         const int row = k * RPI + lane / LPR;
-         const f4 lo = mine[slot(row, 2 * (lane % LPR))], hi = mine[slot(row, 2 * (lane % LPR) + 1)];
-         float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-         finish<T, 8>(a, row0 + wr + 32 * j + row, col, y, bias);
+      lds_barrier();                                                  // everybody has read the last tile of k: its stage is free
+      const int64_t row = row0, col = col0;
+      index += gridDim.x;
+      const bool more = index < tiles;
+      if (more) {
+         aim(index);
+         if constexpr (DMA)
+            for (int i = 0; i < ahead; ++i) issue(i, step(stage, i));
       }
+      leave(DMA ? step(stage, STAGES - 1) : 0, row, col);
+      if (!more) break;
    }
 }
 
@@ -330,7 +353,8 @@ __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_arg
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
 template <typename T, int BM, int BN, int WR, int WC, int STAGES> static void launch_tile(const vadc_amd_linear_args &a, hipStream_t s, bool dma)
 {
-   const dim3 grid((unsigned)(((a.rows + BM - 1) / BM) * ((a.out_features + BN - 1) / BN)));
+   constexpr int64_t slots = 256 * (512 / (64 * WR * WC));             // 512 threads a CU at a time
+   const dim3 grid((unsigned)std::min(slots, ((a.rows + BM - 1) / BM) * ((a.out_features + BN - 1) / BN)));
    if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, STAGES, true>), grid, dim3(64 * WR * WC), 0, s, a);
    else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, 2, false>), grid, dim3(64 * WR * WC), 0, s, a);
 }
