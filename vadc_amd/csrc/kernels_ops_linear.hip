@@ -54,21 +54,21 @@ __device__ __forceinline__ void finish(const vadc_amd_linear_args &a, int64_t ro
          if (i < left) out[i] = (T)y[i];
 }
 
-// ---- operands in LDS: rows of 128 bytes (KT elements of k), eight 16-byte pieces, the piece index mixed with the row so that the rows of a fragment lie in different banks
-__device__ __forceinline__ int piece_at(int row, int piece) { return row * 128 + ((piece ^ ((row >> 1) & 7)) << 4); }
-template <typename T> struct Tile { static constexpr int k = 128 / (int)sizeof(T); };      // 64 elements of 16 bits, 32 of 32
+// ---- operands in LDS: rows of RB = 64 or 128 bytes, 16-byte pieces, the piece index mixed with the row so that the rows of a fragment lie in different banks
+template <int RB> __device__ __forceinline__ int mixed(int row, int piece) { return RB == 128 ? piece ^ ((row >> 1) & 7) : piece ^ ((row >> 2) & 3); }
+template <int RB> __device__ __forceinline__ int piece_at(int row, int piece) { return row * RB + (mixed<RB>(row, piece) << 4); }
 
 // one product step: 16 k's of a 32 x 32 tile (float32: in three bfloat16 parts, ops_prims.h)
 template <typename T> struct Frag;
 template <> struct Frag<__bf16> { b8 v; };
 template <> struct Frag<_Float16> { h8 v; };
 template <> struct Frag<float> { p8 p[3]; };
-template <typename T> __device__ __forceinline__ Frag<T> load_frag(const char *tile, int row, int step, int half)
+template <typename T, int RB> __device__ __forceinline__ Frag<T> load_frag(const char *tile, int row, int step, int half)
 {
    Frag<T> f;
-   if constexpr (sizeof(T) == 2) f.v = *reinterpret_cast<const decltype(f.v) *>(tile + piece_at(row, 2 * step + half));
+   if constexpr (sizeof(T) == 2) f.v = *reinterpret_cast<const decltype(f.v) *>(tile + piece_at<RB>(row, 2 * step + half));
    else {
-      const f4 lo = *reinterpret_cast<const f4 *>(tile + piece_at(row, 4 * step + 2 * half)), hi = *reinterpret_cast<const f4 *>(tile + piece_at(row, 4 * step + 2 * half + 1));
+      const f4 lo = *reinterpret_cast<const f4 *>(tile + piece_at<RB>(row, 4 * step + 2 * half)), hi = *reinterpret_cast<const f4 *>(tile + piece_at<RB>(row, 4 * step + 2 * half + 1));
       const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       split8<float>(x, f.p);
    }
@@ -104,13 +104,14 @@ template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_wai
 // features of one row.  STAGES tiles of k are in LDS or on their way there: with DMA (16-byte aligned rows) a wave waits for the oldest with a counted vmcnt -- an operation the count does
 // not know of can only make it wait longer -- and one barrier a tile lets everybody read it and the next one overwrite the last; without, tiles pass through registers.
 // A workgroup does every gridDim-th output tile; the next one's first tiles of k are fetched before this one's outputs leave, which takes as long as a few tiles of k.
-// Outputs leave through LDS, 32 rows of up to 64 of the wave's features at a time in float32, so that a row's features leave (and its residuals come) as one run, eight to a lane: a
+// Outputs leave through LDS, 32 rows of 64 or 32 of the wave's features at a time in float32, so that a row's features leave (and its residuals come) as one run, 16 bytes to a lane: a
 // lane's own accumulators lie in pieces of four features of 32 different rows (8192 x 4096 x 4096 bfloat16 with a residual: 340 us with stores straight from them, 260 us so).
-template <typename T, int BM, int BN, int WR, int WC, int STAGES, bool DMA>
+template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES, bool DMA>
 __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_tile(const vadc_amd_linear_args a)
 {
-   constexpr int WAVES = WR * WC, KT = Tile<T>::k, TM = BM / WR / 32, TN = BN / WC / 32, BYTES = (BM + BN) * 128, PIECES = (BM + BN) / 8 / WAVES, PER = 16 / (int)sizeof(T);
-   static_assert((BM + BN) / 8 % WAVES == 0 && (BM / 8) % PIECES == 0, "a wave's pieces lie in one operand");
+   constexpr int WAVES = WR * WC, KT = RB / (int)sizeof(T), TM = BM / WR / 32, TN = BN / WC / 32, BYTES = (BM + BN) * RB, PER = 16 / (int)sizeof(T);
+   constexpr int ROWS = 1024 / RB, XP = BM / ROWS / WAVES, PIECES = (BM + BN) / ROWS / WAVES;      // LDS rows of a DMA instruction; a wave's instructions for x, for both
+   static_assert(BM % (ROWS * WAVES) == 0 && BN % (ROWS * WAVES) == 0, "every wave does the same");
    __shared__ __attribute__((aligned(16))) char lds[STAGES * BYTES];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
    const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.out_features + BN - 1) / BN;
@@ -118,39 +119,39 @@ __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_t
    const int wr = wave % WR * (BM / WR), wc = wave / WR * (BN / WC);
    const int64_t whole = a.in_features / KT;                          // full tiles of k
 
-   // this wave's pieces of eight LDS rows: rows 8 PIECES wave .. of x's tile, then of the weight's
-   const bool of_x = wave * PIECES < BM / 8;
-   const int at = wave * PIECES * 8 - (of_x ? 0 : BM);                // first row in its operand
-   const int64_t stride = of_x ? a.x_stride : a.weight_stride;
-   int64_t row0, col0, last;
-   const T *src;
+   // this wave's instructions: of x's tile, then of the weight's, each ROWS of its rows; rows behind the last are copies of it, their outputs are dropped
+   int64_t row0, col0;
+   int lastx, lastw;
+   const T *srcx, *srcw;
    uint32_t offset[PIECES];
-   const auto row_of = [&](int p) { return (int)min((int64_t)(at + 8 * p + (lane >> 3)), last); };      // rows behind the last are copies of it: their outputs are dropped
-   const auto piece_of = [&](int p) { return (lane & 7) ^ (((at + 8 * p + (lane >> 3)) >> 1) & 7); };
+   const auto row_in = [&](int p) { return ((p < XP ? p : p - XP) * WAVES + wave) * ROWS + lane / (RB / 16); };
+   const auto row_of = [&](int p) { return min(row_in(p), p < XP ? lastx : lastw); };
+   const auto piece_of = [&](int p) { return mixed<RB>(row_in(p), lane % (RB / 16)); };
    const auto aim = [&](unsigned index) {
       // launch order -> tile: the workgroups of one XCD (every eighth) take consecutive tiles, which go down eight row tiles before the next feature tile: their operands stay in its L2
       const unsigned x = index % 8, q = tiles / 8, r = tiles % 8;
       const int64_t id = x * q + min(x, r) + index / 8, group = id / (8 * tiles_n), first = group * 8, high = min((int64_t)8, tiles_m - first), in = id - group * 8 * tiles_n;
       row0 = (first + in % high) * BM;
       col0 = in / high * BN;
-      const int64_t top = of_x ? row0 : col0;
-      last = (of_x ? a.rows : a.out_features) - 1 - top;
-      src = (const T *)(of_x ? a.x : a.weight) + top * stride;
+      lastx = (int)min(a.rows - 1 - row0, (int64_t)BM);
+      lastw = (int)min(a.out_features - 1 - col0, (int64_t)BN);
+      srcx = (const T *)a.x + row0 * a.x_stride;
+      srcw = (const T *)a.weight + col0 * a.weight_stride;
       if constexpr (DMA)
 #pragma unroll
-         for (int p = 0; p < PIECES; ++p) offset[p] = (uint32_t)(row_of(p) * (int)(stride * sizeof(T)) + 16 * piece_of(p));
+         for (int p = 0; p < PIECES; ++p) offset[p] = (uint32_t)(row_of(p) * (int)((p < XP ? a.x_stride : a.weight_stride) * sizeof(T)) + 16 * piece_of(p));
    };
    const auto issue = [&](int64_t kt, int stage) {
-      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (uint32_t)stage * BYTES + wave * PIECES * 1024;
-      const void *from = uniform(src + kt * KT);
+      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (uint32_t)stage * BYTES + wave * 1024;
+      const void *fromx = uniform(srcx + kt * KT), *fromw = uniform(srcw + kt * KT);
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) dma(to + p * 1024, offset[p], from);
+      for (int p = 0; p < PIECES; ++p) dma(to + p * WAVES * 1024, offset[p], p < XP ? fromx : fromw);
    };
    const auto fetch = [&](int64_t kt, auto &h) {                      // through registers: any alignment, zeros behind the last k
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
          const int64_t k = kt * KT + piece_of(p) * PER, left = a.in_features - k;
-         const T *from = src + row_of(p) * stride + k;
+         const T *from = p < XP ? srcx + row_of(p) * a.x_stride + k : srcw + row_of(p) * a.weight_stride + k;
          if (left >= PER) {
             const Pack<T, PER> u = *reinterpret_cast<const Pack<T, PER> *>(from);
 #pragma unroll
@@ -162,34 +163,34 @@ __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_t
    };
    const auto place = [&](int stage, const auto &h) {
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) __builtin_memcpy(__builtin_assume_aligned(lds + stage * BYTES + (wave * PIECES + p) * 1024 + lane * 16, 16), &h[p], 16);
+      for (int p = 0; p < PIECES; ++p) __builtin_memcpy(__builtin_assume_aligned(lds + stage * BYTES + (p * WAVES + wave) * 1024 + lane * 16, 16), &h[p], 16);
    };
    f16v acc[TN][TM];
    const auto compute = [&](int stage) {
-      const char *sx = lds + stage * BYTES, *sw = sx + BM * 128;
+      const char *sx = lds + stage * BYTES, *sw = sx + BM * RB;
 #pragma unroll
       for (int s = 0; s < KT / 16; ++s) {
          Frag<T> fa[TN], fb[TM];
 #pragma unroll
-         for (int i = 0; i < TN; ++i) fa[i] = load_frag<T>(sw, wc + 32 * i + (lane & 31), s, lane >> 5);
+         for (int i = 0; i < TN; ++i) fa[i] = load_frag<T, RB>(sw, wc + 32 * i + (lane & 31), s, lane >> 5);
 #pragma unroll
-         for (int j = 0; j < TM; ++j) fb[j] = load_frag<T>(sx, wr + 32 * j + (lane & 31), s, lane >> 5);
+         for (int j = 0; j < TM; ++j) fb[j] = load_frag<T, RB>(sx, wr + 32 * j + (lane & 31), s, lane >> 5);
 #pragma unroll
          for (int i = 0; i < TN; ++i)
 #pragma unroll
             for (int j = 0; j < TM; ++j) acc[i][j] = product(fa[i], fb[j], acc[i][j]);
       }
    };
-   constexpr int FEATS = BN / WC < 64 ? BN / WC : 64, PP = FEATS / 4, LPR = FEATS / 8, RPI = 64 / LPR;
+   constexpr int FEATS = BN / WC >= 64 && BYTES >= WAVES * 32 * 64 * 4 ? 64 : 32, PP = FEATS / 4, OUT = PER, LPR = FEATS / OUT, RPI = 64 / LPR;      // OUT features (16 bytes) to a lane, LPR lanes to a row
    static_assert(BYTES >= WAVES * 32 * FEATS * 4, "the outputs leave through one stage");
    const auto leave = [&](int stage, int64_t row0, int64_t col0) {
       f4 *mine = reinterpret_cast<f4 *>(lds + stage * BYTES) + wave * 32 * PP;
       const auto slot = [&](int row, int piece) { return row * PP + (piece ^ (PP == 8 ? (row >> 1) & 7 : row & (PP - 1))); };
 #pragma unroll
       for (int h = 0; h < TN * 32 / FEATS; ++h) {
-         const int64_t col = col0 + wc + h * FEATS + 8 * (lane % LPR);
-         float bias[8];
-         load_bias<T, 8>(a, col, bias);
+         const int64_t col = col0 + wc + h * FEATS + OUT * (lane % LPR);
+         float bias[OUT];
+         load_bias<T, OUT>(a, col, bias);
 #pragma unroll
          for (int j = 0; j < TM; ++j) {
 #pragma unroll
@@ -202,9 +203,14 @@ __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_t
 #pragma unroll
             for (int k = 0; k < 32 / RPI; ++k) {
                const int row = k * RPI + lane / LPR;
-               const f4 lo = mine[slot(row, 2 * (lane % LPR))], hi = mine[slot(row, 2 * (lane % LPR) + 1)];
-               float y[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-               finish<T, 8>(a, row0 + wr + 32 * j + row, col, y, bias);
+               float y[OUT];
+#pragma unroll
+               for (int p = 0; p < OUT / 4; ++p) {
+                  const f4 c = mine[slot(row, OUT / 4 * (lane % LPR) + p)];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) y[4 * p + e] = c[e];
+               }
+               finish<T, OUT>(a, row0 + wr + 32 * j + row, col, y, bias);
             }
          }
       }
@@ -351,12 +357,12 @@ __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_arg
 }
 
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
-template <typename T, int BM, int BN, int WR, int WC, int STAGES> static void launch_tile(const vadc_amd_linear_args &a, hipStream_t s, bool dma)
+template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES> static void launch_tile(const vadc_amd_linear_args &a, hipStream_t s, bool dma)
 {
    constexpr int64_t slots = 256 * (512 / (64 * WR * WC));             // 512 threads a CU at a time
    const dim3 grid((unsigned)std::min(slots, ((a.rows + BM - 1) / BM) * ((a.out_features + BN - 1) / BN)));
-   if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, STAGES, true>), grid, dim3(64 * WR * WC), 0, s, a);
-   else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, 2, false>), grid, dim3(64 * WR * WC), 0, s, a);
+   if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, STAGES, true>), grid, dim3(64 * WR * WC), 0, s, a);
+   else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, 2, false>), grid, dim3(64 * WR * WC), 0, s, a);
 }
 template <typename T, int TM> static void launch_narrow(const vadc_amd_linear_args &a, hipStream_t s)
 {
@@ -370,9 +376,9 @@ template <typename T> static void launch(const vadc_amd_linear_args &a, hipStrea
    const bool dma = ((uintptr_t)a.x | (uintptr_t)a.weight) % 16 == 0 && a.x_stride % per == 0 && a.weight_stride % per == 0 &&
                     std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) < (int64_t(1) << 31) / 256;      // a tile's rows within 32-bit offsets
    const auto tiles = [&](int64_t t) { return ((a.rows + t - 1) / t) * ((a.out_features + t - 1) / t); };
-   if constexpr (sizeof(T) == 2) if (tiles(256) >= 200) return launch_tile<T, 256, 256, 4, 2, 2>(a, s, dma);
-   if (tiles(128) >= 200) return launch_tile<T, 128, 128, 2, 2, 2>(a, s, dma);
-   launch_tile<T, 64, 64, 2, 2, 4>(a, s, dma);
+   if constexpr (sizeof(T) == 2) if (tiles(256) >= 200) return launch_tile<T, 256, 256, 2, 4, 128, 2>(a, s, dma);
+   if (tiles(128) >= 200) return launch_tile<T, 128, 128, 2, 2, 128, 2>(a, s, dma);
+   launch_tile<T, 64, 64, 2, 2, 128, 4>(a, s, dma);
 }
 
 void launch_linear(const vadc_amd_linear_args &a, hipStream_t s)
