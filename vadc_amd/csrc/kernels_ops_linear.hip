@@ -24,12 +24,8 @@ template <typename T, int N> __device__ __forceinline__ void load_bias(const vad
          if (i < left) b[i] = (float)bias[i];
 }
 template <typename T, int N>
-__device__ __forceinline__ void finish(const vadc_amd_linear_args &a, int64_t row, int64_t col, float (&y)[N], const float (&b)[N])
+__device__ __forceinline__ void finish(const vadc_amd_linear_args &a, const T *res, T *out, int left, float (&y)[N], const float (&b)[N])
 {
-   const int64_t left = a.out_features - col;
-   if (row >= a.rows || left <= 0) return;
-   const T *res = (const T *)a.residual + row * a.residual_stride + col;
-   T *out = (T *)a.out + row * a.out_stride + col;
    float r[N];
 #pragma unroll
    for (int i = 0; i < N; ++i) { r[i] = 0.0f; y[i] += b[i]; }
@@ -54,36 +50,71 @@ __device__ __forceinline__ void finish(const vadc_amd_linear_args &a, int64_t ro
          if (i < left) out[i] = (T)y[i];
 }
 
+// Outputs leave through LDS, 32 rows of FEATS of the wave's features at a time in float32, so that a row's features leave (and its residuals come) as one run, 16 bytes to a lane: a
+// lane's own accumulators lie in pieces of four features of 32 different rows (8192 x 4096 x 4096 bfloat16 with a residual: 340 us with stores straight from them, 260 us so).
+// row, col: the wave's first; mine: 32 FEATS floats of its own.  KG > 1: as many waves hold sums over their part of the k's, `apart` further in LDS each; all write, and each does its
+// share of the rows from the sums of all.
+template <typename T, int TN, int TM, int FEATS, int KG>
+__device__ __forceinline__ void leave(const vadc_amd_linear_args &a, f4 *mine, int kg, int apart, const f16v (&acc)[TN][TM], int64_t row, int64_t col, int lane)
+{
+   static_assert(KG == 1 || (TN == 1 && TM == 1 && FEATS == 32), "one round: the sums of all are there behind one barrier");
+   constexpr int OUT = 16 / (int)sizeof(T), PP = FEATS / 4, LPR = FEATS / OUT, RPI = 64 / LPR;      // OUT features to a lane, LPR lanes to a row
+   const auto slot = [&](int r, int piece) { return r * PP + (piece ^ (PP == 8 ? (r >> 1) & 7 : r & (PP - 1))); };
+   const int64_t from = row + kg * RPI + lane / LPR;
+#pragma unroll
+   for (int h = 0; h < TN * 32 / FEATS; ++h) {
+      const int64_t c = col + h * FEATS + OUT * (lane % LPR);
+      const int left = (int)min((int64_t)OUT, a.out_features - c);
+      float bias[OUT];
+      load_bias<T, OUT>(a, c, bias);
+      const T *res = (const T *)a.residual + from * a.residual_stride + c;
+      T *out = (T *)a.out + from * a.out_stride + c;
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+#pragma unroll
+         for (int i = 0; i < FEATS / 32; ++i)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+               const f16v &v = acc[h * (FEATS / 32) + i][j];
+               mine[kg * apart + slot(lane & 31, 8 * i + 2 * g + (lane >> 5))] = f4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]};
+            }
+         if constexpr (KG > 1) lds_barrier();
+#pragma unroll
+         for (int k = 0; k < 32 / RPI / KG; ++k) {
+            const int r = (k * KG + kg) * RPI + lane / LPR;
+            float y[OUT];
+#pragma unroll
+            for (int p = 0; p < OUT / 4; ++p) {
+               f4 v = mine[slot(r, OUT / 4 * (lane % LPR) + p)];
+#pragma unroll
+               for (int g = 1; g < KG; ++g) v += mine[g * apart + slot(r, OUT / 4 * (lane % LPR) + p)];
+#pragma unroll
+               for (int e = 0; e < 4; ++e) y[4 * p + e] = v[e];
+            }
+            if (from + 32 * j + k * KG * RPI < a.rows && left > 0) finish<T, OUT>(a, res, out, left, y, bias);
+            res += KG * RPI * a.residual_stride;
+            out += KG * RPI * a.out_stride;
+         }
+      }
+   }
+}
+
+// Output tile of a launch's index: the workgroups of one XCD (every eighth) take consecutive tiles, which go down eight row tiles before the next feature tile: their operands stay in its L2
+__device__ __forceinline__ void tile_of(unsigned index, unsigned tiles, int64_t tiles_m, int64_t tiles_n, int64_t &tm, int64_t &tn)
+{
+   const unsigned x = index % 8, q = tiles / 8, r = tiles % 8;
+   const int64_t id = x * q + min(x, r) + index / 8, group = id / (8 * tiles_n), first = group * 8, high = min((int64_t)8, tiles_m - first), in = id - group * 8 * tiles_n;
+   tm = first + in % high;
+   tn = in / high;
+}
+
 // ---- operands in LDS: rows of RB = 64 or 128 bytes, 16-byte pieces, the piece index mixed with the row so that the rows of a fragment lie in different banks
 template <int RB> __device__ __forceinline__ int mixed(int row, int piece) { return RB == 128 ? piece ^ ((row >> 1) & 7) : piece ^ ((row >> 2) & 3); }
 template <int RB> __device__ __forceinline__ int piece_at(int row, int piece) { return row * RB + (mixed<RB>(row, piece) << 4); }
 
-// one product step: 16 k's of a 32 x 32 tile (float32: in three bfloat16 parts, ops_prims.h)
-template <typename T> struct Frag;
-template <> struct Frag<__bf16> { b8 v; };
-template <> struct Frag<_Float16> { h8 v; };
-template <> struct Frag<float> { p8 p[3]; };
-template <typename T, int RB> __device__ __forceinline__ Frag<T> load_frag(const char *tile, int row, int step, int half)
-{
-   Frag<T> f;
-   if constexpr (sizeof(T) == 2) f.v = *reinterpret_cast<const decltype(f.v) *>(tile + piece_at<RB>(row, 2 * step + half));
-   else {
-      const f4 lo = *reinterpret_cast<const f4 *>(tile + piece_at<RB>(row, 4 * step + 2 * half)), hi = *reinterpret_cast<const f4 *>(tile + piece_at<RB>(row, 4 * step + 2 * half + 1));
-      const float x[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      split8<float>(x, f.p);
-   }
-   return f;
-}
-__device__ __forceinline__ f16v product(const Frag<__bf16> &a, const Frag<__bf16> &b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0); }
-__device__ __forceinline__ f16v product(const Frag<_Float16> &a, const Frag<_Float16> &b, f16v c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.v, b.v, c, 0, 0, 0); }
-__device__ __forceinline__ f16v product(const Frag<float> &a, const Frag<float> &b, f16v c)
-{
-#pragma unroll
-   for (int o = 2; o >= 0; --o)
-#pragma unroll
-      for (int i = 0; i <= o; ++i) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a.p[i]), __builtin_bit_cast(b8, b.p[o - i]), c, 0, 0, 0);
-   return c;
-}
+// one product step: 16 k's of a 32 x 32 tile
+__device__ __forceinline__ f16v product(const p8 &a, const p8 &b, f16v c, __bf16) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0); }
+__device__ __forceinline__ f16v product(const p8 &a, const p8 &b, f16v c, _Float16) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0); }
 
 // 1024 bytes (eight LDS rows) from global memory straight into LDS, 16 bytes a lane, no registers between.  The caller waits with vm_wait before a barrier; M0 is written and
 // read in one statement.
@@ -104,20 +135,19 @@ template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_wai
 // features of one row.  STAGES tiles of k are in LDS or on their way there: with DMA (16-byte aligned rows) a wave waits for the oldest with a counted vmcnt -- an operation the count does
 // not know of can only make it wait longer -- and one barrier a tile lets everybody read it and the next one overwrite the last; without, tiles pass through registers.
 // A workgroup does every gridDim-th output tile; the next one's first tiles of k are fetched before this one's outputs leave, which takes as long as a few tiles of k.
-// Outputs leave through LDS, 32 rows of 64 or 32 of the wave's features at a time in float32, so that a row's features leave (and its residuals come) as one run, 16 bytes to a lane: a
-// lane's own accumulators lie in pieces of four features of 32 different rows (8192 x 4096 x 4096 bfloat16 with a residual: 340 us with stores straight from them, 260 us so).
-template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES, bool DMA>
-__global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_tile(const vadc_amd_linear_args a)
+// KG groups of waves take every KG-th tile of k each, where there are too few output tiles to fill the device with work.
+template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES, int KG, bool DMA>
+__global__ __launch_bounds__(64 * WR * WC * KG, (512 + 64 * WR * WC * KG - 1) / (64 * WR * WC * KG)) void k_linear_tile(const vadc_amd_linear_args a)
 {
    constexpr int WAVES = WR * WC, KT = RB / (int)sizeof(T), TM = BM / WR / 32, TN = BN / WC / 32, BYTES = (BM + BN) * RB, PER = 16 / (int)sizeof(T);
    constexpr int ROWS = 1024 / RB, XP = BM / ROWS / WAVES, PIECES = (BM + BN) / ROWS / WAVES;      // LDS rows of a DMA instruction; a wave's instructions for x, for both
    static_assert(BM % (ROWS * WAVES) == 0 && BN % (ROWS * WAVES) == 0, "every wave does the same");
-   __shared__ __attribute__((aligned(16))) char lds[STAGES * BYTES];
-   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+   __shared__ __attribute__((aligned(16))) char lds[STAGES * KG * BYTES];
+   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % WAVES, kg = __builtin_amdgcn_readfirstlane(tid >> 6) / WAVES;
    const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.out_features + BN - 1) / BN;
    const unsigned tiles = (unsigned)(tiles_m * tiles_n);
    const int wr = wave % WR * (BM / WR), wc = wave / WR * (BN / WC);
-   const int64_t whole = a.in_features / KT;                          // full tiles of k
+   const int64_t full = a.in_features / KT, rounds = (full + KG - 1) / KG, whole = (full - kg + KG - 1) / KG;      // full tiles of k; this group's are kg, kg + KG, ...
 
    // this wave's instructions: of x's tile, then of the weight's, each ROWS of its rows; rows behind the last are copies of it, their outputs are dropped
    int64_t row0, col0;
@@ -128,11 +158,10 @@ __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_t
    const auto row_of = [&](int p) { return min(row_in(p), p < XP ? lastx : lastw); };
    const auto piece_of = [&](int p) { return mixed<RB>(row_in(p), lane % (RB / 16)); };
    const auto aim = [&](unsigned index) {
-      // launch order -> tile: the workgroups of one XCD (every eighth) take consecutive tiles, which go down eight row tiles before the next feature tile: their operands stay in its L2
-      const unsigned x = index % 8, q = tiles / 8, r = tiles % 8;
-      const int64_t id = x * q + min(x, r) + index / 8, group = id / (8 * tiles_n), first = group * 8, high = min((int64_t)8, tiles_m - first), in = id - group * 8 * tiles_n;
-      row0 = (first + in % high) * BM;
-      col0 = in / high * BN;
+      int64_t tm, tn;
+      tile_of(index, tiles, tiles_m, tiles_n, tm, tn);
+      row0 = tm * BM;
+      col0 = tn * BN;
       lastx = (int)min(a.rows - 1 - row0, (int64_t)BM);
       lastw = (int)min(a.out_features - 1 - col0, (int64_t)BN);
       srcx = (const T *)a.x + row0 * a.x_stride;
@@ -142,8 +171,8 @@ __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_t
          for (int p = 0; p < PIECES; ++p) offset[p] = (uint32_t)(row_of(p) * (int)((p < XP ? a.x_stride : a.weight_stride) * sizeof(T)) + 16 * piece_of(p));
    };
    const auto issue = [&](int64_t kt, int stage) {
-      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (uint32_t)stage * BYTES + wave * 1024;
-      const void *fromx = uniform(srcx + kt * KT), *fromw = uniform(srcw + kt * KT);
+      const uint32_t to = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)lds + (uint32_t)(stage * KG + kg) * BYTES + wave * 1024;
+      const void *fromx = uniform(srcx + (kt * KG + kg) * KT), *fromw = uniform(srcw + (kt * KG + kg) * KT);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) dma(to + p * WAVES * 1024, offset[p], p < XP ? fromx : fromw);
    };
@@ -163,58 +192,26 @@ __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_t
    };
    const auto place = [&](int stage, const auto &h) {
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) __builtin_memcpy(__builtin_assume_aligned(lds + stage * BYTES + (p * WAVES + wave) * 1024 + lane * 16, 16), &h[p], 16);
+      for (int p = 0; p < PIECES; ++p) __builtin_memcpy(__builtin_assume_aligned(lds + (stage * KG + kg) * BYTES + (p * WAVES + wave) * 1024 + lane * 16, 16), &h[p], 16);
    };
    f16v acc[TN][TM];
    const auto compute = [&](int stage) {
-      const char *sx = lds + stage * BYTES, *sw = sx + BM * RB;
+      const char *sx = lds + (stage * KG + kg) * BYTES, *sw = sx + BM * RB;
 #pragma unroll
       for (int s = 0; s < KT / 16; ++s) {
-         Frag<T> fa[TN], fb[TM];
+         p8 fa[TN], fb[TM];
 #pragma unroll
-         for (int i = 0; i < TN; ++i) fa[i] = load_frag<T, RB>(sw, wc + 32 * i + (lane & 31), s, lane >> 5);
+         for (int i = 0; i < TN; ++i) fa[i] = *reinterpret_cast<const p8 *>(sw + piece_at<RB>(wc + 32 * i + (lane & 31), 2 * s + (lane >> 5)));
 #pragma unroll
-         for (int j = 0; j < TM; ++j) fb[j] = load_frag<T, RB>(sx, wr + 32 * j + (lane & 31), s, lane >> 5);
+         for (int j = 0; j < TM; ++j) fb[j] = *reinterpret_cast<const p8 *>(sx + piece_at<RB>(wr + 32 * j + (lane & 31), 2 * s + (lane >> 5)));
 #pragma unroll
          for (int i = 0; i < TN; ++i)
 #pragma unroll
-            for (int j = 0; j < TM; ++j) acc[i][j] = product(fa[i], fb[j], acc[i][j]);
+            for (int j = 0; j < TM; ++j) acc[i][j] = product(fa[i], fb[j], acc[i][j], T());
       }
    };
-   constexpr int FEATS = BN / WC >= 64 && BYTES >= WAVES * 32 * 64 * 4 ? 64 : 32, PP = FEATS / 4, OUT = PER, LPR = FEATS / OUT, RPI = 64 / LPR;      // OUT features (16 bytes) to a lane, LPR lanes to a row
+   constexpr int FEATS = BN / WC >= 64 && BYTES >= WAVES * 32 * 64 * 4 ? 64 : 32;
    static_assert(BYTES >= WAVES * 32 * FEATS * 4, "the outputs leave through one stage");
-   const auto leave = [&](int stage, int64_t row0, int64_t col0) {
-      f4 *mine = reinterpret_cast<f4 *>(lds + stage * BYTES) + wave * 32 * PP;
-      const auto slot = [&](int row, int piece) { return row * PP + (piece ^ (PP == 8 ? (row >> 1) & 7 : row & (PP - 1))); };
-#pragma unroll
-      for (int h = 0; h < TN * 32 / FEATS; ++h) {
-         const int64_t col = col0 + wc + h * FEATS + OUT * (lane % LPR);
-         float bias[OUT];
-         load_bias<T, OUT>(a, col, bias);
-#pragma unroll
-         for (int j = 0; j < TM; ++j) {
-#pragma unroll
-            for (int i = 0; i < FEATS / 32; ++i)
-#pragma unroll
-               for (int g = 0; g < 4; ++g) {
-                  const f16v &c = acc[h * (FEATS / 32) + i][j];
-                  mine[slot(lane & 31, 8 * i + 2 * g + (lane >> 5))] = f4{c[4 * g], c[4 * g + 1], c[4 * g + 2], c[4 * g + 3]};
-               }
-#pragma unroll
-            for (int k = 0; k < 32 / RPI; ++k) {
-               const int row = k * RPI + lane / LPR;
-               float y[OUT];
-#pragma unroll
-               for (int p = 0; p < OUT / 4; ++p) {
-                  const f4 c = mine[slot(row, OUT / 4 * (lane % LPR) + p)];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) y[4 * p + e] = c[e];
-               }
-               finish<T, OUT>(a, row0 + wr + 32 * j + row, col, y, bias);
-            }
-         }
-      }
-   };
 
    unsigned index = blockIdx.x;
    aim(index);
@@ -229,56 +226,34 @@ __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_t
 #pragma unroll
          for (int j = 0; j < TM; ++j) acc[i][j] = (f16v)(0.0f);
       if constexpr (DMA) {
-         if (a.in_features % KT) {                                    // the part of a tile at the end comes first, through registers, into the stage that is free
+         if (a.in_features % KT) {                                    // the part of a tile at the end comes first, through registers, into the stage that is free; the last group has the least else
             T part[PIECES][PER];
-            fetch(whole, part);
+            if (kg == KG - 1) fetch(full, part);
             lds_barrier();
-            place(step(stage, STAGES - 1), part);
+            if (kg == KG - 1) place(step(stage, STAGES - 1), part);
             lds_barrier();
-            compute(step(stage, STAGES - 1));
+            if (kg == KG - 1) compute(step(stage, STAGES - 1));
          }
-         for (int64_t kt = 0; kt < whole; ++kt) {
+         for (int64_t kt = 0; kt < rounds; ++kt) {
             if (whole - kt >= STAGES - 1) vm_wait<PIECES * (STAGES - 2)>(); else vm_wait<0>();
             lds_barrier();
             if (kt + STAGES - 1 < whole) issue(kt + STAGES - 1, step(stage, STAGES - 1));
-            compute(stage);
+            if (KG == 1 || kt < whole) compute(stage);
             stage = step(stage, 1);
          }
       } else {
-         const int64_t all = (a.in_features + KT - 1) / KT;
+         const int64_t all = (a.in_features + KT - 1) / KT, turns = (all + KG - 1) / KG, own = (all - kg + KG - 1) / KG;
          T held[PIECES][PER];
-         if (all) { fetch(0, held); lds_barrier(); place(0, held); }
-         for (int64_t kt = 0; kt < all; ++kt) {
-            if (kt + 1 < all) fetch(kt + 1, held);
+         if (turns) {
+            if (own) fetch(kg, held);
             lds_barrier();
-            compute((int)(kt & 1));
-            if (kt + 1 < all) place((int)((kt + 1) & 1), held);       // its readers are behind the barrier above
+            if (own) place(0, held);
          }
-      }
-      if constexpr (sizeof(T) == 4) {
-         // An infinity times a part that is zero makes a NaN, and a value whose first part rounds to infinity one too: a wave that finds one does its outputs again, on the float32
-         // pipe, straight from memory.  Every NaN of the definition ends here as well and stays one.
-         bool nan = false;
-#pragma unroll
-         for (int i = 0; i < TN; ++i)
-#pragma unroll
-            for (int j = 0; j < TM; ++j)
-#pragma unroll
-               for (int e = 0; e < 16; ++e) nan |= acc[i][j][e] != acc[i][j][e];
-         if (__any(nan)) {
-#pragma unroll
-            for (int i = 0; i < TN; ++i)
-#pragma unroll
-               for (int j = 0; j < TM; ++j) {
-                  const float *px = (const float *)a.x + min(row0 + wr + 32 * j + (lane & 31), a.rows - 1) * a.x_stride;
-                  const float *pw = (const float *)a.weight + min(col0 + wc + 32 * i + (lane & 31), a.out_features - 1) * a.weight_stride;
-                  acc[i][j] = (f16v)(0.0f);
-#pragma unroll 1
-                  for (int64_t k = lane >> 5; k - (lane >> 5) < a.in_features; k += 2) {
-                     const bool in = k < a.in_features;
-                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? pw[k] : 0.0f, in ? px[k] : 0.0f, acc[i][j], 0, 0, 0);
-                  }
-               }
+         for (int64_t kt = 0; kt < turns; ++kt) {
+            if (kt + 1 < own) fetch((kt + 1) * KG + kg, held);
+            lds_barrier();
+            if (KG == 1 || kt < own) compute((int)(kt & 1));
+            if (kt + 1 < own) place((int)((kt + 1) & 1), held);       // its readers are behind the barrier above
          }
       }
       lds_barrier();                                                  // everybody has read the last tile of k: its stage is free
@@ -290,7 +265,132 @@ __global__ __launch_bounds__(64 * WR * WC, 512 / (64 * WR * WC)) void k_linear_t
          if constexpr (DMA)
             for (int i = 0; i < ahead; ++i) issue(i, step(stage, i));
       }
-      leave(DMA ? step(stage, STAGES - 1) : 0, row, col);
+      leave<T, TN, TM, FEATS, KG>(a, reinterpret_cast<f4 *>(lds + (DMA ? step(stage, STAGES - 1) : 0) * KG * BYTES) + wave * 8 * FEATS, kg, BYTES / 16, acc, row + wr, col + wc, lane);
+      if (!more) break;
+   }
+}
+
+// float32, BM x BN outputs per tile, four waves: operands go through registers into LDS in three bfloat16 parts (ops_prims.h), 32 k's at a time, six products for one.  Splitting on the
+// way in costs a value 5.5 instructions once; split where a wave reads them, every value was split twice (98304 x 128 x 512: 110 us so, 105 us this way).  One set of tiles, two barriers a
+// step: two workgroups share a CU and fill each other's gaps (a third would cost 30 spilled registers: 118 us).
+template <int BM, int BN, int WR, int WC>
+__global__ __launch_bounds__(256, 2) void k_linear_parts(const vadc_amd_linear_args a)
+{
+   constexpr int WAVES = WR * WC, KT = 32, TM = BM / WR / 32, TN = BN / WC / 32, PLANE = (BM + BN) * 64, XP = BM / 16 / WAVES, PIECES = (BM + BN) / 16 / WAVES;
+   static_assert(WAVES == 4 && BM % (16 * WAVES) == 0 && BN % (16 * WAVES) == 0, "every wave does the same");
+   __shared__ __attribute__((aligned(16))) char lds[3 * PLANE];
+   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+   const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.out_features + BN - 1) / BN;
+   const unsigned tiles = (unsigned)(tiles_m * tiles_n);
+   const int wr = wave % WR * (BM / WR), wc = wave / WR * (BN / WC);
+   const int64_t all = (a.in_features + KT - 1) / KT;
+   const auto row_in = [&](int p) { return ((p < XP ? p : p - XP) * WAVES + wave) * 16 + (lane >> 2); };      // a lane's eight k's of this row of its operand, lane % 4 of the four eights
+   int64_t row0, col0;
+   const float *from[PIECES];
+   const auto aim = [&](unsigned index) {
+      int64_t tm, tn;
+      tile_of(index, tiles, tiles_m, tiles_n, tm, tn);
+      row0 = tm * BM;
+      col0 = tn * BN;
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p)                                // rows behind the last are copies of it: their outputs are dropped
+         from[p] = (p < XP ? (const float *)a.x + min(row0 + row_in(p), a.rows - 1) * a.x_stride : (const float *)a.weight + min(col0 + row_in(p), a.out_features - 1) * a.weight_stride) + 8 * (lane & 3);
+   };
+   float held[PIECES][8];
+   const auto fetch = [&](int64_t kt) {
+      const int64_t k = kt * KT;
+      if (k + KT <= a.in_features) {
+#pragma unroll
+         for (int p = 0; p < PIECES; ++p) load_f32<float, 8>(from[p] + k, held[p]);
+      } else {
+         const int left = (int)(a.in_features - k) - 8 * (lane & 3);
+#pragma unroll
+         for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) held[p][i] = i < left ? from[p][k + i] : 0.0f;
+      }
+   };
+   const auto place = [&] {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+         p8 w[3];
+         split8<float>(held[p], w);
+#pragma unroll
+         for (int n = 0; n < 3; ++n) *reinterpret_cast<p8 *>(lds + n * PLANE + (p < XP ? 0 : BM * 64) + piece_at<64>(row_in(p), lane & 3)) = w[n];
+      }
+   };
+   constexpr int FEATS = BN / WC >= 64 ? 64 : 32;
+   static_assert(3 * PLANE >= WAVES * 32 * FEATS * 4, "the outputs leave through the same LDS");
+
+   unsigned index = blockIdx.x;
+   aim(index);
+   if (all) fetch(0);
+   for (;;) {
+      f16v acc[TN][TM];
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+         for (int j = 0; j < TM; ++j) acc[i][j] = (f16v)(0.0f);
+      for (int64_t kt = 0; kt < all; ++kt) {
+         lds_barrier();                                               // everybody is through with the last tiles, or with the last outputs
+         place();
+         if (kt + 1 < all) fetch(kt + 1);
+         lds_barrier();
+#pragma unroll
+         for (int s = 0; s < 2; ++s) {
+            p8 fb[TM][3];
+#pragma unroll
+            for (int n = 0; n < 3; ++n)
+#pragma unroll
+               for (int j = 0; j < TM; ++j) fb[j][n] = *reinterpret_cast<const p8 *>(lds + n * PLANE + piece_at<64>(wr + 32 * j + (lane & 31), 2 * s + (lane >> 5)));
+#pragma unroll
+            for (int i = 0; i < TN; ++i) {
+               p8 fa[3];
+#pragma unroll
+               for (int n = 0; n < 3; ++n) fa[n] = *reinterpret_cast<const p8 *>(lds + n * PLANE + BM * 64 + piece_at<64>(wc + 32 * i + (lane & 31), 2 * s + (lane >> 5)));
+#pragma unroll
+               for (int o = 2; o >= 0; --o)                           // the small products first
+#pragma unroll
+                  for (int n = 0; n <= o; ++n)
+#pragma unroll
+                     for (int j = 0; j < TM; ++j) acc[i][j] = product(fa[n], fb[j][o - n], acc[i][j], __bf16());
+            }
+         }
+      }
+      // An infinity times a part that is zero makes a NaN, and a value whose first part rounds to infinity one too: a wave that finds one does its outputs again, on the float32 pipe,
+      // straight from memory.  Every NaN of the definition ends here as well and stays one.
+      f16v sum = (f16v)(0.0f);
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+         for (int j = 0; j < TM; ++j) sum += acc[i][j] * 0.0f;
+      float nan = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) nan += sum[e];
+      if (__any(nan != 0.0f)) {
+#pragma unroll
+         for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int j = 0; j < TM; ++j) {
+               const float *px = (const float *)a.x + min(row0 + wr + 32 * j + (lane & 31), a.rows - 1) * a.x_stride;
+               const float *pw = (const float *)a.weight + min(col0 + wc + 32 * i + (lane & 31), a.out_features - 1) * a.weight_stride;
+               acc[i][j] = (f16v)(0.0f);
+#pragma unroll 1
+               for (int64_t k = lane >> 5; k - (lane >> 5) < a.in_features; k += 2) {
+                  const bool in = k < a.in_features;
+                  acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? pw[k] : 0.0f, in ? px[k] : 0.0f, acc[i][j], 0, 0, 0);
+               }
+            }
+      }
+      const int64_t row = row0, col = col0;
+      index += gridDim.x;
+      const bool more = index < tiles;
+      if (more) {
+         aim(index);
+         if (all) fetch(0);
+      }
+      lds_barrier();                                                  // everybody has read the last tiles
+      leave<float, TN, TM, FEATS, 1>(a, reinterpret_cast<f4 *>(lds) + wave * 8 * FEATS, 0, 0, acc, row + wr, col + wc, lane);
       if (!more) break;
    }
 }
@@ -334,11 +434,11 @@ __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_arg
          } else {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-               Frag<T> fa, fb;
-#pragma unroll
-               for (int i = 0; i < 8; ++i) { fa.v[i] = w[8 * s + i]; fb.v[i] = x[j][8 * s + i]; }
-               if constexpr (__is_same(T, __bf16)) acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa.v, fb.v, acc[j], 0, 0, 0);
-               else acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa.v, fb.v, acc[j], 0, 0, 0);
+               p8 fa, fb;
+               __builtin_memcpy(&fa, &w[8 * s], sizeof(fa));
+               __builtin_memcpy(&fb, &x[j][8 * s], sizeof(fb));
+               if constexpr (__is_same(T, __bf16)) acc[j] = mfma16(fa, fb, acc[j]);
+               else acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, fa), __builtin_bit_cast(h8, fb), acc[j], 0, 0, 0);
             }
          }
       }
@@ -350,35 +450,48 @@ __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_arg
       f4 sum = part[0][j][lane];
 #pragma unroll
       for (int w = 1; w < WAVES; ++w) sum += part[w][j][lane];
+      const int64_t row = row0 + 16 * j + l15, col = col0 + 4 * l4;
       float y[4] = {sum[0], sum[1], sum[2], sum[3]}, bias[4];
-      load_bias<T, 4>(a, col0 + 4 * l4, bias);
-      finish<T, 4>(a, row0 + 16 * j + l15, col0 + 4 * l4, y, bias);
+      load_bias<T, 4>(a, col, bias);
+      const int left = (int)min((int64_t)4, a.out_features - col);
+      if (row < a.rows && left > 0) finish<T, 4>(a, (const T *)a.residual + row * a.residual_stride + col, (T *)a.out + row * a.out_stride + col, left, y, bias);
    }
 }
 
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
-template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES> static void launch_tile(const vadc_amd_linear_args &a, hipStream_t s, bool dma)
+template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES, int KG> static void launch_tile(const vadc_amd_linear_args &a, hipStream_t s, bool dma)
 {
-   constexpr int64_t slots = 256 * (512 / (64 * WR * WC));             // 512 threads a CU at a time
+   constexpr int threads = 64 * WR * WC * KG;
+   constexpr int64_t slots = 256 * std::max(1, 512 / threads);         // 512 threads a CU at a time
    const dim3 grid((unsigned)std::min(slots, ((a.rows + BM - 1) / BM) * ((a.out_features + BN - 1) / BN)));
-   if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, STAGES, true>), grid, dim3(64 * WR * WC), 0, s, a);
-   else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, 2, false>), grid, dim3(64 * WR * WC), 0, s, a);
+   if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, STAGES, KG, true>), grid, dim3(threads), 0, s, a);
+   else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, 2, KG, false>), grid, dim3(threads), 0, s, a);
 }
 template <typename T, int TM> static void launch_narrow(const vadc_amd_linear_args &a, hipStream_t s)
 {
    hipLaunchKernelGGL((k_linear_narrow<T, TM>), dim3((unsigned)(((a.rows + 16 * TM - 1) / (16 * TM)) * ((a.out_features + 15) / 16))), dim3(512), 0, s, a);
 }
+template <int BM, int BN> static void launch_parts(const vadc_amd_linear_args &a, hipStream_t s)
+{
+   const dim3 grid((unsigned)std::min<int64_t>(256 * 2, ((a.rows + BM - 1) / BM) * ((a.out_features + BN - 1) / BN)));
+   hipLaunchKernelGGL((k_linear_parts<BM, BN, 2, 2>), grid, dim3(256), 0, s, a);
+}
 template <typename T> static void launch(const vadc_amd_linear_args &a, hipStream_t s)
 {
    if (a.rows <= 16) return launch_narrow<T, 1>(a, s);
    if (a.rows <= 64) return launch_narrow<T, 4>(a, s);
-   constexpr int64_t per = 16 / sizeof(T);
-   const bool dma = ((uintptr_t)a.x | (uintptr_t)a.weight) % 16 == 0 && a.x_stride % per == 0 && a.weight_stride % per == 0 &&
-                    std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) < (int64_t(1) << 31) / 256;      // a tile's rows within 32-bit offsets
    const auto tiles = [&](int64_t t) { return ((a.rows + t - 1) / t) * ((a.out_features + t - 1) / t); };
-   if constexpr (sizeof(T) == 2) if (tiles(256) >= 200) return launch_tile<T, 256, 256, 2, 4, 128, 2>(a, s, dma);
-   if (tiles(128) >= 200) return launch_tile<T, 128, 128, 2, 2, 128, 2>(a, s, dma);
-   launch_tile<T, 64, 64, 2, 2, 128, 4>(a, s, dma);
+   if constexpr (sizeof(T) == 4) {
+      if (tiles(128) >= 200) launch_parts<128, 128>(a, s);
+      else launch_parts<64, 64>(a, s);
+   } else {
+      const bool dma = ((uintptr_t)a.x | (uintptr_t)a.weight) % 16 == 0 && a.x_stride % 8 == 0 && a.weight_stride % 8 == 0 &&
+                       std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) < (int64_t(1) << 31) / 256;      // a tile's rows within 32-bit offsets
+      if (tiles(256) >= 200) launch_tile<T, 256, 256, 2, 4, 128, 2, 1>(a, s, dma);
+      else if (tiles(128) >= 200) launch_tile<T, 128, 128, 2, 2, 128, 2, 1>(a, s, dma);
+      else if (tiles(64) > 256 || a.in_features < 512) launch_tile<T, 64, 64, 2, 2, 128, 4, 1>(a, s, dma);
+      else launch_tile<T, 64, 64, 2, 2, 128, 4, 2>(a, s, dma);
+   }
 }
 
 void launch_linear(const vadc_amd_linear_args &a, hipStream_t s)
