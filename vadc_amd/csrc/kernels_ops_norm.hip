@@ -12,7 +12,7 @@ namespace ops {
 struct Stats { float n, mean, m2; };
 __device__ __forceinline__ Stats merge(const Stats &a, const Stats &b)
 {
-   const float n = a.n + b.n, d = b.mean - a.mean, w = n > 0.0f ? b.n / n : 0.0f;
+   const float n = a.n + b.n, d = b.mean - a.mean, w = n > 0.0f ? b.n * __builtin_amdgcn_rcpf(n) : 0.0f;      // a step of the reciprocal is one of the mean's distance, no more
    return {n, a.mean + d * w, a.m2 + b.m2 + d * d * (a.n * w)};
 }
 __device__ __forceinline__ Stats shuffle_xor(const Stats &s, int d) { return {__shfl_xor(s.n, d), __shfl_xor(s.mean, d), __shfl_xor(s.m2, d)}; }

@@ -96,11 +96,11 @@ template <typename T> __device__ __forceinline__ void split8(const T (&x)[8], p8
       }
    }
 }
-__device__ __forceinline__ void split4(const f4 &x, p4 (&p)[3])
+template <int N> __device__ __forceinline__ void split4(const f4 &x, p4 (&p)[N])
 {
    f2 lo = {x[0], x[1]}, hi = {x[2], x[3]};
 #pragma unroll
-   for (int k = 0; k < 3; ++k) p[k] = p4{next_part(lo), next_part(hi)};
+   for (int k = 0; k < N; ++k) p[k] = p4{next_part(lo), next_part(hi)};
 }
 __device__ __forceinline__ p8 join(const p4 &lo, const p4 &hi) { return p8{lo[0], lo[1], hi[0], hi[1]}; }
 __device__ __forceinline__ f4 mfma16(const p8 &a, const p8 &b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0); }
@@ -115,16 +115,16 @@ template <int NA, int NB> __device__ __forceinline__ f4 mfma_parts(const p8 (&a)
    return acc;
 }
 // two of them at once, product by product: the matrix pipe has the other's while one's result is under way
-template <int NA, int NB> __device__ __forceinline__ void mfma_parts2(const p8 (&a)[NA], const p8 (&b)[NB], f4 &x, const p8 (&c)[NA], const p8 (&d)[NB], f4 &y)
+template <int NA, int NB, int NC, int ND>
+__device__ __forceinline__ void mfma_parts2(const p8 (&a)[NA], const p8 (&b)[NB], f4 &x, const p8 (&c)[NC], const p8 (&d)[ND], f4 &y)
 {
 #pragma unroll
    for (int o = 2; o >= 0; --o)
 #pragma unroll
-      for (int i = 0; i < NA; ++i)
-         if (o - i >= 0 && o - i < NB) {
-            x = mfma16(a[i], b[o - i], x);
-            y = mfma16(c[i], d[o - i], y);
-         }
+      for (int i = 0; i <= o; ++i) {
+         if (i < NA && o - i < NB) x = mfma16(a[i], b[o - i], x);
+         if (i < NC && o - i < ND) y = mfma16(c[i], d[o - i], y);
+      }
 }
 
 // LDS is ready for the other waves and theirs for this one; global loads stay in flight (__syncthreads would wait for them)
