@@ -42,21 +42,33 @@ __global__ __launch_bounds__(256) void k_delta_step(const vadc_amd_gated_delta_a
    const T *v = (const T *)a.v + stream * a.v_stride[0] + head * a.v_stride[2] + col;
    T *out = (T *)a.out + stream * a.out_stride[0] + head * a.out_stride[2] + col;
    const float *pg = a.log_decay + stream * a.decay_stride[0] + head, *pb = a.beta + stream * a.beta_stride[0] + head;
+   // a step's operands are fetched while the one before is computed; column and row are moved inside where they lie behind the end
+   const int64_t krow = min(tid, kd - 1), vback = live ? 0 : col;
+   T nq, nk, nv[VEC];
+   float ng, nb;
+   const auto fetch = [&](int64_t t) {
+      nq = q[t * a.q_stride[1] + krow]; nk = k[t * a.k_stride[1] + krow];
+      const Pack<T, VEC> u = *reinterpret_cast<const Pack<T, VEC> *>(v + t * a.v_stride[1] - vback);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) nv[j] = u.v[j];
+      ng = pg[t * a.decay_stride[1]]; nb = pb[t * a.beta_stride[1]];
+   };
+   fetch(0);
    for (int64_t t = 0; t < steps; ++t) {
       const int at = t & 1;                                          // two sets of LDS buffers: two barriers a step
-      const float decay = expf(pg[t * a.decay_stride[1]]), beta = pb[t * a.beta_stride[1]];
-      float vv[VEC] = {};
-      if (live) load_f32<T, VEC>(v + t * a.v_stride[1], vv);
-      float qi = 0.0f, ki = 0.0f;
-      if (tid < kd) { qi = (float)q[t * a.q_stride[1] + tid]; ki = (float)k[t * a.k_stride[1] + tid]; }
+      const float decay = expf(ng), beta = nb, qi = tid < kd ? (float)nq : 0.0f, ki = tid < kd ? (float)nk : 0.0f;
+      float vv[VEC];
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) vv[j] = (float)nv[j];
+      if (t + 1 < steps) fetch(t + 1);
       if (tid < 16 * ROWS) { sq[at][tid] = qi; sk[at][tid] = ki; }
       const float qq = sum_lanes(qi * qi, 64), kk = sum_lanes(ki * ki, 64), qk = sum_lanes(qi * ki, 64);
       if (lane == 0) { dots[at][wave][0] = qq; dots[at][wave][1] = kk; dots[at][wave][2] = qk; }
-      __syncthreads();
+      lds_barrier();
       float d[3];
 #pragma unroll
       for (int i = 0; i < 3; ++i) d[i] = (dots[at][0][i] + dots[at][1][i]) + (dots[at][2][i] + dots[at][3][i]);
-      const float rq = a.normalize ? a.scale / sqrtf(d[0] + 1e-6f) : a.scale, rk = a.normalize ? 1.0f / sqrtf(d[1] + 1e-6f) : 1.0f;
+      const float rq = a.normalize ? a.scale * __builtin_amdgcn_rsqf(d[0] + 1e-6f) : a.scale, rk = a.normalize ? __builtin_amdgcn_rsqf(d[1] + 1e-6f) : 1.0f;      // 1 ulp
       float ks[VEC] = {}, qs[VEC] = {};
 #pragma unroll
       for (int i = 0; i < ROWS; ++i)
@@ -67,13 +79,13 @@ __global__ __launch_bounds__(256) void k_delta_step(const vadc_amd_gated_delta_a
          }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {                                // the wave's four rows of threads
-         ks[j] += __shfl_xor(ks[j], 16); ks[j] += __shfl_xor(ks[j], 32);
-         qs[j] += __shfl_xor(qs[j], 16); qs[j] += __shfl_xor(qs[j], 32);
+         ks[j] = plus_half(plus_row(ks[j]));
+         qs[j] = plus_half(plus_row(qs[j]));
       }
       if (lane < 16)
 #pragma unroll
          for (int j = 0; j < VEC; ++j) { part[at][wave][0][c + j] = ks[j]; part[at][wave][1][c + j] = qs[j]; }
-      __syncthreads();
+      lds_barrier();
       float o[VEC];
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -304,7 +316,7 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
 #pragma unroll
          for (int n = 0; n < NT; ++n) *reinterpret_cast<p8 *>(&sk[n][place<KD>(row, (tid & 3) + 4 * s)]) = p[n];
       }
-      if ((tid & 3) == 0) srk[row] = a.normalize ? 1.0f / sqrtf((odd != 0.0f ? 1.0f : kk) + 1e-6f) : 1.0f;
+      if ((tid & 3) == 0) srk[row] = a.normalize ? __builtin_amdgcn_rsqf((odd != 0.0f ? 1.0f : kk) + 1e-6f) : 1.0f;
       float qq = 0.0f;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -314,8 +326,8 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
 #pragma unroll
          for (int i = 0; i < 8; ++i) { const float f = (float)x[i]; qq = fmaf(f, f, qq); }
       }
-      qq += __shfl_xor(qq, 16); qq += __shfl_xor(qq, 32);
-      if (l4 == 0) srq[mine] = a.normalize ? a.scale / sqrtf(qq + 1e-6f) : a.scale;
+      qq = plus_half(plus_row(qq));
+      if (l4 == 0) srq[mine] = a.normalize ? a.scale * __builtin_amdgcn_rsqf(qq + 1e-6f) : a.scale;
    }
    __syncthreads();
    const double gi = sg[mine];
@@ -641,12 +653,18 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
 }
 
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
-// Blocks from 16 steps on, for keys of 8 to 128 and values of 4 and more; the workspace holds as many blocks as stay in the last-level cache between the two launches, longer calls go out in segments of steps
-static bool in_blocks(const vadc_amd_gated_delta_args &a) { return a.steps >= 16 && a.key_dim >= 8 && a.key_dim <= 128 && a.value_dim >= 4; }
+// Blocks for keys of 8 to 128 and values of 4 and more, from as many steps on as they are the faster form.  Step by step a step takes 1.1 us; blocks take two launches and, with many
+// states, whole blocks of work: 1 stream, 16 heads of 128, bfloat16: 16 us up to 64 steps, against 14 for 8 steps and 19 for 12; 256 streams, 4 heads of 64: 56 us, against 41 for 16 steps
+// and 57 for 24; 8 heads of 128: 235 us against 223 for 24.
+static bool in_blocks(const vadc_amd_gated_delta_args &a)
+{
+   return a.steps >= (a.streams * a.heads <= 256 ? 10 : 24) && a.key_dim >= 8 && a.key_dim <= 128 && a.value_dim >= 4;
+}
 // Columns of S per workgroup: with keys of up to 64, 16 -- several workgroups a CU, one computes while another waits at its barriers (61 streams of up to 333 steps, 6 heads of 48 x 80,
 // float32: 70.6 us a launch against 81.3 with 32) --; with longer keys, where staging k and q again for every 16 columns costs more than that gains, 32 (2 x 4096 steps, 32 heads of
 // 128 x 128, bfloat16: 244 us against 269 with 16)
 template <int KD> constexpr int scan_columns() { return KD == 64 ? 16 : 32; }
+// The workspace holds as many blocks as stay in the last-level cache between the two launches (4096 of 37 or 31 KB); longer calls go out in segments of steps
 static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
 {
    const int64_t blocks = (a.steps + kBlock - 1) / kBlock, most = std::max<int64_t>(1, 4096 / (a.streams * a.heads));
