@@ -664,7 +664,8 @@ static bool in_blocks(const vadc_amd_gated_delta_args &a)
 // float32: 70.6 us a launch against 81.3 with 32) --; with longer keys, where staging k and q again for every 16 columns costs more than that gains, 32 (2 x 4096 steps, 32 heads of
 // 128 x 128, bfloat16: 244 us against 269 with 16)
 template <int KD> constexpr int scan_columns() { return KD == 64 ? 16 : 32; }
-// The workspace holds as many blocks as stay in the last-level cache between the two launches (4096 of 37 or 31 KB); longer calls go out in segments of steps
+// The workspace holds 4096 blocks of 37 or 31 KB, which stay in the last-level cache between the two launches; longer calls go out in segments of steps (2 x 8192 steps, 32 heads: 512 us so,
+// 526 with 2048, 504 with 8192)
 static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
 {
    const int64_t blocks = (a.steps + kBlock - 1) / kBlock, most = std::max<int64_t>(1, 4096 / (a.streams * a.heads));

@@ -108,8 +108,8 @@ __device__ __forceinline__ void tile_of(unsigned index, unsigned tiles, int64_t 
    tn = in / high;
 }
 
-// ---- operands in LDS: rows of RB = 64 or 128 bytes, 16-byte pieces, the piece index mixed with the row so that the rows of a fragment lie in different banks
-template <int RB> __device__ __forceinline__ int mixed(int row, int piece) { return RB == 128 ? piece ^ ((row >> 1) & 7) : piece ^ ((row >> 2) & 3); }
+// ---- operands in LDS: rows of RB = 64, 128 or 256 bytes, 16-byte pieces, the piece index mixed with the row so that the rows of a fragment lie in different banks
+template <int RB> __device__ __forceinline__ int mixed(int row, int piece) { return RB == 256 ? piece ^ (row & 15) : RB == 128 ? piece ^ ((row >> 1) & 7) : piece ^ ((row >> 2) & 3); }
 template <int RB> __device__ __forceinline__ int piece_at(int row, int piece) { return row * RB + (mixed<RB>(row, piece) << 4); }
 
 // one product step: 16 k's of a 32 x 32 tile
@@ -489,8 +489,8 @@ template <typename T> static void launch(const vadc_amd_linear_args &a, hipStrea
                        std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) < (int64_t(1) << 31) / 256;      // a tile's rows within 32-bit offsets
       if (tiles(256) >= 200) launch_tile<T, 256, 256, 2, 4, 128, 2, 1>(a, s, dma);
       else if (tiles(128) >= 200) launch_tile<T, 128, 128, 2, 2, 128, 2, 1>(a, s, dma);
-      else if (tiles(64) > 256 || a.in_features < 512) launch_tile<T, 64, 64, 2, 2, 128, 4, 1>(a, s, dma);
-      else launch_tile<T, 64, 64, 2, 2, 128, 4, 2>(a, s, dma);
+      else if (tiles(64) > 256 || a.in_features < 512) launch_tile<T, 64, 64, 2, 2, 256, 2, 1>(a, s, dma);
+      else launch_tile<T, 64, 64, 2, 2, 256, 2, 2>(a, s, dma);
    }
 }
 
