@@ -558,3 +558,42 @@ def test_long_offsets(ops):
     v.copy_(gen(7)(1, 70, 1, 48))
     state = gen(8)(1, 1, 32, 48)
     check_delta(ops, q, k, v, torch.full((1, 70, 1), -0.1, device="cuda"), torch.full((1, 70, 1), 0.5, device="cuda"), state, True)
+
+
+def test_slices_of_a_long_call(ops):
+    """more streams, sequences or rows than one launch takes: the last, short slice takes the form of the others (on its own it would choose another, whose workspace nobody gave)"""
+    for t in (1, 12, 30):
+        q, k, v, g, beta, state = delta_inputs(t, 2049, t, 1, 4, 8, 12, torch.float32, True)
+        check_delta(ops, q, k, v, g, beta, state, True)
+    x = torch.empty(4097, 64, 1024, dtype=torch.bfloat16, device="cuda")
+    x.copy_(gen(1)(1, 64, 1024) + torch.arange(4097, device="cuda")[:, None, None] % 5)
+    got = ops.group_norm(x, 1024)
+    for rows in (slice(0, 3), slice(4094, 4097)):
+        want, spread, _ = norm64(x[rows], 1024, None, None, 1e-5, "none", None, None)
+        within(got[rows], want, norm_tol(want, spread, torch.bfloat16, 64))
+    del x, got
+    x, w = gen(2)(70001, 8).half(), gen(3)(1024, 8).half()
+    want = linear64(x, w, None, "none", None, False)
+    within(ops.linear(x, w), want, linear_tol(x, w, None, None, want, torch.float16))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_linear_of_no_features(ops, dtype):
+    """a sum of nothing, in every form"""
+    dt, b = TYPES[dtype], gen(1)(200).to(TYPES[dtype])
+    for m in (1, 40, 300, 20000):
+        x = torch.empty(m, 0, dtype=dt, device="cuda")
+        assert torch.equal(ops.linear(x, torch.empty(200, 0, dtype=dt, device="cuda"), bias=b), b.expand(m, 200))
+
+
+def test_broadcast_inputs(ops):
+    """rows, heads and streams that are one piece of memory"""
+    rnd = gen(4)
+    x, w, r = rnd(1, 64).bfloat16().expand(300, 64), rnd(96, 64).bfloat16(), rnd(1, 96).bfloat16().expand(300, 96)
+    want = linear64(x, w, None, "none", r, False)
+    within(ops.linear(x, w, residual=r), want, linear_tol(x, w, None, r, want, torch.bfloat16))
+    z = rnd(1, 64).expand(50, 64)
+    want, spread, _ = norm64(z[:, None], 4, None, None, 1e-5, "none", None, None)
+    within(ops.group_norm(z, 4), want[:, 0], norm_tol(want, spread, torch.float32, 24)[:, 0])
+    q, k, v, g, beta, state = delta_inputs(3, 2, 70, 2, 4, 32, 32, torch.bfloat16, True)
+    check_delta(ops, q[:, :, :1].expand(2, 70, 2, 32), k[:1].expand(2, 70, 2, 32), v[:, :, :1].expand(2, 70, 4, 32), g, beta, state, True)

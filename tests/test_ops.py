@@ -61,6 +61,7 @@ def test_linear_refuses(kw, error):
     (dict(x=t(8), groups=2), ValueError),
     (dict(x=t(3, 8), groups=3), ValueError),
     (dict(x=t(3, 8), groups=0), ValueError),
+    (dict(x=t(3, 8), groups=2.0), TypeError),
     (dict(x=t(3, 8), groups=2, eps=-1.0), ValueError),
     (dict(x=t(3, 8), groups=2, eps=float("nan")), ValueError),
     (dict(x=t(3, 8), groups=2, weight=t(4)), ValueError),

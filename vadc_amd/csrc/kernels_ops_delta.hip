@@ -671,10 +671,10 @@ static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
    const int64_t blocks = (a.steps + kBlock - 1) / kBlock, most = std::max<int64_t>(1, 4096 / (a.streams * a.heads));
    return std::min(blocks, most);
 }
-template <typename T, int KD> static void launch_blocks(const vadc_amd_gated_delta_args &a, hipStream_t s)
+template <typename T, int KD> static void launch_blocks(const vadc_amd_gated_delta_args &a, const vadc_amd_gated_delta_args &first, hipStream_t s)
 {
    constexpr int cols = scan_columns<KD>();
-   const int64_t step = segment_blocks(a), tiles = (a.value_dim + cols - 1) / cols;
+   const int64_t step = segment_blocks(first), tiles = (a.value_dim + cols - 1) / cols;
    for (Segment seg = {0, 0}; seg.from < a.steps; seg.from += step * kBlock) {
       seg.blocks = std::min(step, (a.steps - seg.from + kBlock - 1) / kBlock);
       hipLaunchKernelGGL((k_delta_blocks<T, KD>), dim3((unsigned)(a.streams * a.heads * seg.blocks)), dim3(256), 0, s, a, seg);
@@ -682,9 +682,9 @@ template <typename T, int KD> static void launch_blocks(const vadc_amd_gated_del
    }
 }
 
-template <typename T> static void launch(const vadc_amd_gated_delta_args &a, hipStream_t s)
+template <typename T> static void launch(const vadc_amd_gated_delta_args &a, const vadc_amd_gated_delta_args &first, hipStream_t s)
 {
-   if (in_blocks(a)) return a.key_dim <= 64 ? launch_blocks<T, 64>(a, s) : launch_blocks<T, 128>(a, s);
+   if (in_blocks(first)) return a.key_dim <= 64 ? launch_blocks<T, 64>(a, first, s) : launch_blocks<T, 128>(a, first, s);
    const bool four = a.value_dim % 4 == 0;
    if (a.key_dim <= 64) four ? launch_step<T, 4, 4>(a, s) : launch_step<T, 1, 4>(a, s);
    else if (a.key_dim <= 128) four ? launch_step<T, 4, 8>(a, s) : launch_step<T, 1, 8>(a, s);
@@ -696,11 +696,11 @@ int64_t gated_delta_workspace(const vadc_amd_gated_delta_args &a)
    return in_blocks(a) ? a.streams * a.heads * segment_blocks(a) * (int64_t)(a.dtype == VADC_AMD_F32 ? sizeof(BlockData<float>) : sizeof(BlockData<__bf16>)) : 0;
 }
 
-void launch_gated_delta(const vadc_amd_gated_delta_args &a, hipStream_t s)
+void launch_gated_delta(const vadc_amd_gated_delta_args &a, const vadc_amd_gated_delta_args &first, hipStream_t s)
 {
-   if (a.dtype == VADC_AMD_F32) launch<float>(a, s);
-   else if (a.dtype == VADC_AMD_F16) launch<_Float16>(a, s);
-   else launch<__bf16>(a, s);
+   if (a.dtype == VADC_AMD_F32) launch<float>(a, first, s);
+   else if (a.dtype == VADC_AMD_F16) launch<_Float16>(a, first, s);
+   else launch<__bf16>(a, first, s);
 }
 
 }  // namespace ops

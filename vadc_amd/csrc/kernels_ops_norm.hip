@@ -232,9 +232,9 @@ static Shape shape_of(const vadc_amd_group_norm_args &a, int vec)
    return h;
 }
 
-template <typename T, int VEC> static void launch_columns(const vadc_amd_group_norm_args &a, hipStream_t s)
+template <typename T, int VEC> static void launch_columns(const vadc_amd_group_norm_args &a, const vadc_amd_group_norm_args &first, hipStream_t s)
 {
-   const Shape h = shape_of(a, VEC);
+   const Shape h = shape_of(first, VEC);
    const int64_t others = a.sequences * h.chunks;
    if (h.spans == 1) {
       hipLaunchKernelGGL((k_norm_columns<T, VEC, kWhole>), dim3((unsigned)others), dim3(256), 0, s, a, h);
@@ -243,10 +243,10 @@ template <typename T, int VEC> static void launch_columns(const vadc_amd_group_n
       hipLaunchKernelGGL((k_norm_columns<T, VEC, kApply>), dim3((unsigned)(others * h.apply_spans)), dim3(256), 0, s, a, h);
    }
 }
-template <typename T, int VEC> static void launch_vec(const vadc_amd_group_norm_args &a, hipStream_t s)
+template <typename T, int VEC> static void launch_vec(const vadc_amd_group_norm_args &a, const vadc_amd_group_norm_args &first, hipStream_t s)
 {
    const int64_t per = a.channels / a.groups / VEC, items = a.sequences * a.groups;
-   if (a.positions > 1 || per > 512) return launch_columns<T, VEC>(a, s);     // a group of more than 512 vectors does not fit a wave's registers
+   if (a.positions > 1 || per > 512) return launch_columns<T, VEC>(a, first, s);     // a group of more than 512 vectors does not fit a wave's registers
    int lanes = 1;
    while (lanes < 64 && lanes < per) lanes *= 2;
    const int r = (int)((per + lanes - 1) / lanes);
@@ -256,13 +256,13 @@ template <typename T, int VEC> static void launch_vec(const vadc_amd_group_norm_
    else if (r <= 4) hipLaunchKernelGGL((k_norm_token<T, VEC, 4>), grid, dim3(256), 0, s, a, lanes, (unsigned)items);
    else hipLaunchKernelGGL((k_norm_token<T, VEC, 8>), grid, dim3(256), 0, s, a, lanes, (unsigned)items);
 }
-template <typename T> static void launch(const vadc_amd_group_norm_args &a, hipStream_t s)
+template <typename T> static void launch(const vadc_amd_group_norm_args &a, const vadc_amd_group_norm_args &first, hipStream_t s)
 {
    const int v = vector_of(a);
-   if constexpr (sizeof(T) == 2) if (v == 8) return launch_vec<T, 8>(a, s);
-   if (v == 4) launch_vec<T, 4>(a, s);
-   else if (v == 2) launch_vec<T, 2>(a, s);
-   else launch_vec<T, 1>(a, s);
+   if constexpr (sizeof(T) == 2) if (v == 8) return launch_vec<T, 8>(a, first, s);
+   if (v == 4) launch_vec<T, 4>(a, first, s);
+   else if (v == 2) launch_vec<T, 2>(a, first, s);
+   else launch_vec<T, 1>(a, first, s);
 }
 
 int64_t group_norm_workspace(const vadc_amd_group_norm_args &a)
@@ -272,11 +272,11 @@ int64_t group_norm_workspace(const vadc_amd_group_norm_args &a)
    return h.spans == 1 ? 0 : a.sequences * h.spans * a.groups * (int64_t)sizeof(float3);
 }
 
-void launch_group_norm(const vadc_amd_group_norm_args &a, hipStream_t s)
+void launch_group_norm(const vadc_amd_group_norm_args &a, const vadc_amd_group_norm_args &first, hipStream_t s)
 {
-   if (a.dtype == VADC_AMD_F32) launch<float>(a, s);
-   else if (a.dtype == VADC_AMD_F16) launch<_Float16>(a, s);
-   else launch<__bf16>(a, s);
+   if (a.dtype == VADC_AMD_F32) launch<float>(a, first, s);
+   else if (a.dtype == VADC_AMD_F16) launch<_Float16>(a, first, s);
+   else launch<__bf16>(a, first, s);
 }
 
 }  // namespace ops

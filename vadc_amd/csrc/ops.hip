@@ -127,11 +127,18 @@ const void *ahead(const void *p, int64_t elements, int64_t w) { return p ? (cons
 
 // ---- slices: of rows, sequences or streams, as many as one launch takes; launches of one stream follow each other, so that all slices may use one workspace
 int64_t rows_per_launch(const vadc_amd_linear_args &a) { return std::max<int64_t>(1, kMaxBlocks / ((a.out_features + 15) / 16)); }
-int64_t sequences_per_launch(const vadc_amd_group_norm_args &a) { return std::max<int64_t>(1, kMaxBlocks / a.groups); }
-int64_t streams_per_launch(const vadc_amd_gated_delta_args &a)
+vadc_amd_group_norm_args first_slice(const vadc_amd_group_norm_args &a)
+{
+   vadc_amd_group_norm_args s = a;
+   s.sequences = std::min(a.sequences, std::max<int64_t>(1, kMaxBlocks / a.groups));
+   return s;
+}
+vadc_amd_gated_delta_args first_slice(const vadc_amd_gated_delta_args &a)
 {
    const int64_t most = kMaxBlocks / (a.heads * ((a.value_dim + 15) / 16));
-   return std::max<int64_t>(1, a.steps > 1 ? std::min(most, 8192 / a.heads) : most);      // many steps: a slice's workspace has a block of each head at once
+   vadc_amd_gated_delta_args s = a;
+   s.streams = std::min(a.streams, std::max<int64_t>(1, a.steps > 1 ? std::min(most, 8192 / a.heads) : most));      // many steps: a slice's workspace has a block of each head at once
+   return s;
 }
 
 }  // namespace
@@ -156,9 +163,7 @@ extern "C" int64_t vadc_amd_group_norm_workspace(const vadc_amd_group_norm_args 
 {
    if (int rc = check_norm(a)) return rc;
    if (a->sequences == 0 || a->positions == 0 || a->channels == 0) return 0;
-   vadc_amd_group_norm_args s = *a;
-   s.sequences = std::min(a->sequences, sequences_per_launch(*a));
-   return vadc::ops::group_norm_workspace(s);
+   return vadc::ops::group_norm_workspace(first_slice(*a));
 }
 
 extern "C" int vadc_amd_group_norm(const vadc_amd_group_norm_args *a, void *hip_stream)
@@ -176,12 +181,13 @@ extern "C" int vadc_amd_group_norm(const vadc_amd_group_norm_args *a, void *hip_
       return fail(VADC_AMD_EINVAL, "group_norm: the workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
    OnDevice d;
    if (int rc = d.enter(a->device, "group_norm")) return rc;
-   for (int64_t from = 0, most = sequences_per_launch(*a); from < a->sequences; from += most) {
+   const vadc_amd_group_norm_args first = first_slice(*a);
+   for (int64_t from = 0, most = first.sequences; from < a->sequences; from += most) {
       vadc_amd_group_norm_args s = *a;
       s.sequences = std::min(most, a->sequences - from);
       s.x = ahead(a->x, from * a->x_stride[0], w); s.gate = ahead(a->gate, from * a->gate_stride[0], w); s.out = (void *)ahead(a->out, from * a->out_stride[0], w);
       s.lengths = (const int32_t *)ahead(a->lengths, from, 4);
-      vadc::ops::launch_group_norm(s, (hipStream_t)hip_stream);
+      vadc::ops::launch_group_norm(s, first, (hipStream_t)hip_stream);
    }
    return d.left("group_norm");
 }
@@ -190,9 +196,7 @@ extern "C" int64_t vadc_amd_gated_delta_workspace(const vadc_amd_gated_delta_arg
 {
    if (int rc = check_delta(a)) return rc;
    if (a->streams == 0 || a->steps == 0 || a->heads == 0 || a->value_dim == 0) return 0;
-   vadc_amd_gated_delta_args s = *a;
-   s.streams = std::min(a->streams, streams_per_launch(*a));
-   return vadc::ops::gated_delta_workspace(s);
+   return vadc::ops::gated_delta_workspace(first_slice(*a));
 }
 
 extern "C" int vadc_amd_gated_delta(const vadc_amd_gated_delta_args *a, void *hip_stream)
@@ -211,14 +215,15 @@ extern "C" int vadc_amd_gated_delta(const vadc_amd_gated_delta_args *a, void *hi
       return fail(VADC_AMD_EINVAL, "gated_delta: the workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
    OnDevice d;
    if (int rc = d.enter(a->device, "gated_delta")) return rc;
-   for (int64_t from = 0, most = streams_per_launch(*a); from < a->streams; from += most) {
+   const vadc_amd_gated_delta_args first = first_slice(*a);
+   for (int64_t from = 0, most = first.streams; from < a->streams; from += most) {
       vadc_amd_gated_delta_args s = *a;
       s.streams = std::min(most, a->streams - from);
       s.q = ahead(a->q, from * a->q_stride[0], w); s.k = ahead(a->k, from * a->k_stride[0], w); s.v = ahead(a->v, from * a->v_stride[0], w);
       s.out = (void *)ahead(a->out, from * a->out_stride[0], w);
       s.log_decay = a->log_decay + from * a->decay_stride[0]; s.beta = a->beta + from * a->beta_stride[0]; s.state = a->state + from * a->state_stride;
       s.lengths = (const int32_t *)ahead(a->lengths, from, 4);
-      vadc::ops::launch_gated_delta(s, (hipStream_t)hip_stream);
+      vadc::ops::launch_gated_delta(s, first, (hipStream_t)hip_stream);
    }
    return d.left("gated_delta");
 }

@@ -218,6 +218,8 @@ def _plan_norm(x, groups, weight, bias, eps, activation, gate, lengths, out) -> 
     if len(x.shape) not in (2, 3):
         raise ValueError(f"group_norm: x {tuple(x.shape)} is neither [sequences, positions, channels] nor [tokens, channels]")
     n, l, c = x.shape if len(x.shape) == 3 else (x.shape[0], 1, x.shape[1])
+    if not isinstance(groups, int):
+        raise TypeError(f"group_norm: groups must be a whole number, not {groups!r}")
     if groups < 1 or c % groups:
         raise ValueError(f"group_norm: {c} channels do not divide into {groups} groups")
     if not 0 <= eps < float("inf"):
