@@ -43,11 +43,12 @@ __device__ __forceinline__ void finish(const vadc_amd_linear_args &a, const T *r
    if (a.residual && !a.residual_first)
 #pragma unroll
       for (int i = 0; i < N; ++i) y[i] += r[i];
-   if (left >= N) store_f32<T, N>(out, y);
-   else
+   if (left < N) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
          if (i < left) out[i] = (T)y[i];
+   } else if (a.rows * a.out_features * (int64_t)sizeof(T) >= kStreamBytes) stream_f32<T, N>(out, y);
+   else store_f32<T, N>(out, y);
 }
 
 // Outputs leave through LDS, 32 rows of FEATS of the wave's features at a time in float32, so that a row's features leave (and its residuals come) as one run, 16 bytes to a lane: a

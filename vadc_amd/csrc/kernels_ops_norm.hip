@@ -47,7 +47,8 @@ __device__ __forceinline__ void apply(const vadc_amd_group_norm_args &a, const f
 #pragma unroll
       for (int i = 0; i < VEC; ++i) y[i] *= g[i];
    } else activate_all<VEC>(y, a.activation);
-   store_f32<T, VEC>(out, y);
+   if (a.sequences * a.positions * a.channels * (int64_t)sizeof(T) >= kStreamBytes) stream_f32<T, VEC>(out, y);
+   else store_f32<T, VEC>(out, y);
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void affine(const vadc_amd_group_norm_args &a, int64_t c, float (&w)[VEC], float (&b)[VEC])
