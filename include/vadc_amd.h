@@ -361,7 +361,8 @@ int  vadc_amd_group_norm(const vadc_amd_group_norm_args *args, void *hip_stream)
  * (each stream's part contiguous).  heads is a multiple of key_heads: head h reads key head h / (heads / key_heads).  1 <= key_dim <= 256.  normalize: q and k are divided by
  * sqrt(sum of squares + 1e-6) first.  log_decay <= 0 (-inf: the state is forgotten); keys of length one at most keep the recurrence stable, as its definition needs.
  * lengths [streams] (int32, on the device; NULL = none): stream b has its first lengths[b] steps only (clamped to 0 ... steps); the rest of its inputs is not read, the rest of its
- * output not written; a stream of no steps keeps its state.  workspace: as above. */
+ * output not written; a stream of no steps keeps its state.  A value that is not finite makes NaN of what it reaches, from its step on: its column of its head's state and outputs (a key or
+ * gate: every column, a query: its own outputs); nothing before it, beside it or in another head.  workspace: as above. */
 typedef struct vadc_amd_gated_delta_args {
    const void *q, *k, *v;
    const float *log_decay, *beta;
