@@ -81,6 +81,28 @@ def test_linear(ops, m, k, n, dtype):
     within(got, want, linear_tol(x, w, b, r, want, dt))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, k, n", [(100, 640, 70), (100, 513, 70), (90, 1153, 200), (1700, 200, 1800), (1700, 201, 1800), (3000, 200, 4000), (3000, 65, 4000), (8200, 129, 4100), (8200, 136, 4100)])
+def test_linear_several_tiles_a_workgroup(ops, m, k, n, dtype):
+    """more tiles than workgroups, groups of waves with unequal shares of k; odd k: rows at every alignment"""
+    dt, rnd = TYPES[dtype], gen(m + k)
+    x, w, b = rnd(m, k).to(dt), (rnd(n, k) * k ** -0.5).to(dt), rnd(n).to(dt)
+    want = linear64(x, w, b, "relu", None, False)
+    within(ops.linear(x, w, bias=b, activation="relu"), want, linear_tol(x, w, b, None, want, dt))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m, k, n", [(100, 131, 70), (300, 515, 140), (2000, 67, 3000), (9000, 65, 4000)])
+def test_linear_part_of_a_piece(ops, m, k, n, dtype):
+    """16-byte aligned rows that end inside 16 bytes; what lies behind their ends is NaN"""
+    dt, rnd = TYPES[dtype], gen(m + k)
+    x, w = torch.full((m, k + 8 - k % 8), math.nan, dtype=dt, device="cuda"), torch.full((n, k + 16 - k % 8), math.nan, dtype=dt, device="cuda")
+    x[:, :k], w[:, :k] = rnd(m, k).to(dt), (rnd(n, k) * k ** -0.5).to(dt)
+    x, w = x[:, :k], w[:, :k]
+    want = linear64(x, w, None, "none", None, False)
+    within(ops.linear(x, w), want, linear_tol(x, w, None, None, want, dt))
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("mode", ("none", "after", "before"))
 @pytest.mark.parametrize("m", (3, 40, 300))

@@ -50,6 +50,7 @@ def test_argument_structs_are_packed_as_the_header_lays_them_out(tmp_path):
     (dict(x=t(5, 3).T, weight=t(4, 5)), ValueError),                 # the last dimension is not contiguous
     (dict(x=t(3, 5), weight=t(5, 4).T), ValueError),
     (dict(x=t(3, 5), weight=t(4, 5).requires_grad_()), ValueError),
+    (dict(x=t(3, 5), weight=t(4, 5), residual_first=t(1)), TypeError),
     (dict(x=t(3, 5), weight=t(4, 5)), ValueError),                   # no device
 ])
 def test_linear_refuses(kw, error):
@@ -62,6 +63,8 @@ def test_linear_refuses(kw, error):
     (dict(x=t(3, 8), groups=3), ValueError),
     (dict(x=t(3, 8), groups=0), ValueError),
     (dict(x=t(3, 8), groups=2.0), TypeError),
+    (dict(x=t(3, 8), groups=2, eps=t(1)), TypeError),
+    (dict(x=t(3, 8), groups=2, eps=1e39), ValueError),
     (dict(x=t(3, 8), groups=2, eps=-1.0), ValueError),
     (dict(x=t(3, 8), groups=2, eps=float("nan")), ValueError),
     (dict(x=t(3, 8), groups=2, weight=t(4)), ValueError),
@@ -100,6 +103,10 @@ def delta_args(b=2, steps=3, hk=1, h=2, dk=4, dv=5, **kw):
     (dict(v=t(2, 3, 2, 5, dtype=torch.float16)), TypeError),
     (dict(out=t(2, 3, 5, 2)), ValueError),
     (dict(lengths=torch.zeros(2)), TypeError),
+    (dict(scale=t(1)), TypeError),
+    (dict(normalize=t(1)), TypeError),
+    (dict(scale=float("inf")), ValueError),
+    (dict(scale=float("nan")), ValueError),
     (dict(lengths=torch.zeros(3, dtype=torch.int32)), ValueError),
     (dict(q=t(2, 3, 1, 8)[..., ::2]), ValueError),
     (dict(state=t(2, 2, 4, 5).requires_grad_()), ValueError),

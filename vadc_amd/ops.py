@@ -12,6 +12,7 @@ argument raises ValueError or TypeError before the device is touched, a failure 
 from __future__ import annotations
 
 import functools
+import numbers
 import struct
 from typing import NamedTuple, Optional
 
@@ -81,6 +82,15 @@ def _same_device(what: str, *ls: Optional[_Layout]) -> int:
     if d.type != "cuda":
         raise ValueError(f"{what}: tensors must be on a gfx950 device, not on {d} (vadc_amd has no CPU fallback)")
     return d.index
+
+
+_LARGEST = 3.4e38            # of float32, short of its last digits
+
+
+def _flag(what: str, **flags):
+    for name, v in flags.items():
+        if not isinstance(v, (bool, int)):           # a tensor's truth would be read once and kept
+            raise TypeError(f"{what}: {name} must be True or False, not {v!r}")
 
 
 def _activation(what: str, name: str) -> int:
@@ -180,6 +190,7 @@ def _plan_linear(x, weight, bias, residual, out, activation, residual_first) -> 
     _shaped("linear", (n,), bias=bias)
     _shaped("linear", shape, residual=residual, out=out)
     act = _activation("linear", activation)
+    _flag("linear", residual_first=residual_first)
     dtype = _same_dtype("linear", x, weight, bias, residual, out)
     _inner("linear", x=x, weight=weight, bias=bias, residual=residual, out=out)
     _distinct("linear", out)
@@ -218,11 +229,11 @@ def _plan_norm(x, groups, weight, bias, eps, activation, gate, lengths, out) -> 
     if len(x.shape) not in (2, 3):
         raise ValueError(f"group_norm: x {tuple(x.shape)} is neither [sequences, positions, channels] nor [tokens, channels]")
     n, l, c = x.shape if len(x.shape) == 3 else (x.shape[0], 1, x.shape[1])
-    if not isinstance(groups, int):
-        raise TypeError(f"group_norm: groups must be a whole number, not {groups!r}")
+    if not isinstance(groups, numbers.Integral) or not isinstance(eps, numbers.Real):
+        raise TypeError(f"group_norm: groups must be a whole number, eps a number, not {groups!r}, {eps!r}")
     if groups < 1 or c % groups:
         raise ValueError(f"group_norm: {c} channels do not divide into {groups} groups")
-    if not 0 <= eps < float("inf"):
+    if not 0 <= eps <= _LARGEST:
         raise ValueError(f"group_norm: eps {eps} must be finite and not negative")
     _shaped("group_norm", (c,), weight=weight, bias=bias)
     _shaped("group_norm", x.shape, gate=gate, out=out)
@@ -286,9 +297,12 @@ def _plan_delta(q, k, v, log_decay, beta, state, scale, normalize, lengths, out)
     part = dk * dv
     if 0 not in state.shape and any(n > 1 and have != want for n, have, want in zip(state.shape[1:], state.stride[1:], (part, dv, 1))):
         raise ValueError("gated_delta: each stream's part of state must be contiguous")
+    _flag("gated_delta", normalize=normalize)
+    if scale is not None and not isinstance(scale, numbers.Real):
+        raise TypeError(f"gated_delta: scale must be a number, not {scale!r}")
     scale = dk ** -0.5 if scale is None else float(scale)
-    if not abs(scale) < float("inf"):
-        raise ValueError("gated_delta: scale must be finite")
+    if not abs(scale) <= _LARGEST:
+        raise ValueError(f"gated_delta: scale {scale} must be finite")
     device = _same_device("gated_delta", q, k, v, log_decay, beta, state, lengths, out)
     empty = 0 in v.shape
     fields = (b, t, hk, h, dk, dv, *q.stride[:3], *k.stride[:3], *v.stride[:3], *(out.stride[:3] if out else (t * h * dv, h * dv, dv)), *log_decay.stride[:2], *beta.stride[:2],
