@@ -103,6 +103,32 @@ def test_linear_part_of_a_piece(ops, m, k, n, dtype):
     within(ops.linear(x, w), want, linear_tol(x, w, None, None, want, dt))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset, gap", [(0, 0), (1, 0), (1, 2), (3, 1), (0, 1), (2, 2)])
+@pytest.mark.parametrize("m, n", [(1, 37), (16, 16), (17, 90), (32, 33), (33, 70), (64, 129), (65, 20), (1025, 1900)])
+def test_linear_any_alignment(ops, m, n, offset, gap, dtype):
+    """rows that begin and end anywhere, k's from one up; what lies around them is NaN"""
+    dt, rnd = TYPES[dtype], gen(m + n)
+    for k in (1, 3, 7, 8, 9, 15, 17, 63, 64, 65, 127, 129) if m > 1000 else (1, 2, 5, 7, 8, 9, 16, 31, 63, 64, 65, 127, 128, 129, 511, 513, 575, 577, 1031, 1217):
+        x, w = (torch.full((offset + r * (k + gap),), math.nan, dtype=dt, device="cuda")[offset:].view(r, k + gap)[:, :k] for r in (m, n))
+        x.copy_(rnd(m, k))
+        w.copy_(rnd(n, k) * k ** -0.5)
+        want = linear64(x, w, None, "none", None, False)
+        within(ops.linear(x, w), want, linear_tol(x, w, None, None, want, dt))
+
+
+def test_linear_rows_far_apart(ops):
+    """rows further apart than 32-bit offsets within a tile reach"""
+    m, n, k, rnd = 70, 200, 131, gen(5)
+    x = torch.empty(m, 4_200_001, dtype=torch.bfloat16, device="cuda")[:, :k]
+    x.copy_(rnd(m, k))
+    w = rnd(n, k).bfloat16()
+    want = linear64(x, w, None, "none", None, False)
+    within(ops.linear(x, w), want, linear_tol(x, w, None, None, want, torch.bfloat16))
+    want = linear64(w, x, None, "none", None, False)
+    within(ops.linear(w, x), want, linear_tol(w, x, None, None, want, torch.bfloat16))
+
+
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("mode", ("none", "after", "before"))
 @pytest.mark.parametrize("m", (3, 40, 300))

@@ -3,6 +3,7 @@
 #include "ops_prims.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace vadc {
 namespace ops {
@@ -15,6 +16,7 @@ typedef unsigned __int128 u128;
 template <typename T> __device__ __forceinline__ u128 load_end(const T *from, int64_t k, int64_t n)
 {
    constexpr int PER = 16 / (int)sizeof(T), BITS = 8 * (int)sizeof(T);
+   typedef std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t> bits;
    u128 u = 0;
    if (n >= PER) {
       const int over = (int)min(max(k - (n - PER), (int64_t)0), (int64_t)PER);
@@ -22,8 +24,26 @@ template <typename T> __device__ __forceinline__ u128 load_end(const T *from, in
       u = over == PER ? (u128)0 : u >> (over * BITS);
    } else
 #pragma unroll 1
-      for (int i = (int)min(n - k, (int64_t)PER) - 1; i >= 0; --i) u = u << BITS | __builtin_bit_cast(unsigned short, from[i]);
+      for (int i = (int)min(n - k, (int64_t)PER) - 1; i >= 0; --i) u = u << BITS | __builtin_bit_cast(bits, from[i]);
    return u;
+}
+
+// 16 values in one run.  ODD: two-byte values may begin within a dword, where a wide load takes about four times as long: whole dwords are loaded and shifted; the last dword is the one
+// that the last value lies in (16 x 4095 x 4095 bfloat16: 27 us with loads from where the values begin, 11 us so; rows that need no shift lose 3 of 10 us by it)
+template <typename T, bool ODD> __device__ __forceinline__ void load16(const T *from, T (&x)[16])
+{
+   if constexpr (!ODD) __builtin_memcpy(x, from, sizeof(x));
+   else {
+      static_assert(sizeof(T) == 2, "a float begins where a dword does");
+      const uint32_t in = (uint32_t)(uintptr_t)from & 3;
+      const char *base = (const char *)from - in;
+      uint32_t d[9];
+      __builtin_memcpy(d, __builtin_assume_aligned(base, 4), 32);
+      __builtin_memcpy(&d[8], __builtin_assume_aligned(base + 28 + 2 * in, 4), 4);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = __builtin_amdgcn_alignbyte(d[i + 1], d[i], in);
+      __builtin_memcpy(x, d, sizeof(x));
+   }
 }
 
 // The epilogue of N consecutive output features of one row: bias, residual, activation in float32, one rounding at the end.  `left` features are left in the row.
@@ -424,12 +444,12 @@ __global__ __launch_bounds__(256, 2) void k_linear_parts(const vadc_amd_linear_a
 // ---- few rows: the weight goes once through registers, nothing is shared -------------------------------------------------------------------------------
 // A workgroup does 16 features of up to 16 TM rows; its eight waves take every eighth 64 k's and add up in LDS in a fixed order.  A lane reads 32 (float32: 64) consecutive bytes of its
 // row, so that the four lanes of a row read a run: the k's of an operand fragment may come in any order that both operands share.
-template <typename T, int TM>
+template <typename T, int TM, bool ODD>
 __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_args a)
 {
    constexpr int WAVES = 8;
    __shared__ __attribute__((aligned(16))) f4 part[WAVES][TM][64];
-   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, l15 = lane & 15, l4 = lane >> 4;
+   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, l4 = lane >> 4;
    const int64_t tiles_n = (a.out_features + 15) / 16, row0 = blockIdx.x / tiles_n * (16 * TM), col0 = blockIdx.x % tiles_n * 16;
    const T *pw = (const T *)a.weight + min(col0 + l15, a.out_features - 1) * a.weight_stride, *px[TM];
 #pragma unroll
@@ -437,37 +457,63 @@ __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_arg
    f4 acc[TM];
 #pragma unroll
    for (int j = 0; j < TM; ++j) acc[j] = (f4)(0.0f);
-   const auto load16 = [&](const T *p, int64_t k, T (&x)[16]) {
-      const int64_t left = a.in_features - k;
-      if (left >= 16) {
-         const Pack<T, 16> u = *reinterpret_cast<const Pack<T, 16> *>(p + k);
-#pragma unroll
-         for (int i = 0; i < 16; ++i) x[i] = u.v[i];
-      } else
-#pragma unroll
-         for (int i = 0; i < 16; ++i) x[i] = i < left ? p[k + i] : (T)0.0f;
-   };
-   for (int64_t k = 64 * wave; k < a.in_features; k += 64 * WAVES) {
-      T w[16], x[TM][16];
-      load16(pw, k + 16 * l4, w);
-#pragma unroll
-      for (int j = 0; j < TM; ++j) load16(px[j], k + 16 * l4, x[j]);
+   struct Held { T w[16], x[TM][16]; };
+   const auto products = [&](const Held &h) {
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
          if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int s = 0; s < 16; ++s) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[s], x[j][s], acc[j], 0, 0, 0);
+            for (int s = 0; s < 16; ++s) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(h.w[s], h.x[j][s], acc[j], 0, 0, 0);
          } else {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                p8 fa, fb;
-               __builtin_memcpy(&fa, &w[8 * s], sizeof(fa));
-               __builtin_memcpy(&fb, &x[j][8 * s], sizeof(fb));
+               __builtin_memcpy(&fa, &h.w[8 * s], sizeof(fa));
+               __builtin_memcpy(&fb, &h.x[j][8 * s], sizeof(fb));
                if constexpr (__is_same(T, __bf16)) acc[j] = mfma16(fa, fb, acc[j]);
                else acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, fa), __builtin_bit_cast(h8, fb), acc[j], 0, 0, 0);
             }
          }
       }
+   };
+   // Whole pieces of 64 k's in a loop of their own; at most one wave has the part at the end
+   const auto load = [&](int64_t k, Held &h) {
+      load16<T, ODD>(pw + k + 16 * l4, h.w);
+#pragma unroll
+      for (int j = 0; j < TM; ++j) load16<T, ODD>(px[j] + k + 16 * l4, h.x[j]);
+   };
+   Held even, odd;
+   int64_t k = 64 * wave;
+   if constexpr (TM == 1) {                                           // the next piece's loads are on their way under a piece's products (1 x 4096 x 4096 float32: 20.0 us without, 16.7 us so)
+      if (k + 64 <= a.in_features) load(k, even);
+      while (k + 64 <= a.in_features) {
+         k += 64 * WAVES;
+         const bool more = k + 64 <= a.in_features;
+         if (more) load(k, odd);
+         products(even);
+         if (!more) break;
+         k += 64 * WAVES;
+         if (k + 64 <= a.in_features) load(k, even);
+         products(odd);
+      }
+   } else                                                             // there is enough on its way (64 x 4096 x 4096 float32: 39.7 us so, 46.5 us as above)
+      for (; k + 64 <= a.in_features; k += 64 * WAVES) {
+         load(k, even);
+         products(even);
+      }
+   if (k < a.in_features) {
+      k += 16 * l4;
+#pragma unroll
+      for (int i = 0; i < 16; i += 16 / (int)sizeof(T)) {
+         const u128 u = load_end(pw + k + i, k + i, a.in_features);
+         __builtin_memcpy(&even.w[i], &u, 16);
+#pragma unroll
+         for (int j = 0; j < TM; ++j) {
+            const u128 v = load_end(px[j] + k + i, k + i, a.in_features);
+            __builtin_memcpy(&even.x[j][i], &v, 16);
+         }
+      }
+      products(even);
    }
 #pragma unroll
    for (int j = 0; j < TM; ++j) part[wave][j][lane] = acc[j];
@@ -495,7 +541,13 @@ template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES, int KG
 }
 template <typename T, int TM> static void launch_narrow(const vadc_amd_linear_args &a, hipStream_t s)
 {
-   hipLaunchKernelGGL((k_linear_narrow<T, TM>), dim3((unsigned)(((a.rows + 16 * TM - 1) / (16 * TM)) * ((a.out_features + 15) / 16))), dim3(512), 0, s, a);
+   const dim3 grid((unsigned)(((a.rows + 16 * TM - 1) / (16 * TM)) * ((a.out_features + 15) / 16)));
+   if constexpr (sizeof(T) == 2)
+      if (((uintptr_t)a.x | (uintptr_t)a.weight) % 4 || a.x_stride % 2 || a.weight_stride % 2) {
+         hipLaunchKernelGGL((k_linear_narrow<T, TM, true>), grid, dim3(512), 0, s, a);
+         return;
+      }
+   hipLaunchKernelGGL((k_linear_narrow<T, TM, false>), grid, dim3(512), 0, s, a);
 }
 template <int BM, int BN> static void launch_parts(const vadc_amd_linear_args &a, hipStream_t s)
 {
@@ -505,13 +557,15 @@ template <int BM, int BN> static void launch_parts(const vadc_amd_linear_args &a
 template <typename T> static void launch(const vadc_amd_linear_args &a, hipStream_t s)
 {
    if (a.rows <= 16) return launch_narrow<T, 1>(a, s);
-   if (a.rows <= 64) return launch_narrow<T, 4>(a, s);
    const auto tiles = [&](int64_t t) { return ((a.rows + t - 1) / t) * ((a.out_features + t - 1) / t); };
    if constexpr (sizeof(T) == 4) {
-      if (tiles(128) >= 200) launch_parts<128, 128>(a, s);
+      // 64 x 4096 x 4096: 40 us, in tiles 95 us; 512 x 8192 x 512: 74, 181 us; twice as many workgroups: 256 x 2048 x 2048 40, 50 us, but 1000 x 300 x 300 14.2, 10.8 us
+      if ((a.rows + 63) / 64 * ((a.out_features + 15) / 16) <= (a.in_features >= 1024 ? 512 : 256)) launch_narrow<T, 4>(a, s);
+      else if (tiles(128) >= 200) launch_parts<128, 128>(a, s);
       else launch_parts<64, 64>(a, s);
    } else {
-      if (std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) >= (int64_t(1) << 31) / 256) return launch_narrow<T, 4>(a, s);      // a tile's rows are not within 32-bit offsets
+      // 32 x 4096 x 4096: 13.2 us, in tiles 16.6 us; 64 rows: 20.4 us.  The other case: a tile's rows are not within 32-bit offsets
+      if (a.rows <= 32 || std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) >= (int64_t(1) << 31) / 256) return launch_narrow<T, 2>(a, s);
       const bool dma = ((uintptr_t)a.x | (uintptr_t)a.weight) % 16 == 0 && a.x_stride % 8 == 0 && a.weight_stride % 8 == 0;
       if (tiles(256) >= 200) launch_tile<T, 256, 256, 2, 4, 128, 2, 1>(a, s, dma);
       else if (tiles(128) >= 200) launch_tile<T, 128, 128, 2, 2, 128, 2, 1>(a, s, dma);
