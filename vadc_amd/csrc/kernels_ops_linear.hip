@@ -11,21 +11,27 @@ namespace ops {
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef unsigned __int128 u128;
 
-// 16 bytes of a row from value k on (from points there), zeros behind the row's n values: a piece that passes the end is the row's last 16 bytes, shifted
-// (1111 x 1000 x 1537 bfloat16 with a load per value: 17.9 us, so 11.5 us)
-template <typename T> __device__ __forceinline__ u128 load_end(const T *from, int64_t k, int64_t n)
+// N pieces of 16 bytes of rows of n values: left(i) values of piece i are in its row from from(i) on (none: that points behind the row), zeros behind.  A piece that passes the end is the
+// row's last 16 bytes, shifted; the loads stand together, before any branch (1111 x 1000 x 1537 bfloat16 with a load per value: 17.9 us, with a wait per piece 12.8 us, so 10.9 us)
+template <typename T, int N, typename From, typename Left> __device__ __forceinline__ void load_ends(int64_t n, const From &from, const Left &left, u128 (&u)[N])
 {
    constexpr int PER = 16 / (int)sizeof(T), BITS = 8 * (int)sizeof(T);
    typedef std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t> bits;
-   u128 u = 0;
    if (n >= PER) {
-      const int over = (int)min(max(k - (n - PER), (int64_t)0), (int64_t)PER);
-      __builtin_memcpy(&u, from - max(k - (n - PER), (int64_t)0), 16);
-      u = over == PER ? (u128)0 : u >> (over * BITS);
+#pragma unroll
+      for (int i = 0; i < N; ++i) __builtin_memcpy(&u[i], from(i) - max(PER - left(i), 0), 16);
+      if (n % PER)                                                    // pieces of other rows are whole or empty
+#pragma unroll
+         for (int i = 0; i < N; ++i) u[i] >>= min(max(PER - left(i), 0), PER - 1) * BITS;
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i] = left(i) <= 0 ? (u128)0 : u[i];
    } else
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+         u[i] = 0;
 #pragma unroll 1
-      for (int i = (int)min(n - k, (int64_t)PER) - 1; i >= 0; --i) u = u << BITS | __builtin_bit_cast(bits, from[i]);
-   return u;
+         for (int e = min(left(i), PER) - 1; e >= 0; --e) u[i] = u[i] << BITS | __builtin_bit_cast(bits, from(i)[e]);
+      }
 }
 
 // 16 values in one run.  ODD: two-byte values may begin within a dword, where a wide load takes about four times as long: whole dwords are loaded and shifted; the last dword is the one
@@ -165,7 +171,7 @@ __device__ __forceinline__ const void *uniform(const void *p)
 {
    const uint64_t v = (uint64_t)(uintptr_t)p;
    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-   return (const void *)(uintptr_t)((uint64_t)hi << 32 | lo);
+   return (const void *)(const __attribute__((address_space(1))) char *)(uintptr_t)((uint64_t)hi << 32 | lo);      // global: a generic pointer's loads would count with those of LDS
 }
 template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 
@@ -220,11 +226,10 @@ __global__ __launch_bounds__(64 * WR * WC * KG, (512 + 64 * WR * WC * KG - 1) / 
    };
    const auto fetch_part = [&](auto &h) {                             // the part of a tile at the end, zeros behind the last k
       const char *fromx = (const char *)uniform(srcx + full * KT), *fromw = (const char *)uniform(srcw + full * KT);
-#pragma unroll
-      for (int p = 0; p < PIECES; ++p) {
-         const u128 u = load_end((const T *)((p < XP ? fromx : fromw) + offset[p]), full * KT + piece_of(p) * PER, a.in_features);
-         __builtin_memcpy(&h[p], &u, 16);
-      }
+      const int rest = (int)(a.in_features - full * KT);
+      u128 u[PIECES];
+      load_ends<T, PIECES>(a.in_features, [&](int p) { return (const T *)((p < XP ? fromx : fromw) + offset[p]); }, [&](int p) { return rest - piece_of(p) * PER; }, u);
+      __builtin_memcpy(&h, &u, sizeof(u));
    };
    const auto place = [&](int stage, const auto &h) {
 #pragma unroll
@@ -442,43 +447,47 @@ __global__ __launch_bounds__(256, 2) void k_linear_parts(const vadc_amd_linear_a
 }
 
 // ---- few rows: the weight goes once through registers, nothing is shared -------------------------------------------------------------------------------
-// A workgroup does 16 features of up to 16 TM rows; its eight waves take every eighth 64 k's and add up in LDS in a fixed order.  A lane reads 32 (float32: 64) consecutive bytes of its
+// A workgroup does 16 TN features of up to 16 TM rows; its eight waves take every eighth 64 k's and add up in LDS in a fixed order.  A lane reads 32 (float32: 64) consecutive bytes of its
 // row, so that the four lanes of a row read a run: the k's of an operand fragment may come in any order that both operands share.
-template <typename T, int TM, bool ODD>
+template <typename T, int TN, int TM, bool ODD>
 __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_args a)
 {
    constexpr int WAVES = 8;
-   __shared__ __attribute__((aligned(16))) f4 part[WAVES][TM][64];
+   __shared__ __attribute__((aligned(16))) f4 part[WAVES][TN * TM][64];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, l4 = lane >> 4;
-   const int64_t tiles_n = (a.out_features + 15) / 16, row0 = blockIdx.x / tiles_n * (16 * TM), col0 = blockIdx.x % tiles_n * 16;
-   const T *pw = (const T *)a.weight + min(col0 + l15, a.out_features - 1) * a.weight_stride, *px[TM];
+   const int64_t tiles_n = (a.out_features + 16 * TN - 1) / (16 * TN), row0 = blockIdx.x / tiles_n * (16 * TM), col0 = blockIdx.x % tiles_n * (16 * TN);
+   const T *pw[TN], *px[TM];
+#pragma unroll
+   for (int i = 0; i < TN; ++i) pw[i] = (const T *)a.weight + min(col0 + 16 * i + l15, a.out_features - 1) * a.weight_stride;
 #pragma unroll
    for (int j = 0; j < TM; ++j) px[j] = (const T *)a.x + min(row0 + 16 * j + l15, a.rows - 1) * a.x_stride;
-   f4 acc[TM];
+   f4 acc[TN * TM];
 #pragma unroll
-   for (int j = 0; j < TM; ++j) acc[j] = (f4)(0.0f);
-   struct Held { T w[16], x[TM][16]; };
+   for (int j = 0; j < TN * TM; ++j) acc[j] = (f4)(0.0f);
+   struct Held { T w[TN][16], x[TM][16]; };
    const auto products = [&](const Held &h) {
 #pragma unroll
-      for (int j = 0; j < TM; ++j) {
+      for (int t = 0; t < TN * TM; ++t) {
+         const int i = t / TM, j = t % TM;
          if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int s = 0; s < 16; ++s) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(h.w[s], h.x[j][s], acc[j], 0, 0, 0);
+            for (int s = 0; s < 16; ++s) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(h.w[i][s], h.x[j][s], acc[t], 0, 0, 0);
          } else {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
                p8 fa, fb;
-               __builtin_memcpy(&fa, &h.w[8 * s], sizeof(fa));
+               __builtin_memcpy(&fa, &h.w[i][8 * s], sizeof(fa));
                __builtin_memcpy(&fb, &h.x[j][8 * s], sizeof(fb));
-               if constexpr (__is_same(T, __bf16)) acc[j] = mfma16(fa, fb, acc[j]);
-               else acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, fa), __builtin_bit_cast(h8, fb), acc[j], 0, 0, 0);
+               if constexpr (__is_same(T, __bf16)) acc[t] = mfma16(fa, fb, acc[t]);
+               else acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, fa), __builtin_bit_cast(h8, fb), acc[t], 0, 0, 0);
             }
          }
       }
    };
    // Whole pieces of 64 k's in a loop of their own; at most one wave has the part at the end
    const auto load = [&](int64_t k, Held &h) {
-      load16<T, ODD>(pw + k + 16 * l4, h.w);
+#pragma unroll
+      for (int i = 0; i < TN; ++i) load16<T, ODD>(pw[i] + k + 16 * l4, h.w[i]);
 #pragma unroll
       for (int j = 0; j < TM; ++j) load16<T, ODD>(px[j] + k + 16 * l4, h.x[j]);
    };
@@ -502,27 +511,22 @@ __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_arg
          products(even);
       }
    if (k < a.in_features) {
+      const int left = (int)(a.in_features - k) - 16 * l4;
       k += 16 * l4;
-#pragma unroll
-      for (int i = 0; i < 16; i += 16 / (int)sizeof(T)) {
-         const u128 u = load_end(pw + k + i, k + i, a.in_features);
-         __builtin_memcpy(&even.w[i], &u, 16);
-#pragma unroll
-         for (int j = 0; j < TM; ++j) {
-            const u128 v = load_end(px[j] + k + i, k + i, a.in_features);
-            __builtin_memcpy(&even.x[j][i], &v, 16);
-         }
-      }
+      constexpr int PER = 16 / (int)sizeof(T), PP = 16 / PER;
+      u128 u[(TN + TM) * PP];
+      load_ends<T, (TN + TM) * PP>(a.in_features, [&](int i) { return (i < TN * PP ? pw[i / PP] : px[(i - TN * PP) / PP]) + k + i % PP * PER; }, [&](int i) { return left - i % PP * PER; }, u);
+      __builtin_memcpy(&even, &u, sizeof(u));
       products(even);
    }
 #pragma unroll
-   for (int j = 0; j < TM; ++j) part[wave][j][lane] = acc[j];
+   for (int t = 0; t < TN * TM; ++t) part[wave][t][lane] = acc[t];
    __syncthreads();
-   for (int j = wave; j < TM; j += WAVES) {
-      f4 sum = part[0][j][lane];
+   for (int t = wave; t < TN * TM; t += WAVES) {
+      f4 sum = part[0][t][lane];
 #pragma unroll
-      for (int w = 1; w < WAVES; ++w) sum += part[w][j][lane];
-      const int64_t row = row0 + 16 * j + l15, col = col0 + 4 * l4;
+      for (int w = 1; w < WAVES; ++w) sum += part[w][t][lane];
+      const int64_t row = row0 + 16 * (t % TM) + l15, col = col0 + 16 * (t / TM) + 4 * l4;
       float y[4] = {sum[0], sum[1], sum[2], sum[3]}, bias[4];
       load_bias<T, 4>(a, col, bias);
       const int left = (int)min((int64_t)4, a.out_features - col);
@@ -539,15 +543,15 @@ template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES, int KG
    if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, STAGES, KG, true>), grid, dim3(threads), 0, s, a);
    else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, 2, KG, false>), grid, dim3(threads), 0, s, a);
 }
-template <typename T, int TM> static void launch_narrow(const vadc_amd_linear_args &a, hipStream_t s)
+template <typename T, int TN, int TM> static void launch_narrow(const vadc_amd_linear_args &a, hipStream_t s)
 {
-   const dim3 grid((unsigned)(((a.rows + 16 * TM - 1) / (16 * TM)) * ((a.out_features + 15) / 16)));
+   const dim3 grid((unsigned)(((a.rows + 16 * TM - 1) / (16 * TM)) * ((a.out_features + 16 * TN - 1) / (16 * TN))));
    if constexpr (sizeof(T) == 2)
       if (((uintptr_t)a.x | (uintptr_t)a.weight) % 4 || a.x_stride % 2 || a.weight_stride % 2) {
-         hipLaunchKernelGGL((k_linear_narrow<T, TM, true>), grid, dim3(512), 0, s, a);
+         hipLaunchKernelGGL((k_linear_narrow<T, TN, TM, true>), grid, dim3(512), 0, s, a);
          return;
       }
-   hipLaunchKernelGGL((k_linear_narrow<T, TM, false>), grid, dim3(512), 0, s, a);
+   hipLaunchKernelGGL((k_linear_narrow<T, TN, TM, false>), grid, dim3(512), 0, s, a);
 }
 template <int BM, int BN> static void launch_parts(const vadc_amd_linear_args &a, hipStream_t s)
 {
@@ -556,16 +560,19 @@ template <int BM, int BN> static void launch_parts(const vadc_amd_linear_args &a
 }
 template <typename T> static void launch(const vadc_amd_linear_args &a, hipStream_t s)
 {
-   if (a.rows <= 16) return launch_narrow<T, 1>(a, s);
+   if (a.rows <= 16) return launch_narrow<T, 1, 1>(a, s);
    const auto tiles = [&](int64_t t) { return ((a.rows + t - 1) / t) * ((a.out_features + t - 1) / t); };
    if constexpr (sizeof(T) == 4) {
-      // 64 x 4096 x 4096: 40 us, in tiles 95 us; 512 x 8192 x 512: 74, 181 us; twice as many workgroups: 256 x 2048 x 2048 40, 50 us, but 1000 x 300 x 300 14.2, 10.8 us
-      if ((a.rows + 63) / 64 * ((a.out_features + 15) / 16) <= (a.in_features >= 1024 ? 512 : 256)) launch_narrow<T, 4>(a, s);
+      const int64_t blocks = (a.rows + 63) / 64 * ((a.out_features + 15) / 16);
+      // 64 x 4096 x 4096: 39 us, in tiles 95 us; 2048 x 512 x 128: 9.7, 14.3 us.  Twice as many: 256 x 2048 x 2048 34, 50 us; but rows that two workgroups read far apart: 8192 x 512 x 64
+      // 20.6, 15.4 us
+      if (blocks <= 256) launch_narrow<T, 1, 4>(a, s);
+      else if (blocks <= 512 && a.rows <= 2048) launch_narrow<T, 2, 4>(a, s);
       else if (tiles(128) >= 200) launch_parts<128, 128>(a, s);
       else launch_parts<64, 64>(a, s);
    } else {
       // 32 x 4096 x 4096: 13.2 us, in tiles 16.6 us; 64 rows: 20.4 us.  The other case: a tile's rows are not within 32-bit offsets
-      if (a.rows <= 32 || std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) >= (int64_t(1) << 31) / 256) return launch_narrow<T, 2>(a, s);
+      if (a.rows <= 32 || std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) >= (int64_t(1) << 31) / 256) return launch_narrow<T, 1, 2>(a, s);
       const bool dma = ((uintptr_t)a.x | (uintptr_t)a.weight) % 16 == 0 && a.x_stride % 8 == 0 && a.weight_stride % 8 == 0;
       if (tiles(256) >= 200) launch_tile<T, 256, 256, 2, 4, 128, 2, 1>(a, s, dma);
       else if (tiles(128) >= 200) launch_tile<T, 128, 128, 2, 2, 128, 2, 1>(a, s, dma);
