@@ -645,3 +645,28 @@ def test_broadcast_inputs(ops):
     within(ops.group_norm(z, 4), want[:, 0], norm_tol(want, spread, torch.float32, 24)[:, 0])
     q, k, v, g, beta, state = delta_inputs(3, 2, 70, 2, 4, 32, 32, torch.bfloat16, True)
     check_delta(ops, q[:, :, :1].expand(2, 70, 2, 32), k[:1].expand(2, 70, 2, 32), v[:, :, :1].expand(2, 70, 4, 32), g, beta, state, True)
+
+
+# ------------------------------------------------------------------------------------------- what the interface promises
+
+@pytest.mark.parametrize("dtype", ("f16", "bf16"))
+@pytest.mark.parametrize("normalize", (True, False))
+@pytest.mark.parametrize("b, t, hk, h, dk, dv", DELTA_SIZES + [(2, 1000, 1, 2, 128, 64)])
+def test_gated_delta_rounds_an_output_once(ops, b, t, hk, h, dk, dv, normalize, dtype):
+    """sums and states are float32 whatever the type: the 16-bit call's outputs are the float32 call's on the same values, rounded once, and its states the same bits"""
+    q, k, v, g, beta, state = delta_inputs(t + dv, b, t, hk, h, dk, dv, TYPES[dtype], normalize)
+    mine, wide = state.clone(), state.clone()
+    got = ops.gated_delta(q, k, v, g, beta, mine, normalize=normalize)
+    want = ops.gated_delta(q.float(), k.float(), v.float(), g, beta, wide, normalize=normalize)
+    assert torch.equal(got, want.to(got.dtype)) and torch.equal(mine, wide)
+
+
+@pytest.mark.parametrize("normalize", (True, False))
+@pytest.mark.parametrize("b, t, hk, h, dk, dv", DELTA_SIZES + [(2, 1000, 1, 2, 128, 64)])
+def test_gated_delta_float32_outputs_are_as_good_as_the_state(ops, b, t, hk, h, dk, dv, normalize):
+    """an output is a sum over the state's rows through q: it has the state's relative error (3e-6 of the norm, as check_delta's) and that of its own dk + 64 terms, rounded
+    independently: sqrt(dk + 64) half steps, 18 u = 1.1e-6 at most"""
+    q, k, v, g, beta, state = delta_inputs(t + dk + 1, b, t, hk, h, dk, dv, torch.float32, normalize)
+    want, _, _ = delta64(q, k, v, g, beta, state, 0.5, normalize, None)
+    got = ops.gated_delta(q, k, v, g, beta, state, scale=0.5, normalize=normalize)
+    assert (got.double() - want).norm() <= 4.1e-6 * want.norm()

@@ -122,14 +122,14 @@ template <typename T, int VEC, int ROWS> static void launch_step(const vadc_amd_
 // enters (k rows, gates in k_delta_blocks; beta v - c1 x in k_delta_scan, which every non-finite operand reaches in its own step) and the column is NaN from that step on.
 constexpr int kBlock = 64;
 constexpr int kTiles = 6;                                            // 16 x 32 tiles of a lower triangle: rows 0, 16 need columns 0 .. 31 only
-// Parts of P, u and S in the products that make an output: what leaves in 16 bits (half a step: 2^-9, fp16 2^-12) is made from two, which leave 2^-17 of a product out; the state is not.
-template <typename T> constexpr int kOutParts = sizeof(T) == 2 ? 2 : 3;
-template <typename T> struct __align__(16) BlockData {
-   p8 t[kTiles][3][64], p[kTiles][kOutParts<T>][64];                 // operand order, in parts: lane (l4, l15) has row l15, columns 4 l4 .. and 16 + 4 l4 .. of the tile
+// Three parts of P, u and S also where the outputs leave in 16 bits: they are float32 sums rounded once, whatever the type.  (With two, 2^-17 of a product was left out and ten times as many
+// bfloat16 outputs were rounded to the other neighbour, 0.28 % against 0.03 %, for 4 % of the time.)
+struct __align__(16) BlockData {
+   p8 t[kTiles][3][64], p[kTiles][3][64];                            // operand order, in parts: lane (l4, l15) has row l15, columns 4 l4 .. and 16 + 4 l4 .. of the tile
    float c1[kBlock], beta[kBlock], c2[kBlock], c3[kBlock];           // beta a rk, beta, a rq, e^(G_63 - G) rk
    float end[32];                                                    // a_63, four times; the rest keeps the next block on a line of its own
 };
-static_assert(sizeof(BlockData<float>) % 128 == 0 && sizeof(BlockData<__bf16>) % 128 == 0, "a block's tiles start on a cache line");
+static_assert(sizeof(BlockData) % 128 == 0, "a block's tiles start on a cache line");
 __device__ __forceinline__ int tile_of(int mt, int ks) { return mt < 2 ? mt : 2 * mt - 2 + ks; }
 // LDS rows of KD bfloat16 in 16-byte pieces, the piece index mixed with the row: 16 rows' pieces of one column (an operand) and two neighbouring pieces of 4 rows and of the 4 rows
 // eight further (a transposing read) lie in different places of the 256 bytes of banks
@@ -237,16 +237,16 @@ template <int KD> __device__ __forceinline__ p8 load_transposed(const __bf16 *ro
 }
 
 // the tiles of rows 16 mt .. from the sixteen-column pieces a lane holds of its row
-template <int N> __device__ __forceinline__ void store_rows(p8 (&to)[kTiles][N][64], const f4 (&x)[4], int mt, int lane)
+__device__ __forceinline__ void store_rows(p8 (&to)[kTiles][3][64], const f4 (&x)[4], int mt, int lane)
 {
 #pragma unroll
    for (int s = 0; s < 2; ++s)
       if (s == 0 || mt >= 2) {
-         p4 lo[N], hi[N];
+         p4 lo[3], hi[3];
          split4(x[2 * s], lo);
          split4(x[2 * s + 1], hi);
 #pragma unroll
-         for (int n = 0; n < N; ++n) to[tile_of(mt, s)][n][lane] = join(lo[n], hi[n]);
+         for (int n = 0; n < 3; ++n) to[tile_of(mt, s)][n][lane] = join(lo[n], hi[n]);
       }
 }
 
@@ -271,7 +271,7 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
    const bool partial = live < kBlock || kd < KD;
    const int64_t kh = head / (a.heads / a.key_heads);
    const T *q = (const T *)a.q + stream * a.q_stride[0] + t0 * a.q_stride[1] + kh * a.q_stride[2], *k = (const T *)a.k + stream * a.k_stride[0] + t0 * a.k_stride[1] + kh * a.k_stride[2];
-   BlockData<T> &out = ((BlockData<T> *)a.workspace)[blockIdx.x];
+   BlockData &out = ((BlockData *)a.workspace)[blockIdx.x];
    const int mine = 16 * wave + l15;                                 // the row of the block that this lane holds of the wave's sixteen
    Raw8<T> xk[KS], xq[KS];
    {  // rows of q in operand order; k into LDS in its parts, four threads a row
@@ -424,8 +424,8 @@ __global__ __launch_bounds__(256) void k_delta_blocks(const vadc_amd_gated_delta
 template <typename T, int KD, int COLS>
 __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_delta_args a, const Segment seg)
 {
-   constexpr int NT = Parts<T>::n, NO = kOutParts<T>, KS = KD / 32, ST = KD / 64, WAVES = COLS / 4;
-   __shared__ __attribute__((aligned(16))) __bf16 sk[NT][kBlock * KD], sq[NT][kBlock * KD], ss[3][COLS * KD], sr[3][COLS * kBlock], su[NO][COLS * kBlock], sw[3][COLS * kBlock];
+   constexpr int NT = Parts<T>::n, KS = KD / 32, ST = KD / 64, WAVES = COLS / 4;
+   __shared__ __attribute__((aligned(16))) __bf16 sk[NT][kBlock * KD], sq[NT][kBlock * KD], ss[3][COLS * KD], sr[3][COLS * kBlock], su[3][COLS * kBlock], sw[3][COLS * kBlock];
    __shared__ int spoison[COLS];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, l4 = lane >> 4, mt = wave & 3, nt = wave >> 2;
    // the workgroups of one state, which read the same k, q, T and P, lie eight apart: on one XCD, behind one L2
@@ -441,7 +441,7 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
    const T *q = (const T *)a.q + stream * a.q_stride[0] + seg.from * a.q_stride[1] + kh * a.q_stride[2], *k = (const T *)a.k + stream * a.k_stride[0] + seg.from * a.k_stride[1] + kh * a.k_stride[2];
    const T *v = (const T *)a.v + stream * a.v_stride[0] + seg.from * a.v_stride[1] + head * a.v_stride[2] + tile * COLS;
    T *o = (T *)a.out + stream * a.out_stride[0] + seg.from * a.out_stride[1] + head * a.out_stride[2] + tile * COLS;
-   const BlockData<T> *data = (const BlockData<T> *)a.workspace + (stream * a.heads + head) * seg.blocks;
+   const BlockData *data = (const BlockData *)a.workspace + (stream * a.heads + head) * seg.blocks;
    float *state = a.state + stream * a.state_stride + head * a.key_dim * a.value_dim + column;
    f4 S[ST];
 #pragma unroll
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
    const auto rows4 = [&](const float *f) { return *reinterpret_cast<const f4 *>(f + 16 * mt + 4 * l4); };
    const auto tiles2 = [&](const auto &from, auto &to) {
 #pragma unroll
-      for (int n = 0; n < (int)(sizeof(to[0]) / sizeof(p8)); ++n) {
+      for (int n = 0; n < 3; ++n) {
          to[0][n] = from[tile_of(mt, 0)][n][lane];
          to[1][n] = from[tile_of(mt, mt >= 2)][n][lane];             // rows 0 .. 31 have one tile
       }
@@ -495,7 +495,7 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
       const p4 lo = *reinterpret_cast<const p4 *>(from + place<kBlock>(col, 4 * s + (l4 >> 1)) + 4 * (l4 & 1)), hi = *reinterpret_cast<const p4 *>(from + place<kBlock>(col, 4 * s + 2 + (l4 >> 1)) + 4 * (l4 & 1));
       return join(lo, hi);
    };
-   p8 ft[2][3], fp[2][NO];
+   p8 ft[2][3], fp[2][3];
    // the first block's, in the order in which the loop fetches the next one's: the compiler's counts of what is still under way hold for both then
    const auto in_order = [] { asm volatile("" ::: "memory"); };
    f4 c1 = rows4(data->c1), beta = rows4(data->beta);
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
    tiles2(data->p, fp);
    in_order();
    for (int b = 0; b < blocks; ++b) {
-      const BlockData<T> &next = data[min(b + 1, blocks - 1)];
+      const BlockData &next = data[min(b + 1, blocks - 1)];
       const int live = (int)min((int64_t)kBlock, steps - (int64_t)b * kBlock);
       const bool partial = live < kBlock || kd < KD;
 #pragma unroll
@@ -545,10 +545,7 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
             fk[n] = *reinterpret_cast<const p8 *>(&sk[n][place<KD>(16 * mt + l15, 4 * s + l4)]);
             fq[n] = *reinterpret_cast<const p8 *>(&sq[n][place<KD>(16 * mt + l15, 4 * s + l4)]);
          }
-         p8 fo[NO];
-#pragma unroll
-         for (int n = 0; n < NO; ++n) fo[n] = fs[n];
-         mfma_parts2(fk, fs, x, fq, fo, y);
+         mfma_parts2(fk, fs, x, fq, fs, y);
       }
       f4 r = values4<T>(xv);
       if (live < kBlock || width < COLS) r = trim4(r, vrow < live ? vback : 4);
@@ -590,9 +587,9 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
          for (int i = 0; i < ST; ++i)
 #pragma unroll
             for (int n = 0; n < NT; ++n) kt[s][i][n] = load_transposed<KD>(sk[n], 32 * s + 8 * l4, 64 * i + 16 * mt, l15);
-      split4(u, p);                                                  // (its first NO parts)
+      split4(u, p);
 #pragma unroll
-      for (int n = 0; n < NO; ++n) *reinterpret_cast<p4 *>(&su[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
+      for (int n = 0; n < 3; ++n) *reinterpret_cast<p4 *>(&su[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
       split4(c3 * u, p);
 #pragma unroll
       for (int n = 0; n < 3; ++n) *reinterpret_cast<p4 *>(&sw[n][place<kBlock>(col, 2 * mt + (l4 >> 1)) + 4 * (l4 & 1)]) = p[n];
@@ -615,17 +612,17 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
          }
       }
       {
-         p8 f[2][NO];
+         p8 f[2][3];
 #pragma unroll
          for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int n = 0; n < NO; ++n) f[s][n] = rows8(su[n], s);
+            for (int n = 0; n < 3; ++n) f[s][n] = rows8(su[n], s);
          y *= c2;
          if (mt >= 2) {
             f4 y2 = {0, 0, 0, 0};
             mfma_parts2(fp[0], f[0], y, fp[1], f[1], y2);
             y += y2;
-         } else y = mfma_parts<NO, NO>(fp[0], f[0], y);
+         } else y = mfma_parts<3, 3>(fp[0], f[0], y);
       }
       c2 = rows4(next.c2);
       tiles2(next.p, fp);
@@ -664,7 +661,7 @@ static bool in_blocks(const vadc_amd_gated_delta_args &a)
 // float32: 89 us a call against 100 with 32) --; with longer keys, where staging k and q again for every 16 columns costs more than that gains, 32 (2 x 8192 steps, 32 heads of 128 x 128,
 // bfloat16: 507 us against 543 with 16)
 template <int KD> constexpr int scan_columns() { return KD == 64 ? 16 : 32; }
-// The workspace holds 4096 blocks of 37 or 31 KB, which stay in the last-level cache between the two launches; longer calls go out in segments of steps (2 x 8192 steps, 32 heads: 507 us so,
+// The workspace holds 4096 blocks of 37 KB, which stay in the last-level cache between the two launches; longer calls go out in segments of steps (2 x 8192 steps, 32 heads: 507 us so,
 // 523 with 2048, 502 with 8192)
 static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
 {
@@ -693,7 +690,7 @@ template <typename T> static void launch(const vadc_amd_gated_delta_args &a, con
 
 int64_t gated_delta_workspace(const vadc_amd_gated_delta_args &a)
 {
-   return in_blocks(a) ? a.streams * a.heads * segment_blocks(a) * (int64_t)(a.dtype == VADC_AMD_F32 ? sizeof(BlockData<float>) : sizeof(BlockData<__bf16>)) : 0;
+   return in_blocks(a) ? a.streams * a.heads * segment_blocks(a) * (int64_t)sizeof(BlockData) : 0;
 }
 
 void launch_gated_delta(const vadc_amd_gated_delta_args &a, const vadc_amd_gated_delta_args &first, hipStream_t s)
