@@ -670,3 +670,19 @@ def test_gated_delta_float32_outputs_are_as_good_as_the_state(ops, b, t, hk, h, 
     want, _, _ = delta64(q, k, v, g, beta, state, 0.5, normalize, None)
     got = ops.gated_delta(q, k, v, g, beta, state, scale=0.5, normalize=normalize)
     assert (got.double() - want).norm() <= 4.1e-6 * want.norm()
+
+
+@pytest.mark.parametrize("act", ("sigmoid", "silu"))
+def test_float32_sigmoid_far_from_zero(ops, act):
+    """the activation's own error in float32 steps, where 1 + e^-y is all exponential: an exponential and a reciprocal of 1 step each, 1 + e and y sigmoid rounded (half a step each), and what is
+    left of e^-y's own corrections, 1 step -- 4 steps of 2 u relative; beyond its range it ends at 0 and 1"""
+    one = torch.ones(1, 1, device="cuda")
+    y = torch.linspace(-79, 79, 160001, device="cuda")
+    for rows, part in ((1, slice(None)), (300, slice(0, 9000)), (300, slice(75000, 84000))):
+        got, want = ops.linear(one.expand(rows, 1), y[part, None], activation=act)[rows // 2], act64(y[part].double(), act)
+        assert ((got.double() - want).abs() <= 4 * 2 * U * want.abs()).all()
+    y = torch.tensor([-math.inf, -3e38, -1000.0, -200.0, 200.0, 3e38, math.inf, math.nan], device="cuda")
+    got = ops.linear(one, y[:, None], activation="sigmoid")[0]
+    assert torch.equal(got[:7], torch.tensor([0.0, 0.0, 0.0, 0.0, 1.0, 1.0, 1.0], device="cuda")) and torch.isnan(got[7])
+    got = ops.linear(one, y[1:7, None], activation="silu")[0]
+    assert torch.equal(got, torch.tensor([0.0, 0.0, 0.0, 200.0, 3e38, math.inf], device="cuda"))

@@ -82,7 +82,7 @@ __device__ __forceinline__ void finish(const vadc_amd_linear_args &a, const T *r
 #pragma unroll
          for (int i = 0; i < N; ++i) y[i] += r[i];
    }
-   activate_all<N>(y, a.activation);
+   activate_all<T, N>(y, a.activation);
    if (a.residual && !a.residual_first)
 #pragma unroll
       for (int i = 0; i < N; ++i) y[i] += r[i];

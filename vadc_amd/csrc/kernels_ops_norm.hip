@@ -43,10 +43,10 @@ __device__ __forceinline__ void apply(const vadc_amd_group_norm_args &a, const f
 #pragma unroll
    for (int i = 0; i < VEC; ++i) y[i] = fmaf((x[i] - mean) * rstd, w[i], b[i]);
    if (a.gate) {
-      activate_all<VEC>(g, a.activation);
+      activate_all<T, VEC>(g, a.activation);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) y[i] *= g[i];
-   } else activate_all<VEC>(y, a.activation);
+   } else activate_all<T, VEC>(y, a.activation);
    if (a.sequences * a.positions * a.channels * (int64_t)sizeof(T) >= kStreamBytes) stream_f32<T, VEC>(out, y);
    else store_f32<T, VEC>(out, y);
 }
