@@ -686,3 +686,20 @@ def test_float32_sigmoid_far_from_zero(ops, act):
     assert torch.equal(got[:7], torch.tensor([0.0, 0.0, 0.0, 0.0, 1.0, 1.0, 1.0], device="cuda")) and torch.isnan(got[7])
     got = ops.linear(one, y[1:7, None], activation="silu")[0]
     assert torch.equal(got, torch.tensor([0.0, 0.0, 0.0, 200.0, 3e38, math.inf], device="cuda"))
+
+
+def test_outputs_in_the_rows_of_an_operand(ops):
+    """x and out, x and gate, v and out side by side in the same wide rows"""
+    rnd = gen(12)
+    rows = rnd(70, 32 + 48)
+    x, out, w = rows[:, :32], rows[:, 32:], rnd(48, 32)
+    want = ops.linear(x.clone(), w)
+    assert torch.equal(ops.linear(x, w, out=out), want) and torch.equal(rows[:, 32:], want)
+    rows = rnd(3, 40, 3, 24)
+    want = ops.group_norm(rows[:, :, 0].clone(), 4, gate=rows[:, :, 1].clone())
+    assert torch.equal(ops.group_norm(rows[:, :, 0], 4, gate=rows[:, :, 1], out=rows[:, :, 2]), want)
+    q, k, v, g, beta, state = delta_inputs(6, 2, 70, 1, 2, 16, 24, torch.float32, True)
+    rows = torch.cat([v, v], 3)
+    mine = state.clone()
+    want = ops.gated_delta(q, k, v, g, beta, state, normalize=True)
+    assert torch.equal(ops.gated_delta(q, k, rows[..., :24], g, beta, mine, normalize=True, out=rows[..., 24:]), want) and torch.equal(mine, state)

@@ -197,3 +197,44 @@ def test_rows_at_one_distance():
             continue
         with pytest.raises(ValueError, match="rows"):
             rows(bad)
+
+
+def test_tensors_share_a_byte_or_not():
+    """the overlap of two strided tensors, against the sets of their bytes"""
+    import random
+
+    rng, pool = random.Random(5), torch.zeros(4000)
+    exact = found = 0
+    for _ in range(3000):
+        def view():
+            dims = rng.randint(1, 3)
+            shape = [rng.choice((1, 2, 3, 5)) for _ in range(dims)]
+            stride = [rng.choice((0, 1, 2, 3, 4, 6, 8, 20, 24, 40, 120)) for _ in range(dims)]
+            return (pool if rng.random() < 0.7 else pool.view(torch.int16)).as_strided(shape, stride, rng.randint(0, 60))
+
+        def held(a):
+            at = {(a.data_ptr() - pool.data_ptr())}
+            for n, s in zip(a.shape, a.stride()):
+                at = {x + i * s * a.element_size() for x in at for i in range(n)}
+            return {x + i for x in at for i in range(a.element_size())}
+
+        x, y = view(), view()
+        want, got = bool(held(x) & held(y)), ops._shares(x, y)
+        assert got or not want                       # an overlap is never missed
+        exact += got == want
+        found += want
+    assert exact > 2950 and 500 < found < 2500, (exact, found)
+
+
+def test_parts_of_rows_are_apart():
+    """an output may lie in the same wide rows as an operand"""
+    wide, blocks = t(4, 8), t(2, 5, 4, 6)
+    for base, x, y in ((wide, wide[:, :3], wide[:, 3:]), (blocks, blocks[:, :, 1], blocks[:, :, 2:4])):
+        assert not ops._shares(x, y) and not ops._shares(y, x)
+
+        def spans(*ts):
+            return tuple(ops._span(ops._Layout(*ops._layout(a))) for a in ts)
+
+        ops._apart("linear", spans(x, y), y, (("x", x),))
+        with pytest.raises(ValueError, match="overlaps x"):
+            ops._apart("linear", spans(base, y), y, (("x", base),))

@@ -152,14 +152,48 @@ def _span(v: Optional[_Layout]) -> int:
     return (sum((n - 1) * s for n, s in zip(v.shape, v.stride)) + 1) * v.dtype.itemsize
 
 
+def _pieces(shape: tuple, stride: tuple, size: int):
+    """the bytes of a tensor: runs of equal length, and the (distance, count) of their repetitions, the furthest apart first"""
+    run, repeats = size, []
+    for distance, n in sorted((s * size, n) for s, n in zip(stride, shape) if n > 1 and s):
+        if not repeats and distance <= run:
+            run += distance * (n - 1)
+        else:
+            repeats.append((distance, n))
+    return run, repeats[::-1]
+
+
+_FEW = 8                     # repetitions looked at one by one
+
+
+def _meet(by: int, run_a: int, a: list, run_b: int, b: list) -> bool:
+    """whether two tensors' _pieces share a byte, the second's first one `by` behind the first's.  Repetitions at one distance are taken together; where too many would have to be looked
+    at one by one, the answer is yes."""
+    reach_a, reach_b = (run + sum(s * (n - 1) for s, n in t) for run, t in ((run_a, a), (run_b, b)))
+    if by >= reach_a or by + reach_b <= 0:
+        return False
+    if not a and not b:
+        return True
+    s = max(t[0][0] for t in (a, b) if t)
+    n_a, n_b = (t[0][1] if t and t[0][0] == s else 1 for t in (a, b))
+    a, b = (t[1:] if t and t[0][0] == s else t for t in (a, b))
+    reach_a, reach_b = reach_a - s * (n_a - 1), reach_b - s * (n_b - 1)
+    near = range(max(1 - n_a, (-reach_b - by) // s + 1), min(n_b - 1, (reach_a - 1 - by) // s) + 1)      # differences between the repetitions whose spans meet
+    return len(near) > _FEW or any(_meet(by + j * s, run_a, a, run_b, b) for j in near)
+
+
+def _shares(x: Tensor, y: Tensor) -> bool:
+    return _meet(y.data_ptr() - x.data_ptr(), *_pieces(x.shape, x.stride(), x.element_size()), *_pieces(y.shape, y.stride(), y.element_size()))
+
+
 def _apart(what: str, spans: tuple, out: Tensor, ts: tuple, same: tuple = ()):
-    """out overlaps none of `ts` (named, in the order of the plan's spans); those in `same` may be out itself, entry for entry"""
+    """out overlaps none of `ts` (named, in the order of the plan's spans); those in `same` may be out itself, entry for entry.  Spans that meet are looked at closely: rows may hold both."""
     lo = out.data_ptr()
     hi = lo + spans[-1]
     for (name, t), span in zip(ts, spans):
         if t is not None:
             at = t.data_ptr()
-            if at < hi and lo < at + span and not (name in same and at == lo and t.stride() == out.stride()):
+            if at < hi and lo < at + span and not (name in same and at == lo and t.stride() == out.stride()) and _shares(out, t):
                 raise ValueError(f"{what}: out overlaps {name}")
 
 
