@@ -703,3 +703,21 @@ def test_outputs_in_the_rows_of_an_operand(ops):
     mine = state.clone()
     want = ops.gated_delta(q, k, v, g, beta, state, normalize=True)
     assert torch.equal(ops.gated_delta(q, k, rows[..., :24], g, beta, mine, normalize=True, out=rows[..., 24:]), want) and torch.equal(mine, state)
+
+
+@pytest.mark.parametrize("t", (1, 40))
+def test_gated_delta_refuses_a_state_over_its_inputs(ops, t):
+    """views of one pool: values inside the states are refused, with and without an output given; beside them they are taken"""
+    q, k, v, g, beta, state = delta_inputs(7, 2, t, 1, 2, 16, 24, torch.float32, True)
+    part = 2 * 16 * 24
+    pool = torch.zeros(2, part + t * 48, device="cuda")
+    s = pool[:, :part].view(2, 2, 16, 24)
+    s.copy_(state)
+    over = pool.as_strided((2, t, 2, 24), (part + t * 48, 48, 24, 1), part - 1)
+    for out in (None, torch.empty_like(v)):
+        with pytest.raises(ValueError, match="state overlaps v"):
+            ops.gated_delta(q, k, over, g, beta, s, out=out)
+    assert torch.equal(s, state)
+    beside = pool[:, part:].view(2, t, 2, 24)
+    beside.copy_(v)
+    assert torch.equal(ops.gated_delta(q, k, beside, g, beta, s, normalize=True), ops.gated_delta(q, k, v, g, beta, state, normalize=True)) and torch.equal(s, state)

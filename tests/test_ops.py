@@ -238,3 +238,28 @@ def test_parts_of_rows_are_apart():
         ops._apart("linear", spans(x, y), y, (("x", x),))
         with pytest.raises(ValueError, match="overlaps x"):
             ops._apart("linear", spans(base, y), y, (("x", base),))
+
+
+@pytest.mark.parametrize("name", ("q", "k", "v", "log_decay", "beta", "lengths"))
+def test_a_state_that_overlaps_an_input_is_refused(name):
+    names = ("q", "k", "v", "log_decay", "beta", "state", "lengths")
+
+    def check(a):
+        ts = [a[n] for n in names]
+        ops._state_apart(tuple(ops._span(ops._Layout(*ops._layout(x))) for x in ts), [x.data_ptr() for x in ts], *ts)
+
+    a = delta_args(b=2, h=2, dk=4, dv=5, lengths=torch.zeros(2, dtype=torch.int32))
+    check(a)
+    pool = t(2, 60)                                                  # of each stream 40 values of state, then 20 of something else
+    a["state"] = pool.as_strided((2, 2, 4, 5), (60, 20, 5, 1))
+    n = min(20, a[name][0].numel())
+
+    def placed(at):
+        x = a[name]
+        if name == "lengths":
+            return pool.view(torch.int32).as_strided((2,), (1,), at)
+        return pool.as_strided((2, 1, 1, n) if x.dim() == 4 else (2, 1, n), (60, 20, 20, 1) if x.dim() == 4 else (60, 20, 1), at)
+
+    with pytest.raises(ValueError, match=f"state overlaps {name}"):
+        check(dict(a, **{name: placed(39)}))
+    check(dict(a, **{name: placed(40)}))                             # between two streams' states

@@ -186,15 +186,16 @@ def _shares(x: Tensor, y: Tensor) -> bool:
     return _meet(y.data_ptr() - x.data_ptr(), *_pieces(x.shape, x.stride(), x.element_size()), *_pieces(y.shape, y.stride(), y.element_size()))
 
 
-def _apart(what: str, spans: tuple, out: Tensor, ts: tuple, same: tuple = ()):
-    """out overlaps none of `ts` (named, in the order of the plan's spans); those in `same` may be out itself, entry for entry.  Spans that meet are looked at closely: rows may hold both."""
+def _apart(what: str, spans: tuple, out: Tensor, ts: tuple, same: tuple = (), written: str = "out"):
+    """out (or what is `written` else) overlaps none of `ts` (named, in the order of the plan's spans; out's is last); those in `same` may be out itself, entry for entry.  Spans that meet are
+    looked at closely: rows may hold both."""
     lo = out.data_ptr()
     hi = lo + spans[-1]
     for (name, t), span in zip(ts, spans):
         if t is not None:
             at = t.data_ptr()
             if at < hi and lo < at + span and not (name in same and at == lo and t.stride() == out.stride()) and _shares(out, t):
-                raise ValueError(f"{what}: out overlaps {name}")
+                raise ValueError(f"{what}: {written} overlaps {name}")
 
 
 def _rows(what: str, name: str, v: Optional[_Layout]):
@@ -345,6 +346,14 @@ def _plan_delta(q, k, v, log_decay, beta, state, scale, normalize, lengths, out)
     return _Plan(fields, tuple(v.shape), device, tuple(map(_span, (q, k, v, log_decay, beta, state, lengths, out))), space, empty)
 
 
+def _state_apart(spans: tuple, at: list, q, k, v, log_decay, beta, state, lengths):
+    """state, which is written, overlaps no input; `at`: the tensors' addresses"""
+    lo = at[5]
+    hi = lo + spans[5]
+    if sum(p < hi and lo < p + span for p, span in zip(at, spans)) > 1:      # another one than its own
+        _apart("gated_delta", (*spans[:5], spans[6], spans[5]), state, (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("lengths", lengths)), written="state")
+
+
 def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor, state: Tensor, scale: Optional[float] = None, normalize: bool = False,
                 lengths: Optional[Tensor] = None, out: Optional[Tensor] = None) -> Tensor:
     """The gated delta rule.  Per stream and head, for each step: S = e^log_decay S; u = beta (v - S^T k); S = S + k u^T; out = scale S^T q.
@@ -362,8 +371,9 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor
     else:
         _apart("gated_delta", plan.spans, out, (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("state", state), ("lengths", lengths)))
     if not plan.empty:
+        at = [q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), 0 if lengths is None else lengths.data_ptr()]
+        _state_apart(plan.spans, at, q, k, v, log_decay, beta, state, lengths)
         space = torch.empty(plan.workspace, dtype=torch.uint8, device=v.device) if plan.workspace else None
-        _check(_lib.load().vadc_amd_gated_delta(_DELTA.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), out.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
-            0 if space is None else space.data_ptr(), plan.workspace, *plan.fields), torch._C._cuda_getCurrentRawStream(plan.device)))
+        _check(_lib.load().vadc_amd_gated_delta(_DELTA.pack(*at[:6], out.data_ptr(), at[6], 0 if space is None else space.data_ptr(), plan.workspace, *plan.fields),
+                                                torch._C._cuda_getCurrentRawStream(plan.device)))
     return out
