@@ -721,3 +721,26 @@ def test_gated_delta_refuses_a_state_over_its_inputs(ops, t):
     beside = pool[:, part:].view(2, t, 2, 24)
     beside.copy_(v)
     assert torch.equal(ops.gated_delta(q, k, beside, g, beta, s, normalize=True), ops.gated_delta(q, k, v, g, beta, state, normalize=True)) and torch.equal(s, state)
+
+
+@pytest.mark.parametrize("t", (1, 40))
+def test_writes_in_place_are_seen_by_autograd(ops, t):
+    """a graph that saved a tensor which a call then writes raises in its backward, as with torch's own in-place operations, also through a view; a tensor of torch's inference mode is taken"""
+    rnd = gen(13)
+    q, k, v, g, beta, state = delta_inputs(8, 2, t, 1, 2, 16, 24, torch.float32, True)
+    x, w, z = rnd(30, 16), rnd(24, 16), rnd(30, 24)
+    for written, call in ((state, lambda: ops.gated_delta(q, k, v, g, beta, state)), (state, lambda: ops.gated_delta(q, k, v, g, beta, state[:])),
+                          (v, lambda: ops.gated_delta(q, k, v.clone(), g, beta, state, out=v)), (z, lambda: ops.linear(x, w, residual=z, out=z)), (z, lambda: ops.group_norm(z, 4, out=z)),
+                          (z, lambda: ops.linear(x[:10], w, out=z[:10]))):
+        weight = torch.ones_like(written, requires_grad=True)
+        loss = (written * weight).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    before = (q._version, x._version, w._version)
+    ops.linear(x, w)
+    ops.gated_delta(q, k, v, g, beta, state)
+    assert (q._version, x._version, w._version) == before
+    with torch.inference_mode():
+        s = state.clone()
+        assert torch.equal(ops.gated_delta(q, k, v, g, beta, s), ops.gated_delta(q, k, v, g, beta, state))

@@ -6,7 +6,8 @@
 
 Tensors are torch tensors on one gfx950 device, of one type (float32, float16 or bfloat16); the work is enqueued on torch's current stream of that device and may be captured into a
 graph.  Sums, statistics and states are float32, an output is rounded once.  Strided tensors are taken as they are, as long as the innermost dimension is contiguous.  The operators
-have no gradients: tensors that ask for them are refused while autograd records.  All arithmetic happens in libvadc_amd.so (include/vadc_amd.h: vadc_amd_linear, ...); a wrong
+have no gradients: tensors that ask for them are refused while autograd records.  What a call writes in place (`out`, `state`) counts as changed for autograd, as by torch's own in-place
+operations: a graph that saved it raises in its backward.  All arithmetic happens in libvadc_amd.so (include/vadc_amd.h: vadc_amd_linear, ...); a wrong
 argument raises ValueError or TypeError before the device is touched, a failure of the library VadcAmdError.
 """
 from __future__ import annotations
@@ -17,6 +18,7 @@ import struct
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .engine import VadcAmdError
@@ -247,7 +249,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     plan = _plan_linear(_layout(x), _layout(weight), _layout(bias), _layout(residual), _layout(out), activation, residual_first)
     if torch.is_grad_enabled():
         _no_grad("linear", x, weight, bias, residual, out)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = x.new_empty(plan.shape)
     else:
         _apart("linear", plan.spans, out, (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)), ("residual",))
@@ -255,6 +258,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
         _check(_lib.load().vadc_amd_linear(_LINEAR.pack(
             x.data_ptr(), weight.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if residual is None else residual.data_ptr(), out.data_ptr(), *plan.fields),
             torch._C._cuda_getCurrentRawStream(plan.device)))
+        if not fresh:
+            increment_version(out)
     return out
 
 
@@ -297,7 +302,8 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
     plan = _plan_norm(_layout(x), groups, _layout(weight), _layout(bias), eps, activation, _layout(gate), _layout(lengths), _layout(out))
     if torch.is_grad_enabled():
         _no_grad("group_norm", x, weight, bias, gate, out)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = x.new_empty(plan.shape) if lengths is None else x.new_zeros(plan.shape)
     else:
         _apart("group_norm", plan.spans, out, (("x", x), ("weight", weight), ("bias", bias), ("gate", gate), ("lengths", lengths)), ("x", "gate"))
@@ -307,6 +313,8 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
             x.data_ptr(), 0 if weight is None else weight.data_ptr(), 0 if bias is None else bias.data_ptr(), 0 if gate is None else gate.data_ptr(), out.data_ptr(),
             0 if lengths is None else lengths.data_ptr(), 0 if space is None else space.data_ptr(), plan.workspace, *plan.fields),
             torch._C._cuda_getCurrentRawStream(plan.device)))
+        if not fresh:
+            increment_version(out)
     return out
 
 
@@ -366,7 +374,8 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor
     plan = _plan_delta(_layout(q), _layout(k), _layout(v), _layout(log_decay), _layout(beta), _layout(state), scale, normalize, _layout(lengths), _layout(out))
     if torch.is_grad_enabled():
         _no_grad("gated_delta", q, k, v, log_decay, beta, state, out)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = v.new_empty(plan.shape) if lengths is None else v.new_zeros(plan.shape)
     else:
         _apart("gated_delta", plan.spans, out, (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("state", state), ("lengths", lengths)))
@@ -376,4 +385,5 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor
         space = torch.empty(plan.workspace, dtype=torch.uint8, device=v.device) if plan.workspace else None
         _check(_lib.load().vadc_amd_gated_delta(_DELTA.pack(*at[:6], out.data_ptr(), at[6], 0 if space is None else space.data_ptr(), plan.workspace, *plan.fields),
                                                 torch._C._cuda_getCurrentRawStream(plan.device)))
+        increment_version((state,) if fresh else (state, out))
     return out
