@@ -744,3 +744,19 @@ def test_writes_in_place_are_seen_by_autograd(ops, t):
     with torch.inference_mode():
         s = state.clone()
         assert torch.equal(ops.gated_delta(q, k, v, g, beta, s), ops.gated_delta(q, k, v, g, beta, state))
+
+
+def test_tangents_are_refused(ops):
+    from torch.autograd import forward_ad
+
+    rnd = gen(14)
+    x, w = rnd(5, 16), rnd(8, 16)
+    q, k, v, g, beta, state = delta_inputs(8, 2, 3, 1, 2, 16, 24, torch.float32, True)
+    with forward_ad.dual_level():
+        assert torch.equal(ops.linear(x, w), ops.linear(x, w))       # no tangent: taken
+        dual = {a: forward_ad.make_dual(b, torch.ones_like(b)) for a, b in (("x", x), ("w", w), ("state", state), ("g", g))}
+        with torch.no_grad():
+            for call in (lambda: ops.linear(dual["x"], w), lambda: ops.linear(x, dual["w"]), lambda: ops.group_norm(dual["x"], 2), lambda: ops.gated_delta(q, k, v, g, beta, dual["state"]),
+                         lambda: ops.gated_delta(q, k, v, dual["g"], beta, state)):
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call()

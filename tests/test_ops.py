@@ -263,3 +263,24 @@ def test_a_state_that_overlaps_an_input_is_refused(name):
     with pytest.raises(ValueError, match=f"state overlaps {name}"):
         check(dict(a, **{name: placed(39)}))
     check(dict(a, **{name: placed(40)}))                             # between two streams' states
+
+
+def test_a_tangent_is_refused():
+    """forward mode: no result may lose its tangent in silence, under torch.no_grad() either; the same tensors without tangents pass this check"""
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(t(3, 8), t(3, 8))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="linear has no forward-mode derivative"):
+                ops._no_grad("linear", t(3, 8), None, x)
+        ops._no_grad("linear", t(3, 8), forward_ad.unpack_dual(x).primal)
+        with forward_ad._set_fwd_grad_enabled(False):
+            ops._no_grad("linear", x)
+
+    def refused(x):
+        with pytest.raises(ValueError, match="forward-mode"):
+            ops._no_grad("linear", x)
+        return x.sum()
+
+    torch.func.jvp(refused, (t(3),), (t(3),))

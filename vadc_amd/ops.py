@@ -6,7 +6,7 @@
 
 Tensors are torch tensors on one gfx950 device, of one type (float32, float16 or bfloat16); the work is enqueued on torch's current stream of that device and may be captured into a
 graph.  Sums, statistics and states are float32, an output is rounded once.  Strided tensors are taken as they are, as long as the innermost dimension is contiguous.  The operators
-have no gradients: tensors that ask for them are refused while autograd records.  What a call writes in place (`out`, `state`) counts as changed for autograd, as by torch's own in-place
+have no gradients: tensors that ask for them are refused while autograd records, as are tensors with a forward-mode tangent.  What a call writes in place (`out`, `state`) counts as changed for autograd, as by torch's own in-place
 operations: a graph that saved it raises in its backward.  All arithmetic happens in libvadc_amd.so (include/vadc_amd.h: vadc_amd_linear, ...); a wrong
 argument raises ValueError or TypeError before the device is touched, a failure of the library VadcAmdError.
 """
@@ -18,6 +18,7 @@ import struct
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib
@@ -71,9 +72,13 @@ def _check(rc: int) -> int:
 
 
 def _no_grad(what: str, *ts: Optional[Tensor]):
+    """no tensor asks for a gradient while autograd records, none carries a tangent (torch.no_grad() leaves those on)"""
     for t in ts:
-        if t is not None and t.requires_grad:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or with tensors that ask for none")
+        if t is not None and forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and (
+                torch._C._functorch.is_functorch_wrapped_tensor(t) or forward_ad.unpack_dual(t).tangent is not None):
+            raise ValueError(f"{what} has no forward-mode derivative: call it with tensors that carry no tangent")
 
 
 def _same_device(what: str, *ls: Optional[_Layout]) -> int:
@@ -247,7 +252,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     x [..., in], weight [out, in], bias [out], residual [..., out]; returns [..., out] (in `out`, if given, which may be the residual).  Leading dimensions must make up rows at one
     distance.  activation: none, relu, silu, gelu (with erf), sigmoid."""
     plan = _plan_linear(_layout(x), _layout(weight), _layout(bias), _layout(residual), _layout(out), activation, residual_first)
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         _no_grad("linear", x, weight, bias, residual, out)
     fresh = out is None
     if fresh:
@@ -300,7 +305,7 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
     x [sequences, positions, channels], or [tokens, channels] (each token a sequence of one position); gate like x; weight, bias [channels].  lengths [sequences] (int32): sequence n
     has its first lengths[n] positions only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given).  `out` may be x or gate."""
     plan = _plan_norm(_layout(x), groups, _layout(weight), _layout(bias), eps, activation, _layout(gate), _layout(lengths), _layout(out))
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         _no_grad("group_norm", x, weight, bias, gate, out)
     fresh = out is None
     if fresh:
@@ -372,7 +377,7 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor
     only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given); a stream of no steps keeps its state.  A value that is not finite makes NaN of
     what it reaches: its column of the state and of the outputs from its step on (a key or gate: every column of its head; a query: its own outputs)."""
     plan = _plan_delta(_layout(q), _layout(k), _layout(v), _layout(log_decay), _layout(beta), _layout(state), scale, normalize, _layout(lengths), _layout(out))
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         _no_grad("gated_delta", q, k, v, log_decay, beta, state, out)
     fresh = out is None
     if fresh:
