@@ -284,3 +284,25 @@ def test_a_tangent_is_refused():
         return x.sum()
 
     torch.func.jvp(refused, (t(3),), (t(3),))
+
+
+def test_a_refusal_does_not_depend_on_what_ran_before():
+    """an argument that equals one of a kept plan, but is of a type that is refused"""
+    gpu = torch.device("cuda", 0)
+
+    def layout(*shape):
+        return (torch.Size(shape), t(*shape).stride(), torch.float32, gpu)
+
+    def norm(groups):
+        return ops._plan_norm(layout(3, 8), groups, None, None, 1e-5, "none", None, None, None)
+
+    def linear(first):
+        return ops._plan_linear(layout(3, 5), layout(4, 5), None, None, None, "none", first)
+
+    def delta(normalize):
+        return ops._plan_delta(layout(2, 3, 1, 4), layout(2, 3, 1, 4), layout(2, 3, 2, 5), layout(2, 3, 2), layout(2, 3, 2), layout(2, 2, 4, 5), None, normalize, None, None)
+
+    for call, good, bad in ((norm, 2, 2.0), (linear, True, 1.0), (delta, False, 0.0)):
+        assert call(good) is call(good)
+        with pytest.raises(TypeError):
+            call(bad)

@@ -47,7 +47,7 @@ class _Plan(NamedTuple):
     empty: bool              # nothing to do
 
 
-_KEPT = 1024                 # plans, the least recently used go first
+_KEPT = 1024                 # plans, the least recently used go first; by the arguments' types as well: 2.0 equals 2, but is refused as a number of groups, whatever ran before
 
 
 class _Layout(NamedTuple):
@@ -222,7 +222,7 @@ def _rows(what: str, name: str, v: Optional[_Layout]):
     return v.shape[-1] if distance is None else distance
 
 
-@functools.lru_cache(_KEPT)
+@functools.lru_cache(_KEPT, typed=True)
 def _plan_linear(x, weight, bias, residual, out, activation, residual_first) -> _Plan:
     x, weight, bias, residual, out = _layouts(x, weight, bias, residual, out)
     if len(weight.shape) != 2 or len(x.shape) < 1 or x.shape[-1] != weight.shape[1]:
@@ -268,7 +268,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     return out
 
 
-@functools.lru_cache(_KEPT)
+@functools.lru_cache(_KEPT, typed=True)
 def _plan_norm(x, groups, weight, bias, eps, activation, gate, lengths, out) -> _Plan:
     x, weight, bias, gate, lengths, out = _layouts(x, weight, bias, gate, lengths, out)
     if len(x.shape) not in (2, 3):
@@ -323,7 +323,7 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
     return out
 
 
-@functools.lru_cache(_KEPT)
+@functools.lru_cache(_KEPT, typed=True)
 def _plan_delta(q, k, v, log_decay, beta, state, scale, normalize, lengths, out) -> _Plan:
     q, k, v, log_decay, beta, state, lengths, out = _layouts(q, k, v, log_decay, beta, state, lengths, out)
     if len(q.shape) != 4 or k.shape != q.shape or len(v.shape) != 4 or v.shape[:2] != q.shape[:2]:
