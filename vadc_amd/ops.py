@@ -58,7 +58,10 @@ class _Layout(NamedTuple):
 
 
 def _layout(t: Optional[Tensor]):
-    return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    try:
+        return None if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    except (AttributeError, RuntimeError):           # an array, a list; a tensor without strides
+        raise TypeError(f"the operators take strided torch tensors, not {type(t).__name__}") from None
 
 
 def _layouts(*ls):
@@ -92,6 +95,12 @@ def _same_device(what: str, *ls: Optional[_Layout]) -> int:
 
 
 _LARGEST = 3.4e38            # of float32, short of its last digits
+
+
+def _given(what: str, **ls: Optional[_Layout]):
+    for name, v in ls.items():
+        if v is None:
+            raise TypeError(f"{what}: {name} must be a tensor, not None")
 
 
 def _flag(what: str, **flags):
@@ -225,6 +234,7 @@ def _rows(what: str, name: str, v: Optional[_Layout]):
 @functools.lru_cache(_KEPT, typed=True)
 def _plan_linear(x, weight, bias, residual, out, activation, residual_first) -> _Plan:
     x, weight, bias, residual, out = _layouts(x, weight, bias, residual, out)
+    _given("linear", x=x, weight=weight)
     if len(weight.shape) != 2 or len(x.shape) < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"linear: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit")
     n, k = weight.shape
@@ -271,6 +281,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
 @functools.lru_cache(_KEPT, typed=True)
 def _plan_norm(x, groups, weight, bias, eps, activation, gate, lengths, out) -> _Plan:
     x, weight, bias, gate, lengths, out = _layouts(x, weight, bias, gate, lengths, out)
+    _given("group_norm", x=x)
     if len(x.shape) not in (2, 3):
         raise ValueError(f"group_norm: x {tuple(x.shape)} is neither [sequences, positions, channels] nor [tokens, channels]")
     n, l, c = x.shape if len(x.shape) == 3 else (x.shape[0], 1, x.shape[1])
@@ -326,6 +337,7 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
 @functools.lru_cache(_KEPT, typed=True)
 def _plan_delta(q, k, v, log_decay, beta, state, scale, normalize, lengths, out) -> _Plan:
     q, k, v, log_decay, beta, state, lengths, out = _layouts(q, k, v, log_decay, beta, state, lengths, out)
+    _given("gated_delta", q=q, k=k, v=v, log_decay=log_decay, beta=beta, state=state)
     if len(q.shape) != 4 or k.shape != q.shape or len(v.shape) != 4 or v.shape[:2] != q.shape[:2]:
         raise ValueError(f"gated_delta: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit")
     b, t, hk, dk = q.shape
