@@ -308,7 +308,7 @@ def test_a_refusal_does_not_depend_on_what_ran_before():
             call(bad)
 
 
-@pytest.mark.parametrize("what", (None, [[1.0, 2.0]], 3.0, t(3, 5).numpy(), t(3, 5).to_sparse()))
+@pytest.mark.parametrize("what", (None, [[1.0, 2.0]], 3.0, t(3, 5).numpy(), t(3, 5).to_sparse_csr()))
 def test_what_is_no_tensor_is_refused(what):
     for call in (lambda: ops.linear(what, t(4, 5)), lambda: ops.linear(t(3, 5), what), lambda: ops.group_norm(what, 1), lambda: ops.gated_delta(**delta_args(log_decay=what)),
                  lambda: ops.gated_delta(**delta_args(state=what))):
