@@ -729,8 +729,8 @@ def test_writes_in_place_are_seen_by_autograd(ops, t):
     rnd = gen(13)
     q, k, v, g, beta, state = delta_inputs(8, 2, t, 1, 2, 16, 24, torch.float32, True)
     x, w, z = rnd(30, 16), rnd(24, 16), rnd(30, 24)
-    for written, call in ((state, lambda: ops.gated_delta(q, k, v, g, beta, state)), (state, lambda: ops.gated_delta(q, k, v, g, beta, state[:])),
-                          (v, lambda: ops.gated_delta(q, k, v.clone(), g, beta, state, out=v)), (z, lambda: ops.linear(x, w, residual=z, out=z)), (z, lambda: ops.group_norm(z, 4, out=z)),
+    for written, call in ((state, lambda: ops.gated_delta(q, k, v, g, beta, state, normalize=True)), (state, lambda: ops.gated_delta(q, k, v, g, beta, state[:], normalize=True)),
+                          (v, lambda: ops.gated_delta(q, k, v.clone(), g, beta, state, normalize=True, out=v)), (z, lambda: ops.linear(x, w, residual=z, out=z)), (z, lambda: ops.group_norm(z, 4, out=z)),
                           (z, lambda: ops.linear(x[:10], w, out=z[:10]))):
         weight = torch.ones_like(written, requires_grad=True)
         loss = (written * weight).sum()
@@ -739,11 +739,11 @@ def test_writes_in_place_are_seen_by_autograd(ops, t):
             loss.backward()
     before = (q._version, x._version, w._version)
     ops.linear(x, w)
-    ops.gated_delta(q, k, v, g, beta, state)
+    ops.gated_delta(q, k, v, g, beta, state, normalize=True)
     assert (q._version, x._version, w._version) == before
     with torch.inference_mode():
         s = state.clone()
-        assert torch.equal(ops.gated_delta(q, k, v, g, beta, s), ops.gated_delta(q, k, v, g, beta, state))
+        assert torch.equal(ops.gated_delta(q, k, v, g, beta, s, normalize=True), ops.gated_delta(q, k, v, g, beta, state, normalize=True))
 
 
 def test_tangents_are_refused(ops):

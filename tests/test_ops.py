@@ -246,7 +246,7 @@ def test_a_state_that_overlaps_an_input_is_refused(name):
 
     def check(a):
         ts = [a[n] for n in names]
-        ops._state_apart(tuple(ops._span(ops._Layout(*ops._layout(x))) for x in ts), [x.data_ptr() for x in ts], *ts)
+        ops._state_apart(tuple(ops._span(ops._Layout(*ops._layout(x))) for x in ts), *ts)
 
     a = delta_args(b=2, h=2, dk=4, dv=5, lengths=torch.zeros(2, dtype=torch.int32))
     check(a)

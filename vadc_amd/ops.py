@@ -371,12 +371,9 @@ def _plan_delta(q, k, v, log_decay, beta, state, scale, normalize, lengths, out)
     return _Plan(fields, tuple(v.shape), device, tuple(map(_span, (q, k, v, log_decay, beta, state, lengths, out))), space, empty)
 
 
-def _state_apart(spans: tuple, at: list, q, k, v, log_decay, beta, state, lengths):
-    """state, which is written, overlaps no input; `at`: the tensors' addresses"""
-    lo = at[5]
-    hi = lo + spans[5]
-    if sum(p < hi and lo < p + span for p, span in zip(at, spans)) > 1:      # another one than its own
-        _apart("gated_delta", (*spans[:5], spans[6], spans[5]), state, (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("lengths", lengths)), written="state")
+def _state_apart(spans: tuple, q, k, v, log_decay, beta, state, lengths):
+    """state, which is written, overlaps no input"""
+    _apart("gated_delta", (*spans[:5], spans[6], spans[5]), state, (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("lengths", lengths)), written="state")
 
 
 def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor, state: Tensor, scale: Optional[float] = None, normalize: bool = False,
@@ -397,10 +394,14 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor
     else:
         _apart("gated_delta", plan.spans, out, (("q", q), ("k", k), ("v", v), ("log_decay", log_decay), ("beta", beta), ("state", state), ("lengths", lengths)))
     if not plan.empty:
-        at = [q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), 0 if lengths is None else lengths.data_ptr()]
-        _state_apart(plan.spans, at, q, k, v, log_decay, beta, state, lengths)
+        at_q, at_k, at_v, at_g, at_b, lo, at_n = q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), state.data_ptr(), 0 if lengths is None else lengths.data_ptr()
+        n_q, n_k, n_v, n_g, n_b, n_s, n_n, _ = plan.spans
+        hi = lo + n_s
+        if (at_q < hi and lo < at_q + n_q or at_k < hi and lo < at_k + n_k or at_v < hi and lo < at_v + n_v or at_g < hi and lo < at_g + n_g or at_b < hi and lo < at_b + n_b
+                or at_n < hi and lo < at_n + n_n):   # in line: 0.3 us of a step's 8
+            _state_apart(plan.spans, q, k, v, log_decay, beta, state, lengths)
         space = torch.empty(plan.workspace, dtype=torch.uint8, device=v.device) if plan.workspace else None
-        _check(_lib.load().vadc_amd_gated_delta(_DELTA.pack(*at[:6], out.data_ptr(), at[6], 0 if space is None else space.data_ptr(), plan.workspace, *plan.fields),
+        _check(_lib.load().vadc_amd_gated_delta(_DELTA.pack(at_q, at_k, at_v, at_g, at_b, lo, out.data_ptr(), at_n, 0 if space is None else space.data_ptr(), plan.workspace, *plan.fields),
                                                 torch._C._cuda_getCurrentRawStream(plan.device)))
         increment_version((state,) if fresh else (state, out))
     return out
