@@ -760,3 +760,35 @@ def test_tangents_are_refused(ops):
                          lambda: ops.gated_delta(q, k, v, dual["g"], beta, state)):
                 with pytest.raises(ValueError, match="forward-mode"):
                     call()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("normalize", (True, False))
+@pytest.mark.parametrize("t, at, dk, dv", [(1, 0, 32, 24), (6, 2, 64, 32), (6, 5, 40, 3), (90, 40, 64, 32), (90, 89, 128, 40), (90, 0, 100, 17), (40, 30, 200, 24)])
+def test_gated_delta_what_is_not_finite(ops, t, at, dk, dv, normalize, dtype):
+    """one value that is not finite, in each operand, in either form: NaN in its column (a key or gate: all columns; a query: its own outputs) of its head from its step on, every other bit as without it"""
+    q, k, v, g, beta, state = delta_inputs(t + dk, 2, t, 2, 4, dk, dv, TYPES[dtype], normalize)
+    clean = state.clone()
+    want = ops.gated_delta(q, k, v, g, beta, clean, normalize=normalize)
+    for value in (math.inf, -math.inf, math.nan):
+        for name in ("q", "k", "v", "g", "beta", "state"):
+            if name == "g" and value == -math.inf:
+                continue                             # a state that is forgotten
+            a = dict(q=q.clone(), k=k.clone(), v=v.clone(), g=g.clone(), beta=beta.clone(), state=state.clone())
+            outs, states = torch.zeros_like(want, dtype=torch.bool), torch.zeros_like(state, dtype=torch.bool)
+            if name in ("q", "k"):
+                a[name][1, at, 1, 7] = value         # the heads 2 and 3
+                outs[1, at:(at + 1 if name == "q" else t), 2:] = True
+                states[1, 2:] = name == "k"
+            elif name == "v":
+                a[name][1, at, 1, 2] = value
+                outs[1, at:, 1, 2], states[1, 1, :, 2] = True, True
+            elif name == "state":
+                a[name][1, 1, 5, 2] = value
+                outs[1, :, 1, 2], states[1, 1, :, 2] = True, True
+            else:
+                a[name][1, at, 1] = value
+                outs[1, at:, 1], states[1, 1] = True, True
+            got = ops.gated_delta(a["q"], a["k"], a["v"], a["g"], a["beta"], a["state"], normalize=normalize)
+            assert torch.equal(torch.isnan(got), outs) and torch.equal(torch.isnan(a["state"]), states), (name, value)
+            assert torch.equal(got[~outs], want[~outs]) and torch.equal(a["state"][~states], clean[~states]), (name, value)

@@ -16,7 +16,8 @@ __device__ __forceinline__ int64_t live_steps(const vadc_amd_gated_delta_args &a
 }
 
 // Step by step.  A workgroup holds 16 VEC columns of one state in registers: thread (r, c) the rows r, r + 16, ... of VEC columns.  S^T k and S^T q of the OLD state
-// come out of one reduction, because S^T q = e^g S_old^T q + (k . q) u.  Unit length of q and k is a factor behind the sums.
+// come out of one reduction, because S^T q = e^g S_old^T q + (k . q) u.  Unit length of q and k is a factor behind the sums.  What is not finite ends in u, in every column that it reaches, or,
+// of a query, in its outputs: NaN is put there, as blocks put it, so that an infinity leaves the same whichever form a call takes.
 template <typename T, int VEC, int ROWS>
 __global__ __launch_bounds__(256) void k_delta_step(const vadc_amd_gated_delta_args a)
 {
@@ -91,8 +92,10 @@ __global__ __launch_bounds__(256) void k_delta_step(const vadc_amd_gated_delta_a
       for (int j = 0; j < VEC; ++j) {
          const float fk = (part[at][0][0][c + j] + part[at][1][0][c + j]) + (part[at][2][0][c + j] + part[at][3][0][c + j]);
          const float fq = (part[at][0][1][c + j] + part[at][1][1][c + j]) + (part[at][2][1][c + j] + part[at][3][1][c + j]);
-         const float u = beta * (vv[j] - decay * rk * fk);
+         float u = beta * (vv[j] - decay * rk * fk);
+         u = fabsf(u) < INFINITY ? u : NAN;
          o[j] = rq * (decay * fq + d[2] * rk * u);
+         if (!(d[0] < INFINITY)) o[j] = fabsf(o[j]) < INFINITY ? o[j] : NAN;
          const float ku = rk * u;
 #pragma unroll
          for (int i = 0; i < ROWS; ++i) s[i][j] = fmaf(sk[at][r + 16 * i], ku, decay * s[i][j]);
