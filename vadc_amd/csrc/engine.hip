@@ -916,16 +916,19 @@ static int ensure_pipeline_streams(vadc_amd_engine *e, int n_streams, int lk)
    bool masked = false;
    if (want > 0) {
       const int words = (e->n_cus + 31) / 32;
-      const int wb = split ? want / 2 : want;
+      // a mask that leaves an XCD without a CU is refused by some drivers (hipErrorOutOfMemory: bits go to the 8 XCDs in turn, so a half needs 8): the layers then share the partition
+      const bool halves = split && want / 2 >= 8;
+      const int wb = halves ? want / 2 : want;
       std::vector<uint32_t> mb(words, 0u), mc(words, 0u), ma(words, 0u);
       for (int cu = 0; cu < e->n_cus; ++cu) (cu < wb ? mb : (cu < want ? mc : ma))[cu / 32] |= 1u << (cu % 32);
-      if (!split) mc = mb;
+      if (!halves) mc = mb;
       if (shared) for (int cu = 0; cu < want; ++cu) ma[cu / 32] |= 1u << (cu % 32);   // the LSTM keeps its CUs, the other stream may use them too
       hipError_t ea = hipExtStreamCreateWithCUMask(&e->sA, (uint32_t)words, ma.data());
       hipError_t eb = (ea == hipSuccess) ? hipExtStreamCreateWithCUMask(&e->sB, (uint32_t)words, mb.data()) : ea;
       hipError_t ec = (eb == hipSuccess) ? hipExtStreamCreateWithCUMask(&e->sC, (uint32_t)words, mc.data()) : eb;
       masked = (ea == hipSuccess && eb == hipSuccess && ec == hipSuccess);
       if (!masked) {
+         if (getenv("VADC_AMD_DEBUG_CUMASK")) fprintf(stderr, "partition of %d CUs refused: %s\n", want, hipGetErrorString(ec));
          (void)hipGetLastError();
          for (hipStream_t *ps : {&e->sA, &e->sB, &e->sC}) if (*ps) { (void)hipStreamDestroy(*ps); *ps = nullptr; }
       }
