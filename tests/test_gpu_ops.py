@@ -792,3 +792,55 @@ def test_gated_delta_what_is_not_finite(ops, t, at, dk, dv, normalize, dtype):
             got = ops.gated_delta(a["q"], a["k"], a["v"], a["g"], a["beta"], a["state"], normalize=normalize)
             assert torch.equal(torch.isnan(got), outs) and torch.equal(torch.isnan(a["state"]), states), (name, value)
             assert torch.equal(got[~outs], want[~outs]) and torch.equal(a["state"][~states], clean[~states]), (name, value)
+
+
+# float32 products in tiles, both sizes of them: far from the sizes where a narrower form takes over (512 blocks of 64 rows x 16 features) and from each other (200 tiles of 128 x 128)
+PARTS_SIZES = [(1025, 1900), (2049, 2500)]
+
+
+@pytest.mark.parametrize("m, n", PARTS_SIZES)
+@pytest.mark.parametrize("k", (128, 131))
+def test_linear_float32_tiles_infinities_and_nan(ops, m, n, k):
+    """an infinity or NaN reaches the outputs of its row or feature, as in the definition, and no other"""
+    rnd = gen(m + k)
+    x, w = rnd(m, k), rnd(n, k)
+    x[0, 3], x[1, 64], x[m - 1, k - 1], x[700, 0] = math.inf, math.nan, -math.inf, math.inf
+    w[7, 5], w[n - 1, k - 1], w[70, 3] = -math.inf, math.nan, 0.0    # (infinity times zero)
+    got, want = ops.linear(x, w).double(), linear64(x, w, None, "none", None, False)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.isinf(got), torch.isinf(want)) and torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    ok = torch.isfinite(want)
+    x, w = x.nan_to_num(0, 0, 0), w.nan_to_num(0, 0, 0)
+    within(torch.where(ok, got, 0.0), torch.where(ok, want, 0.0), linear_tol(x, w, None, None, torch.where(ok, want, 0.0), torch.float32))
+
+
+@pytest.mark.parametrize("m, n", PARTS_SIZES)
+def test_linear_float32_tiles_range(ops, m, n):
+    """operands near the ends of the range.  An operand's three bfloat16 parts end at bfloat16's smallest number, 2^-133: what is left of it is at most half of that, 2^-134 times the other factor"""
+    w = torch.full((n, 64), 2.0 ** -30, device="cuda")
+    x = torch.full((m, 64), 3.4e38, device="cuda")
+    want = linear64(x, w, None, "none", None, False)
+    within(ops.linear(x, w), want, linear_tol(x, w, None, None, want, torch.float32))
+    w = gen(m)(n, 64) * 2.0 ** 40
+    for e in (-60, -100, -108, -112, -116, -120, -126, -130, -140):
+        x = gen(n)(m, 64) * 2.0 ** e
+        want = linear64(x, w, None, "none", None, False)
+        tol = (64 + 8) * U * (x.double().abs() @ w.double().abs().T) + 2.0 ** -134 * w.double().abs().sum(1)
+        within(ops.linear(x, w), want, tol)
+        within(ops.linear(w, x), want.T, tol.T)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("mode", ("none", "after", "before"))
+@pytest.mark.parametrize("m, n", PARTS_SIZES)
+def test_linear_float32_tiles_epilogues(ops, m, n, mode, act):
+    rnd = gen(m)
+    x, w, b, r = rnd(m, 96), rnd(n, 96) * 0.3, rnd(n), rnd(m, n)
+    r = None if mode == "none" else r
+    want = linear64(x, w, b, act, r, mode == "before")
+    tol = linear_tol(x, w, b, r, want, torch.float32)
+    within(ops.linear(x, w, bias=b, activation=act, residual=r, residual_first=mode == "before"), want, tol)
+    if r is not None:                                # in place, and in rows that are further apart
+        wide = torch.empty(m, n + 5, device="cuda")[:, 3:n + 3]
+        wide.copy_(r)
+        within(ops.linear(x, w, bias=b, activation=act, residual=wide, residual_first=mode == "before", out=wide), want, tol)
