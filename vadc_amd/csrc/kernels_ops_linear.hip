@@ -173,20 +173,20 @@ __device__ __forceinline__ const void *uniform(const void *p)
    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
    return (const void *)(const __attribute__((address_space(1))) char *)(uintptr_t)((uint64_t)hi << 32 | lo);      // global: a generic pointer's loads would count with those of LDS
 }
-template <int N> __device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
+__device__ __forceinline__ void vm_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // BM rows x BN features per tile, WR x WC waves of (BM / WR) x (BN / WC) outputs in 32 x 32 tiles.  The weight is the A operand: a lane's accumulators are groups of four consecutive
-// features of one row.  STAGES tiles of k are in LDS or on their way there: with DMA (16-byte aligned rows) a wave waits for the oldest with a counted vmcnt -- an operation the count does
-// not know of can only make it wait longer -- and one barrier a tile lets everybody read it and the next one overwrite the last; without, tiles pass through registers.
+// features of one row.  Two tiles of k are in LDS, one that is read and one on its way there: with DMA (16-byte aligned rows) a wave waits for all that it has on its way -- the next tile of k,
+// and, in the first step behind outputs, their stores -- and one barrier a tile lets everybody read it and the one after overwrite the last; without, tiles pass through registers.
 // A workgroup does every gridDim-th output tile; the next one's first tiles of k are fetched before this one's outputs leave, which takes as long as a few tiles of k.
 // KG groups of waves take every KG-th tile of k each, where there are too few output tiles to fill the device with work.
-template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES, int KG, bool DMA>
+template <typename T, int BM, int BN, int WR, int WC, int RB, int KG, bool DMA>
 __global__ __launch_bounds__(64 * WR * WC * KG, (512 + 64 * WR * WC * KG - 1) / (64 * WR * WC * KG)) void k_linear_tile(const vadc_amd_linear_args a)
 {
    constexpr int WAVES = WR * WC, KT = RB / (int)sizeof(T), TM = BM / WR / 32, TN = BN / WC / 32, BYTES = (BM + BN) * RB, PER = 16 / (int)sizeof(T);
    constexpr int ROWS = 1024 / RB, XP = BM / ROWS / WAVES, PIECES = (BM + BN) / ROWS / WAVES;      // LDS rows of a DMA instruction; a wave's instructions for x, for both
    static_assert(BM % (ROWS * WAVES) == 0 && BN % (ROWS * WAVES) == 0, "every wave does the same");
-   __shared__ __attribute__((aligned(16))) char lds[STAGES * KG * BYTES];
+   __shared__ __attribute__((aligned(16))) char lds[2 * KG * BYTES];
    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6) % WAVES, kg = __builtin_amdgcn_readfirstlane(tid >> 6) / WAVES;
    const int64_t tiles_m = (a.rows + BM - 1) / BM, tiles_n = (a.out_features + BN - 1) / BN;
    const unsigned tiles = (unsigned)(tiles_m * tiles_n);
@@ -256,11 +256,9 @@ __global__ __launch_bounds__(64 * WR * WC * KG, (512 + 64 * WR * WC * KG - 1) / 
 
    unsigned index = blockIdx.x;
    aim(index);
-   int stage = 0;                                                     // of the next tile of k
-   const auto step = [](int stage, int by) { const int s = stage + by; return s < STAGES ? s : s - STAGES; };
-   const int ahead = (int)min(whole, (int64_t)(STAGES - 1));
+   int stage = 0;                                                     // of the next tile of k; the other one is free, or about to be
    if constexpr (DMA)
-      for (int i = 0; i < ahead; ++i) issue(i, step(stage, i));
+      if (whole) issue(0, stage);
    const bool part = a.in_features % KT != 0, parts_mine = kg == KG - 1;      // the part of a tile at the end comes first, while no sums are held; the last group has the least else
    const auto clear = [&] {
 #pragma unroll
@@ -274,17 +272,17 @@ __global__ __launch_bounds__(64 * WR * WC * KG, (512 + 64 * WR * WC * KG - 1) / 
          if (part) {                                                  // through registers, into the stage that is free
             if (parts_mine) fetch_part(held);
             lds_barrier();
-            if (parts_mine) place(step(stage, STAGES - 1), held);
+            if (parts_mine) place(stage ^ 1, held);
             lds_barrier();
          }
          clear();
-         if (part && parts_mine) compute(step(stage, STAGES - 1));
+         if (part && parts_mine) compute(stage ^ 1);
          for (int64_t kt = 0; kt < rounds; ++kt) {
-            if (whole - kt >= STAGES - 1) vm_wait<PIECES * (STAGES - 2)>(); else vm_wait<0>();
+            vm_wait();
             lds_barrier();
-            if (kt + STAGES - 1 < whole) issue(kt + STAGES - 1, step(stage, STAGES - 1));
+            if (kt + 1 < whole) issue(kt + 1, stage ^ 1);
             if (KG == 1 || kt < whole) compute(stage);
-            stage = step(stage, 1);
+            stage ^= 1;
          }
       } else {
          if (part && parts_mine) fetch_part(held);
@@ -314,9 +312,9 @@ __global__ __launch_bounds__(64 * WR * WC * KG, (512 + 64 * WR * WC * KG - 1) / 
       if (more) {
          aim(index);
          if constexpr (DMA)
-            for (int i = 0; i < ahead; ++i) issue(i, step(stage, i));
+            if (whole) issue(0, stage);
       }
-      leave<T, TN, TM, FEATS, KG>(a, reinterpret_cast<f4 *>(lds + (DMA ? step(stage, STAGES - 1) : 0) * KG * BYTES) + wave * 8 * FEATS, kg, BYTES / 16, acc, row + wr, col + wc, lane);
+      leave<T, TN, TM, FEATS, KG>(a, reinterpret_cast<f4 *>(lds + (DMA ? stage ^ 1 : 0) * KG * BYTES) + wave * 8 * FEATS, kg, BYTES / 16, acc, row + wr, col + wc, lane);
       if (!more) break;
    }
 }
@@ -535,13 +533,13 @@ __global__ __launch_bounds__(512) void k_linear_narrow(const vadc_amd_linear_arg
 }
 
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
-template <typename T, int BM, int BN, int WR, int WC, int RB, int STAGES, int KG> static void launch_tile(const vadc_amd_linear_args &a, hipStream_t s, bool dma)
+template <typename T, int BM, int BN, int WR, int WC, int RB, int KG> static void launch_tile(const vadc_amd_linear_args &a, hipStream_t s, bool dma)
 {
    constexpr int threads = 64 * WR * WC * KG;
    constexpr int64_t slots = 256 * std::max(1, 512 / threads);         // 512 threads a CU at a time
    const dim3 grid((unsigned)std::min(slots, ((a.rows + BM - 1) / BM) * ((a.out_features + BN - 1) / BN)));
-   if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, STAGES, KG, true>), grid, dim3(threads), 0, s, a);
-   else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, 2, KG, false>), grid, dim3(threads), 0, s, a);
+   if (dma) hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, KG, true>), grid, dim3(threads), 0, s, a);
+   else hipLaunchKernelGGL((k_linear_tile<T, BM, BN, WR, WC, RB, KG, false>), grid, dim3(threads), 0, s, a);
 }
 template <typename T, int TN, int TM> static void launch_narrow(const vadc_amd_linear_args &a, hipStream_t s)
 {
@@ -574,10 +572,10 @@ template <typename T> static void launch(const vadc_amd_linear_args &a, hipStrea
       // 32 x 4096 x 4096: 13.2 us, in tiles 16.6 us; 64 rows: 20.4 us.  The other case: a tile's rows are not within 32-bit offsets
       if (a.rows <= 32 || std::max(a.x_stride, a.weight_stride) * (int64_t)sizeof(T) >= (int64_t(1) << 31) / 256) return launch_narrow<T, 1, 2>(a, s);
       const bool dma = ((uintptr_t)a.x | (uintptr_t)a.weight) % 16 == 0 && a.x_stride % 8 == 0 && a.weight_stride % 8 == 0;
-      if (tiles(256) >= 200) launch_tile<T, 256, 256, 2, 4, 128, 2, 1>(a, s, dma);
-      else if (tiles(128) >= 200) launch_tile<T, 128, 128, 2, 2, 128, 2, 1>(a, s, dma);
-      else if (tiles(64) > 256 || a.in_features < 512) launch_tile<T, 64, 64, 2, 2, 256, 2, 1>(a, s, dma);
-      else launch_tile<T, 64, 64, 2, 2, 256, 2, 2>(a, s, dma);
+      if (tiles(256) >= 200) launch_tile<T, 256, 256, 2, 4, 128, 1>(a, s, dma);
+      else if (tiles(128) >= 200) launch_tile<T, 128, 128, 2, 2, 128, 1>(a, s, dma);
+      else if (tiles(64) > 256 || a.in_features < 512) launch_tile<T, 64, 64, 2, 2, 256, 1>(a, s, dma);
+      else launch_tile<T, 64, 64, 2, 2, 256, 2>(a, s, dma);
    }
 }
 
