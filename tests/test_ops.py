@@ -273,14 +273,14 @@ def test_a_tangent_is_refused():
         x = forward_ad.make_dual(t(3, 8), t(3, 8))
         for grad in (True, False):
             with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="linear has no forward-mode derivative"):
-                ops._no_grad("linear", t(3, 8), None, x)
-        ops._no_grad("linear", t(3, 8), forward_ad.unpack_dual(x).primal)
+                ops._no_tangent("linear", t(3, 8), None, x)
+        ops._no_tangent("linear", t(3, 8), forward_ad.unpack_dual(x).primal)
         with forward_ad._set_fwd_grad_enabled(False):
-            ops._no_grad("linear", x)
+            ops._no_tangent("linear", x)
 
     def refused(x):
         with pytest.raises(ValueError, match="forward-mode"):
-            ops._no_grad("linear", x)
+            ops._no_tangent("linear", x)
         return x.sum()
 
     torch.func.jvp(refused, (t(3),), (t(3),))

@@ -75,12 +75,15 @@ def _check(rc: int) -> int:
 
 
 def _no_grad(what: str, *ts: Optional[Tensor]):
-    """no tensor asks for a gradient while autograd records, none carries a tangent (torch.no_grad() leaves those on)"""
     for t in ts:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
+        if t is not None and t.requires_grad:
             raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or with tensors that ask for none")
-        if t is not None and forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and (
-                torch._C._functorch.is_functorch_wrapped_tensor(t) or forward_ad.unpack_dual(t).tangent is not None):
+
+
+def _no_tangent(what: str, *ts: Optional[Tensor]):
+    """inside a dual level of forward mode, which torch.no_grad() leaves on"""
+    for t in ts:
+        if t is not None and torch._C._is_fwd_grad_enabled() and (torch._C._functorch.is_functorch_wrapped_tensor(t) or forward_ad.unpack_dual(t).tangent is not None):
             raise ValueError(f"{what} has no forward-mode derivative: call it with tensors that carry no tangent")
 
 
@@ -262,8 +265,10 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, activation:
     x [..., in], weight [out, in], bias [out], residual [..., out]; returns [..., out] (in `out`, if given, which may be the residual).  Leading dimensions must make up rows at one
     distance.  activation: none, relu, silu, gelu (with erf), sigmoid."""
     plan = _plan_linear(_layout(x), _layout(weight), _layout(bias), _layout(residual), _layout(out), activation, residual_first)
-    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+    if torch.is_grad_enabled():
         _no_grad("linear", x, weight, bias, residual, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent("linear", x, weight, bias, residual, out)
     fresh = out is None
     if fresh:
         out = x.new_empty(plan.shape)
@@ -316,8 +321,10 @@ def group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Op
     x [sequences, positions, channels], or [tokens, channels] (each token a sequence of one position); gate like x; weight, bias [channels].  lengths [sequences] (int32): sequence n
     has its first lengths[n] positions only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given).  `out` may be x or gate."""
     plan = _plan_norm(_layout(x), groups, _layout(weight), _layout(bias), eps, activation, _layout(gate), _layout(lengths), _layout(out))
-    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+    if torch.is_grad_enabled():
         _no_grad("group_norm", x, weight, bias, gate, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent("group_norm", x, weight, bias, gate, out)
     fresh = out is None
     if fresh:
         out = x.new_empty(plan.shape) if lengths is None else x.new_zeros(plan.shape)
@@ -386,8 +393,10 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor
     only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given); a stream of no steps keeps its state.  A value that is not finite makes NaN of
     what it reaches: its column of the state and of the outputs from its step on (a key or gate: every column of its head; a query: its own outputs)."""
     plan = _plan_delta(_layout(q), _layout(k), _layout(v), _layout(log_decay), _layout(beta), _layout(state), scale, normalize, _layout(lengths), _layout(out))
-    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+    if torch.is_grad_enabled():
         _no_grad("gated_delta", q, k, v, log_decay, beta, state, out)
+    if forward_ad._current_level >= 0:
+        _no_tangent("gated_delta", q, k, v, log_decay, beta, state, out)
     fresh = out is None
     if fresh:
         out = v.new_empty(plan.shape) if lengths is None else v.new_zeros(plan.shape)
