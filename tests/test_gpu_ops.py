@@ -844,3 +844,20 @@ def test_linear_float32_tiles_epilogues(ops, m, n, mode, act):
         wide = torch.empty(m, n + 5, device="cuda")[:, 3:n + 3]
         wide.copy_(r)
         within(ops.linear(x, w, bias=b, activation=act, residual=wide, residual_first=mode == "before", out=wide), want, tol)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gelu_keeps_its_negative_tail(ops, dtype):
+    """relative, down to y = -12 (fp16: to its smallest numbers): the argument y / sqrt 2 and its constant are rounded, which erfc takes 2 (y / sqrt 2)^2 times, 2 y^2 u; erfc itself is good to 16
+    steps of 2 u, two products to u each; then half a step of the output's type"""
+    dt = TYPES[dtype]
+    y = torch.linspace(-12, 12, 48001, device="cuda").to(dt)
+    one = torch.ones(1, 1, dtype=dt, device="cuda")
+    want = 0.5 * y.double() * torch.special.erfc(-y.double() / 2 ** 0.5)
+    for rows, part in ((1, slice(None)), (300, slice(0, 9000)), (300, slice(20000, 29000))):
+        got = ops.linear(one.expand(rows, 1), y[part, None], activation="gelu")[rows // 2]
+        tol = (2 * y[part].double() ** 2 + 34) * U * want[part].abs()
+        within(got, want[part], tol * (1 + torch.finfo(dt).eps) + half_step(want[part], dt))
+    far = torch.tensor([-math.inf, -100.0, 100.0, math.inf, math.nan], dtype=dt, device="cuda")
+    got = ops.linear(one, far[:, None], activation="gelu")[0]
+    assert got[1] == 0 and got[2] == 100 and got[3] == math.inf and torch.isnan(got[4])

@@ -29,12 +29,14 @@ template <typename T> __device__ __forceinline__ float sigmoid_f32(float y)
    return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
+// gelu by the complement: 1 + erf loses every digit of a negative tail (y = -5: a tenth of the value, y = -6: all of it).  What is left is the argument's rounding, y^2 2^-23 relative, and
+// erfc's own.  (1111 x 1000 x 1537 bfloat16 with it: 13.95 us, with 1 + erf 13.75)
 template <typename T> __device__ __forceinline__ float activate(float y, int act)
 {
    switch (act) {
       case kActRelu:    return y < 0.0f ? 0.0f : y;          // NaN stays NaN
       case kActSilu:    return y * sigmoid_f32<T>(y);
-      case kActGelu:    return 0.5f * y * (1.0f + erff(y * 0.70710678118654752f));
+      case kActGelu:    return 0.5f * y * erfcf(y * -0.70710678118654752f);
       case kActSigmoid: return sigmoid_f32<T>(y);
       default:          return y;
    }
