@@ -314,3 +314,27 @@ def test_what_is_no_tensor_is_refused(what):
                  lambda: ops.gated_delta(**delta_args(state=what))):
         with pytest.raises(TypeError, match="tensor"):
             call()
+
+
+def test_what_the_library_refuses_is_a_wrong_argument():
+    """sizes and strides that only the library looks at: a ValueError with its words, as of every wrong argument"""
+    gpu = torch.device("cuda", 0)
+
+    def layout(*shape, dtype=torch.float32):
+        stride, n = [], 1
+        for d in reversed(shape):
+            stride.insert(0, n)
+            n *= d
+        return (torch.Size(shape), tuple(stride), dtype, gpu)
+
+    with pytest.raises(ValueError, match="group_norm: more than 2\\^20 channels"):
+        ops._plan_norm(layout(3, 2 ** 21), 2, None, None, 1e-5, "none", None, None, None)
+    steps = 2 ** 27
+    with pytest.raises(ValueError, match="gated_delta: more than 2\\^26 steps"):
+        ops._plan_delta(layout(1, steps, 1, 4), layout(1, steps, 1, 4), layout(1, steps, 2, 5), layout(1, steps, 2), layout(1, steps, 2), layout(1, 2, 4, 5), None, False, None, None)
+    L = _lib.load()
+    with pytest.raises(ValueError, match="linear"):
+        ops._check(L.vadc_amd_linear(pack("linear", _7=2 ** 25, _11=2 ** 25), None))
+    if not torch.cuda.is_available():
+        with pytest.raises(VadcAmdError, match="no CPU fallback"):
+            ops._check(L.vadc_amd_linear(pack("linear"), None))

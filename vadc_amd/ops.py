@@ -68,9 +68,13 @@ def _layouts(*ls):
     return [None if v is None else _Layout(*v) for v in ls]
 
 
+_EINVAL = -1                 # of include/vadc_amd.h
+
+
 def _check(rc: int) -> int:
     if rc < 0:
-        raise VadcAmdError(rc, _lib.load().vadc_amd_last_error().decode())
+        said = _lib.load().vadc_amd_last_error().decode()
+        raise ValueError(said) if rc == _EINVAL else VadcAmdError(rc, said)
     return rc
 
 
