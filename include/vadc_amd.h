@@ -317,8 +317,11 @@ const char *vadc_amd_kernel_name(int kernel);
  *   - a call enqueues kernels on `hip_stream` (a hipStream_t; NULL = HIP's default stream) of device `device` (< 0: the current one) and returns: no allocation, no host
  *     synchronisation, nothing kept for the next call.  It may be issued while the stream is being captured.  The calling thread's current device is the same afterwards.
  *   - strides count ELEMENTS; the innermost dimension of every tensor is contiguous.  Tensors need their element's alignment, no more (16-byte aligned ones run faster).
- *   - x, weights and outputs are of ONE type (`dtype`); sums, statistics and states are float32; an output is rounded once, to nearest even.
- *   - an output must not overlap another operand, but for the exceptions named; entries of an output must be distinct (no stride 0).
+ *   - x, weights and outputs are of ONE type (`dtype`); sums, statistics and states are float32; an output is rounded once, to nearest even.  linear of many rows and gated_delta of many
+ *     steps take float32 factors as sums of three bfloat16 values: float32 accuracy for factors of 2^-109 and more; of a smaller one up to 2^-134 may be left out.
+ *   - activations: relu exact; sigmoid and silu good to three float32 steps up to |y| = 80 where the output is float32, to |y| 2^-24 relative where it has 16 bits; gelu to y^2 2^-23.
+ *   - what a call writes (an output, a state) must not overlap another operand, but for the exceptions named (lying beside one in the same rows is no overlap); entries of an output must be
+ *     distinct (no stride 0).
  *   - a call with a dimension of zero that leaves nothing to write returns VADC_AMD_OK and touches nothing.
  *   - forward only: the operators have no gradients.
  * VADC_AMD_EINVAL: an argument out of range (checked before the device is touched); VADC_AMD_ENODEVICE: no gfx950 device; VADC_AMD_EHIP: the launch failed. */
@@ -361,7 +364,8 @@ int  vadc_amd_group_norm(const vadc_amd_group_norm_args *args, void *hip_stream)
  * (each stream's part contiguous).  heads is a multiple of key_heads: head h reads key head h / (heads / key_heads).  1 <= key_dim <= 256.  normalize: q and k are divided by
  * sqrt(sum of squares + 1e-6) first.  log_decay <= 0 (-inf: the state is forgotten); keys of length one at most keep the recurrence stable, as its definition needs.
  * lengths [streams] (int32, on the device; NULL = none): stream b has its first lengths[b] steps only (clamped to 0 ... steps); the rest of its inputs is not read, the rest of its
- * output not written; a stream of no steps keeps its state.  A value that is not finite makes NaN of what it reaches, from its step on: its column of its head's state and outputs (a key or
+ * output not written; a stream of no steps keeps its state.  Many steps go in blocks of 64 where 8 <= key_dim <= 128 and value_dim >= 4, else one by one (1.4 us a step and more: a long
+ * call with longer keys takes as many microseconds as it has steps).  A value that is not finite makes NaN of what it reaches, from its step on: its column of its head's state and outputs (a key or
  * gate: every column, a query: its own outputs); nothing before it, beside it or in another head.  workspace: as above. */
 typedef struct vadc_amd_gated_delta_args {
    const void *q, *k, *v;

@@ -653,19 +653,20 @@ __global__ __launch_bounds__(16 * COLS) void k_delta_scan(const vadc_amd_gated_d
 }
 
 // ---- choice ---------------------------------------------------------------------------------------------------------------------------------------------
-// Blocks for keys of 8 to 128 and values of 4 and more, from as many steps on as they are the faster form.  One by one a step takes 0.9 us and, with many states, more; blocks take two
-// launches and whole blocks of work: 1 stream, 16 heads of 128, bfloat16: 16 us up to 64 steps, against 12 for 8 steps and 16 for 12; 256 streams, 4 heads of 64: 56 us, against 35 for 16
-// steps and 49 for 24; 8 heads of 128: 240 us against 138 for 16 and 195 for 24.
+// Blocks for keys of 8 to 128 and values of 4 and more, from as many steps on as they are the faster form.  One by one a step takes 1.1 us and, with many states, more; blocks take two
+// launches and whole blocks of work: 1 stream, 16 heads of 128, bfloat16: 17 us up to 64 steps, against 13.5 for 8 steps, 18 for 12 and 76 for 64; 256 streams, 4 heads of 64: 56 us, against
+// 38 for 16 steps, 51 for 24 and 58 for 28; 8 heads of 128: 250 us against 139 for 16, 199 for 24, 230 for 28 and 505 for 64.  Longer keys go one by one however many steps there are (1 stream,
+// 8 heads of 256 x 128: 1.4 us a step; of 128 x 128 in blocks: 0.06).
 static bool in_blocks(const vadc_amd_gated_delta_args &a)
 {
    return a.steps >= (a.streams * a.heads <= 256 ? 12 : 28) && a.key_dim >= 8 && a.key_dim <= 128 && a.value_dim >= 4;
 }
 // Columns of S per workgroup: with keys of up to 64, 16 -- several workgroups a CU, one computes while another waits at its barriers (61 streams of up to 333 steps, 6 heads of 48 x 80,
-// float32: 89 us a call against 100 with 32) --; with longer keys, where staging k and q again for every 16 columns costs more than that gains, 32 (2 x 8192 steps, 32 heads of 128 x 128,
-// bfloat16: 507 us against 543 with 16)
+// float32: 88 us a call against 103 with 32) --; with longer keys, where staging k and q again for every 16 columns costs more than that gains, 32 (2 x 8192 steps, 32 heads of 128 x 128,
+// bfloat16: 540 us against 585 with 16)
 template <int KD> constexpr int scan_columns() { return KD == 64 ? 16 : 32; }
-// The workspace holds 4096 blocks of 37 KB, which stay in the last-level cache between the two launches; longer calls go out in segments of steps (2 x 8192 steps, 32 heads: 507 us so,
-// 523 with 2048, 502 with 8192)
+// The workspace holds 4096 blocks of 37 KB, which stay in the last-level cache between the two launches; longer calls go out in segments of steps (2 x 8192 steps, 32 heads: 540 us so,
+// 560 with 2048, 535 with 8192)
 static int64_t segment_blocks(const vadc_amd_gated_delta_args &a)
 {
    const int64_t blocks = (a.steps + kBlock - 1) / kBlock, most = std::max<int64_t>(1, 4096 / (a.streams * a.heads));

@@ -392,10 +392,10 @@ def gated_delta(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor
     """The gated delta rule.  Per stream and head, for each step: S = e^log_decay S; u = beta (v - S^T k); S = S + k u^T; out = scale S^T q.
 
     q, k [streams, steps, key_heads, key_dim], v [streams, steps, heads, value_dim], log_decay, beta [streams, steps, heads] (float32), state [streams, heads, key_dim, value_dim]
-    (float32), which is UPDATED in place; returns [streams, steps, heads, value_dim].  heads is a multiple of key_heads (consecutive heads share a key head); key_dim is 256 at most.
+    (float32), which is UPDATED in place and overlaps no input; returns [streams, steps, heads, value_dim].  heads is a multiple of key_heads (consecutive heads share a key head); key_dim is 256 at most.
     scale: 1 / sqrt(key_dim) by default.  normalize: q and k are brought to unit length (x / sqrt(sum x^2 + 1e-6)).  lengths [streams] (int32): stream b has its first lengths[b] steps
-    only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given); a stream of no steps keeps its state.  A value that is not finite makes NaN of
-    what it reaches: its column of the state and of the outputs from its step on (a key or gate: every column of its head; a query: its own outputs)."""
+    only; what lies behind them is not read, and stays as it is in `out` (zero, where no `out` is given); a stream of no steps keeps its state.  Many steps go in blocks where key_dim is 8 to
+    128, one by one with longer keys.  A value that is not finite, an infinity as well, makes NaN of what it reaches: its column of the state and of the outputs from its step on (a key or gate: every column of its head; a query: its own outputs)."""
     plan = _plan_delta(_layout(q), _layout(k), _layout(v), _layout(log_decay), _layout(beta), _layout(state), scale, normalize, _layout(lengths), _layout(out))
     if torch.is_grad_enabled():
         _no_grad("gated_delta", q, k, v, log_decay, beta, state, out)
