@@ -916,7 +916,7 @@ static int ensure_pipeline_streams(vadc_amd_engine *e, int n_streams, int lk)
    bool masked = false;
    if (want > 0) {
       const int words = (e->n_cus + 31) / 32;
-      // a mask that leaves an XCD without a CU is refused by some drivers (hipErrorOutOfMemory: bits go to the 8 XCDs in turn, so a half needs 8): the layers then share the partition
+      // a mask that leaves an XCD without a CU is refused by ROCm 7.2 (hipErrorOutOfMemory: bits go to the 8 XCDs in turn, so a half needs 8): the layers then share the partition
       const bool halves = split && want / 2 >= 8;
       const int wb = halves ? want / 2 : want;
       std::vector<uint32_t> mb(words, 0u), mc(words, 0u), ma(words, 0u);
