@@ -338,10 +338,3 @@ def test_what_the_library_refuses_is_a_wrong_argument():
     if not torch.cuda.is_available():
         with pytest.raises(VadcAmdError, match="no CPU fallback"):
             ops._check(L.vadc_amd_linear(pack("linear"), None))
-
-
-def test_an_empty_operand_overlaps_nothing():
-    out = t(4, 8)
-    x = out[:, 3:3]                                                  # no features, inside the output's memory
-    assert not ops._shares(out, x) and not ops._shares(x, out)
-    ops._apart("linear", (0, 4 * 8 * 4), out, (("x", x),))

@@ -206,7 +206,7 @@ def _meet(by: int, run_a: int, a: list, run_b: int, b: list) -> bool:
 
 
 def _shares(x: Tensor, y: Tensor) -> bool:
-    return 0 not in x.shape and 0 not in y.shape and _meet(y.data_ptr() - x.data_ptr(), *_pieces(x.shape, x.stride(), x.element_size()), *_pieces(y.shape, y.stride(), y.element_size()))
+    return _meet(y.data_ptr() - x.data_ptr(), *_pieces(x.shape, x.stride(), x.element_size()), *_pieces(y.shape, y.stride(), y.element_size()))
 
 
 def _apart(what: str, spans: tuple, out: Tensor, ts: tuple, same: tuple = (), written: str = "out"):
